@@ -75,6 +75,9 @@ def build(force: bool = False, jobs: int = 8, verbose: bool = False) -> str:
     ]
     common = [
         f'--offload-arch={ARCH}',
+        # no packed fp32 instructions (v_pk_add / mul / fma_f32): some of their
+        # forms have returned wrong results on this card now and then
+        '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops',
         '-O3',
         '-fPIC',
         '-std=c++17',
