@@ -1634,8 +1634,12 @@ void trinv_upper_(at::Tensor& t) {
                             work.data_ptr<float>(), cur_stream());
 }
 
+// lm_ops.cpp
+void bind_lm_ops(pybind11::module& m);
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "MI355X (gfx950) HIP kernels for distributed K-FAC";
+  bind_lm_ops(m);
   m.def("triu_pack", &triu_pack);
   m.def("triu_unpack", &triu_unpack);
   m.def("scale_copy", &scale_copy);

@@ -1,0 +1,464 @@
+// Torch side of the decoder operators: window attention with sinks, rotary
+// positions with several axes, distillation from a teacher's top logits
+// (kernels in window_attn.hip, rotary.hip, distill.hip).  Argument checks of
+// the public functions are in ops/attention.py, ops/rotary.py and
+// ops/distill.py; the checks here are those that keep a kernel in bounds.
+// Each operator is a C++ autograd node, so that neither its forward nor its
+// backward runs Python.
+#include <torch/extension.h>
+#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+
+#include <tuple>
+#include <vector>
+
+#include "common.h"
+#include "lm_ops.h"
+
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using OptTensor = c10::optional<at::Tensor>;
+
+hipStream_t stream() { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream(); }
+
+int tag(const at::Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return kfac::kF32;
+    case at::kBFloat16: return kfac::kBF16;
+    case at::kHalf: return kfac::kF16;
+    default: TORCH_CHECK(false, "kfac native: unsupported dtype ", t.scalar_type());
+  }
+  return -1;
+}
+
+bool aligned16(const at::Tensor& t) {
+  return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
+}
+
+// rows that 16-byte accesses can read: unit last stride, every other stride
+// of a dimension with more than one element a multiple of 16 bytes
+bool rows16(const at::Tensor& t) {
+  const int64_t unit = 16 / (int64_t)t.element_size();
+  const int64_t n = t.dim();
+  if (!aligned16(t) || (t.stride(n - 1) != 1 && t.size(n - 1) > 1)) return false;
+  for (int64_t i = 0; i + 1 < n; ++i)
+    if (t.size(i) > 1 && t.stride(i) % unit != 0) return false;
+  return true;
+}
+
+// t, or a copy whose rows can be read in 16-byte accesses
+at::Tensor readable(const at::Tensor& t) {
+  return rows16(t) ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+void strides3(const at::Tensor& t, int64_t* s) {  // batch, head, token of [B, H, T, D]
+  s[0] = t.stride(0);
+  s[1] = t.stride(1);
+  s[2] = t.stride(2);
+}
+
+void once_only(const char* op) {
+  // the backward pass is made of kernels: nothing records it for a second one
+  TORCH_CHECK(!at::GradMode::is_enabled(), op, ": gradients of gradients are not supported");
+}
+
+bool records(std::initializer_list<const at::Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const auto* t : ts)
+    if (t->requires_grad()) return true;
+  return false;
+}
+
+void on_device(const at::Tensor& t, const at::Tensor& like, const char* what) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), "kfac native: ", what,
+              " must be on the operands' GPU");
+}
+
+// ----------------------------------------------------------- attention
+struct AttnConf {
+  int64_t window, sinks, start;
+  bool start_given;
+  double scale;
+};
+
+kfac::AttnArgs attn_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                         const OptTensor& lengths, const OptTensor& starts, const AttnConf& c) {
+  TORCH_CHECK(q.is_cuda() && q.dim() == 4 && k.dim() == 4 && v.sizes() == k.sizes(),
+              "window_attention: q, k, v must be 4-D GPU tensors, v like k");
+  on_device(k, q, "k");
+  on_device(v, q, "v");
+  TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(),
+              "window_attention: q, k, v must share a dtype");
+  kfac::AttnArgs a{};
+  TORCH_CHECK(k.size(0) == q.size(0) && k.size(3) == q.size(3) && k.size(1) > 0 &&
+                  q.size(1) % k.size(1) == 0,
+              "window_attention: shapes of q and k do not fit");
+  TORCH_CHECK(q.size(3) % 8 == 0 && q.size(3) >= 8 && q.size(3) <= 128,
+              "window_attention: head size must be a multiple of 8, at most 128");
+  const int64_t lim = (int64_t)1 << 30;
+  TORCH_CHECK(q.size(2) < lim && k.size(2) < lim && q.size(0) * q.size(1) < lim,
+              "window_attention: too large");
+  a.B = (int)q.size(0);
+  a.Hq = (int)q.size(1);
+  a.Tq = (int)q.size(2);
+  a.D = (int)q.size(3);
+  a.Hkv = (int)k.size(1);
+  a.Tk = (int)k.size(2);
+  a.G = a.Hq / a.Hkv;
+  TORCH_CHECK(((int64_t)a.Tq * a.G + 127) / 128 <= 65535,
+              "window_attention: more than 65535 row blocks");
+  TORCH_CHECK(c.window >= 1 && c.sinks >= 0, "window_attention: window >= 1, sinks >= 0");
+  a.W = (int)std::min<int64_t>(c.window, std::max<int64_t>(a.Tk, 1));
+  a.S = (int)std::min<int64_t>(c.sinks, a.Tk);
+  for (const auto* o : {&lengths, &starts})
+    if (o->has_value()) {
+      on_device(**o, q, "lengths / q_start");
+      TORCH_CHECK((*o)->scalar_type() == at::kInt && (*o)->is_contiguous() &&
+                      (*o)->numel() == a.B,
+                  "window_attention: lengths and q_start must be contiguous int32 [B]");
+    }
+  a.lengths = lengths.has_value() ? lengths->data_ptr<int>() : nullptr;
+  a.starts = starts.has_value() ? starts->data_ptr<int>() : nullptr;
+  a.start = (int)std::max<int64_t>(std::min<int64_t>(c.start, lim), -lim);
+  a.start_given = c.start_given;
+  a.scale = (float)c.scale;
+  a.q = q.data_ptr();
+  a.k = k.data_ptr();
+  a.v = v.data_ptr();
+  strides3(q, a.qs);
+  strides3(k, a.ks);
+  strides3(v, a.vs);
+  a.splits = 1;
+  return a;
+}
+
+// out [B, Hq, Tq, D] over memory laid out [B, Tq, Hq, D] (what the output
+// projection reads), and lse [B, Hq, Tq] where a backward pass may follow
+std::tuple<at::Tensor, at::Tensor> attn_forward(const at::Tensor& q, const at::Tensor& k,
+                                                const at::Tensor& v, const OptTensor& lengths,
+                                                const OptTensor& starts, const AttnConf& c,
+                                                bool want_lse) {
+  c10::hip::HIPGuardMasqueradingAsCUDA g(q.device());
+  kfac::AttnArgs a = attn_args(q, k, v, lengths, starts, c);
+  at::Tensor out = at::empty({a.B, a.Tq, a.Hq, a.D}, q.options()).transpose(1, 2);
+  at::Tensor lse;
+  if (want_lse) lse = at::empty({a.B, a.Hq, a.Tq}, q.options().dtype(at::kFloat));
+  a.out = out.data_ptr();
+  strides3(out, a.os);
+  a.lse = want_lse ? lse.data_ptr<float>() : nullptr;
+  int64_t floats = 0;
+  kfac::attn_plan(a, tag(q), &a.splits, &floats);
+  at::Tensor ws;
+  if (floats > 0) {
+    ws = at::empty({floats}, q.options().dtype(at::kFloat));
+    const int64_t rows = (int64_t)a.splits * a.B * a.Hkv * a.Tq * a.G;
+    a.opart = ws.data_ptr<float>();
+    a.lpart = a.opart + rows * a.D;
+  }
+  kfac::attn_forward(tag(q), a, stream());
+  C10_HIP_KERNEL_LAUNCH_CHECK();
+  return {out, lse};
+}
+
+struct WindowAttnFn : public torch::autograd::Function<WindowAttnFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& q_, const at::Tensor& k_,
+                            const at::Tensor& v_, const OptTensor& lengths,
+                            const OptTensor& starts, int64_t window, int64_t sinks, int64_t start,
+                            bool start_given, double scale) {
+    const AttnConf c{window, sinks, start, start_given, scale};
+    const at::Tensor q = readable(q_), k = readable(k_), v = readable(v_);
+    auto [out, lse] = attn_forward(q, k, v, lengths, starts, c, true);
+    ctx->save_for_backward({q, k, v, out, lse, lengths.has_value() ? *lengths : at::Tensor(),
+                            starts.has_value() ? *starts : at::Tensor()});
+    ctx->saved_data["window"] = window;
+    ctx->saved_data["sinks"] = sinks;
+    ctx->saved_data["start"] = start;
+    ctx->saved_data["start_given"] = start_given;
+    ctx->saved_data["scale"] = scale;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once_only("window_attention");
+    auto sv = ctx->get_saved_variables();
+    const at::Tensor &q = sv[0], &k = sv[1], &v = sv[2], &out = sv[3], &lse = sv[4];
+    const AttnConf c{ctx->saved_data["window"].toInt(), ctx->saved_data["sinks"].toInt(),
+                     ctx->saved_data["start"].toInt(), ctx->saved_data["start_given"].toBool(),
+                     ctx->saved_data["scale"].toDouble()};
+    const OptTensor lengths = sv[5].defined() ? OptTensor(sv[5]) : c10::nullopt;
+    const OptTensor starts = sv[6].defined() ? OptTensor(sv[6]) : c10::nullopt;
+    c10::hip::HIPGuardMasqueradingAsCUDA g(q.device());
+    kfac::AttnArgs a = attn_args(q, k, v, lengths, starts, c);
+    const at::Tensor go = readable(grads[0]);
+    at::Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v);
+    if (a.Tq == 0 || q.numel() == 0) {
+      dk.zero_();
+      dv.zero_();
+    } else {
+      at::Tensor delta = at::empty_like(lse);
+      a.out = out.data_ptr();
+      strides3(out, a.os);
+      a.dout = go.data_ptr();
+      strides3(go, a.dos);
+      a.lse = lse.data_ptr<float>();
+      a.delta = delta.data_ptr<float>();
+      a.dq = dq.data_ptr();
+      a.dk = dk.data_ptr();
+      a.dv = dv.data_ptr();
+      strides3(dq, a.dqs);
+      strides3(dk, a.dks);
+      strides3(dv, a.dvs);
+      int64_t floats = 0;
+      kfac::attn_bwd_plan(a, tag(q), &a.sink_blocks, &a.far_chunks, &floats);
+      TORCH_CHECK((int64_t)(a.Tk + 127) / 128 + (int64_t)a.sink_blocks * a.far_chunks <= 65535,
+                  "window_attention: more than 65535 key blocks");
+      at::Tensor ws;
+      if (floats > 0) {
+        ws = at::empty({floats}, lse.options());
+        a.kvpart = ws.data_ptr<float>();
+      }
+      if (a.Tk == 0) dq.zero_();
+      kfac::attn_backward(tag(q), a, stream());
+      C10_HIP_KERNEL_LAUNCH_CHECK();
+    }
+    at::Tensor u;
+    return {dq, dk, dv, u, u, u, u, u, u, u};
+  }
+};
+
+at::Tensor window_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                            const OptTensor& lengths, const OptTensor& starts, int64_t window,
+                            int64_t sinks, int64_t start, bool start_given, double scale) {
+  if (records({&q, &k, &v}))
+    return WindowAttnFn::apply(q, k, v, lengths, starts, window, sinks, start, start_given, scale);
+  const AttnConf c{window, sinks, start, start_given, scale};
+  return std::get<0>(
+      attn_forward(readable(q), readable(k), readable(v), lengths, starts, c, false));
+}
+
+// -------------------------------------------------------------- rotary
+struct RotaryConf {
+  std::vector<double> turn;    // of each pair
+  std::vector<int64_t> axis;
+  bool halves;
+};
+
+// both operands turned by the positions' angles (sign -1: turned back)
+std::tuple<at::Tensor, at::Tensor> rotary_run(const at::Tensor& q, const at::Tensor& k,
+                                              const at::Tensor& pos, const RotaryConf& c,
+                                              double sign) {
+  TORCH_CHECK(q.is_cuda() && q.dim() == 4 && k.dim() == 4 && q.scalar_type() == k.scalar_type() &&
+                  q.size(0) == k.size(0) && q.size(2) == k.size(2) && q.size(3) == k.size(3),
+              "rotary_axes: q and k must be 4-D GPU tensors of one dtype that differ in heads only");
+  on_device(k, q, "k");
+  on_device(pos, q, "positions");
+  const int64_t B = q.size(0), T = q.size(2), D = q.size(3);
+  const int64_t pairs = (int64_t)c.turn.size();
+  TORCH_CHECK(pairs >= 1 && pairs <= kfac::kMaxRotaryPairs && 2 * pairs <= D && D % 2 == 0 &&
+                  c.axis.size() == c.turn.size(),
+              "rotary_axes: pairs do not fit the head");
+  TORCH_CHECK((pos.scalar_type() == at::kLong || pos.scalar_type() == at::kInt) &&
+                  (pos.dim() == 2 || (pos.dim() == 3 && pos.size(0) == B)) &&
+                  pos.size(-2) == T,
+              "rotary_axes: positions must be int32 / int64 [T, axes] or [B, T, axes]");
+  TORCH_CHECK(B * T < (1LL << 31) && B < (1LL << 30) && q.size(1) + k.size(1) < (1LL << 30),
+              "rotary_axes: too large");
+  c10::hip::HIPGuardMasqueradingAsCUDA g(q.device());
+  kfac::RotaryArgs a{};
+  for (int64_t i = 0; i < pairs; ++i) {
+    TORCH_CHECK(c.axis[i] >= 0 && c.axis[i] < pos.size(-1), "rotary_axes: axis of a pair");
+    a.tab.turn[i] = c.turn[i];
+    a.tab.axis[i] = (uint8_t)c.axis[i];
+  }
+  at::Tensor qo = at::empty({B, q.size(1), T, D}, q.options());
+  at::Tensor ko = at::empty({B, k.size(1), T, D}, k.options());
+  a.q = q.data_ptr();
+  a.k = k.data_ptr();
+  a.qo = qo.data_ptr();
+  a.ko = ko.data_ptr();
+  strides3(q, a.qs);
+  strides3(k, a.ks);
+  a.pos = pos.data_ptr();
+  a.pos64 = pos.scalar_type() == at::kLong;
+  a.psB = pos.dim() == 3 ? pos.stride(0) : 0;
+  a.psT = pos.stride(-2);
+  a.psA = pos.stride(-1);
+  a.B = (int)B;
+  a.T = (int)T;
+  a.D = (int)D;
+  a.Hq = (int)q.size(1);
+  a.Hk = (int)k.size(1);
+  a.pairs = (int)pairs;
+  a.sign = (float)sign;
+  const int64_t unit = 16 / (int64_t)q.element_size();
+  const bool vec = rows16(q) && rows16(k) && D % unit == 0 &&
+                   (!c.halves || (pairs % unit == 0 && (D - 2 * pairs) % unit == 0));
+  kfac::rotary_axes(tag(q), a, c.halves, vec, stream());
+  C10_HIP_KERNEL_LAUNCH_CHECK();
+  return {qo, ko};
+}
+
+at::Tensor unit_last(const at::Tensor& t) {
+  return t.stride(-1) == 1 || t.size(-1) <= 1 ? t : t.contiguous();
+}
+
+struct RotaryFn : public torch::autograd::Function<RotaryFn> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k,
+                               const at::Tensor& pos, const std::vector<double>& turn,
+                               const std::vector<int64_t>& axis, bool halves) {
+    const RotaryConf c{turn, axis, halves};
+    auto [qo, ko] = rotary_run(unit_last(q), unit_last(k), pos, c, 1.0);
+    ctx->save_for_backward({pos});
+    ctx->saved_data["turn"] = turn;
+    ctx->saved_data["axis"] = axis;
+    ctx->saved_data["halves"] = halves;
+    return {qo, ko};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once_only("rotary_axes");
+    const RotaryConf c{ctx->saved_data["turn"].toDoubleVector(),
+                       ctx->saved_data["axis"].toIntVector(), ctx->saved_data["halves"].toBool()};
+    auto [dq, dk] = rotary_run(unit_last(grads[0]), unit_last(grads[1]),
+                               ctx->get_saved_variables()[0], c, -1.0);
+    at::Tensor u;
+    return {dq, dk, u, u, u, u};
+  }
+};
+
+std::tuple<at::Tensor, at::Tensor> rotary_axes(const at::Tensor& q, const at::Tensor& k,
+                                               const at::Tensor& pos,
+                                               const std::vector<double>& turn,
+                                               const std::vector<int64_t>& axis, bool halves) {
+  if (records({&q, &k})) {
+    auto r = RotaryFn::apply(q, k, pos, turn, axis, halves);
+    return {r[0], r[1]};
+  }
+  return rotary_run(unit_last(q), unit_last(k), pos, RotaryConf{turn, axis, halves}, 1.0);
+}
+
+// ------------------------------------------------------------- distill
+kfac::DistillArgs distill_args(const at::Tensor& z, const at::Tensor& teacher,
+                               const at::Tensor& index, const OptTensor& rest,
+                               double temperature) {
+  TORCH_CHECK(z.is_cuda() && z.dim() == 3 && (z.stride(2) == 1 || z.size(2) == 1),
+              "topk_distill_loss: logits must be a GPU tensor [.., .., V] with unit last stride");
+  on_device(teacher, z, "teacher_logits");
+  on_device(index, z, "teacher_index");
+  kfac::DistillArgs a{};
+  a.N = z.size(0) * z.size(1);
+  a.V = z.size(2);
+  a.inner = std::max<int64_t>(z.size(1), 1);
+  a.zs0 = z.stride(0);
+  a.zs1 = z.stride(1);
+  TORCH_CHECK(teacher.scalar_type() == at::kFloat && teacher.is_contiguous() &&
+                  index.is_contiguous() && index.numel() == teacher.numel() &&
+                  (index.scalar_type() == at::kInt || index.scalar_type() == at::kLong),
+              "topk_distill_loss: teacher entries must be contiguous fp32 / int32 or int64");
+  TORCH_CHECK(a.V >= 1 && teacher.dim() >= 1, "topk_distill_loss: no columns");
+  a.K = (int)teacher.size(-1);
+  TORCH_CHECK(teacher.size(-1) >= 1 && teacher.size(-1) <= 1024 &&
+                  teacher.numel() == a.N * a.K,
+              "topk_distill_loss: 1 to 1024 teacher entries for each row");
+  if (rest.has_value()) {
+    on_device(*rest, z, "teacher_rest");
+    TORCH_CHECK(rest->scalar_type() == at::kFloat && rest->is_contiguous() &&
+                    rest->numel() == a.N,
+                "topk_distill_loss: teacher_rest must be contiguous fp32, one a row");
+    a.rest = rest->data_ptr<float>();
+  }
+  a.z = z.data_ptr();
+  a.teacher = teacher.data_ptr<float>();
+  a.index = index.data_ptr();
+  a.index64 = index.scalar_type() == at::kLong;
+  a.temperature = (float)temperature;
+  a.aligned = rows16(z);
+  kfac::distill_split(a.N, a.V, rest.has_value(), &a.slice, &a.splits);
+  TORCH_CHECK(a.N * a.splits < (1LL << 31), "topk_distill_loss: too many rows");
+  return a;
+}
+
+struct DistillOut {
+  at::Tensor loss, info, mean;
+};
+
+// reduction: 0 none, 1 sum, 2 mean
+DistillOut distill_run(const at::Tensor& z, const at::Tensor& teacher, const at::Tensor& index,
+                       const OptTensor& rest, double temperature, int64_t reduction) {
+  c10::hip::HIPGuardMasqueradingAsCUDA g(z.device());
+  kfac::DistillArgs a = distill_args(z, teacher, index, rest, temperature);
+  const auto f32 = z.options().dtype(at::kFloat);
+  DistillOut o;
+  o.info = at::empty({a.N, 4}, f32);
+  at::Tensor rows = at::empty({a.N}, f32);
+  at::Tensor part;
+  if (a.splits > 1) part = at::empty({a.N * a.splits, 4}, f32);
+  a.info = reinterpret_cast<float4*>(o.info.data_ptr<float>());
+  a.row_loss = rows.data_ptr<float>();
+  a.part = a.splits > 1 ? reinterpret_cast<float4*>(part.data_ptr<float>()) : nullptr;
+  o.loss = rows;
+  if (reduction != 0) {
+    o.loss = at::empty({}, f32);
+    o.mean = at::empty({1}, f32);
+  }
+  kfac::distill_forward(tag(z), a, reduction != 0 ? o.loss.data_ptr<float>() : nullptr,
+                        reduction != 0 ? o.mean.data_ptr<float>() : nullptr, (int)reduction,
+                        stream());
+  C10_HIP_KERNEL_LAUNCH_CHECK();
+  return o;
+}
+
+struct DistillFn : public torch::autograd::Function<DistillFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& z, const at::Tensor& teacher,
+                            const at::Tensor& index, const OptTensor& rest, double temperature,
+                            int64_t reduction) {
+    auto o = distill_run(z, teacher, index, rest, temperature, reduction);
+    ctx->save_for_backward({z, teacher, index, rest.has_value() ? *rest : at::Tensor(), o.info,
+                            o.mean});
+    ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["reduction"] = reduction;
+    return o.loss;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once_only("topk_distill_loss");
+    auto sv = ctx->get_saved_variables();
+    const at::Tensor& z = sv[0];
+    const OptTensor rest = sv[3].defined() ? OptTensor(sv[3]) : c10::nullopt;
+    c10::hip::HIPGuardMasqueradingAsCUDA g(z.device());
+    kfac::DistillArgs a =
+        distill_args(z, sv[1], sv[2], rest, ctx->saved_data["temperature"].toDouble());
+    const bool rows = ctx->saved_data["reduction"].toInt() == 0;
+    const at::Tensor up = grads[0].to(at::kFloat).contiguous();
+    at::Tensor dz = at::empty(z.sizes(), z.options());
+    a.info = reinterpret_cast<float4*>(sv[4].data_ptr<float>());
+    a.upstream = up.data_ptr<float>();
+    a.upstream_rows = rows;
+    a.mean = rows ? nullptr : sv[5].data_ptr<float>();
+    a.dz = dz.data_ptr();
+    a.dz_aligned = rows16(dz);
+    kfac::distill_backward(tag(z), a, stream());
+    C10_HIP_KERNEL_LAUNCH_CHECK();
+    at::Tensor u;
+    return {dz, u, u, u, u, u};
+  }
+};
+
+at::Tensor topk_distill_loss(const at::Tensor& z, const at::Tensor& teacher,
+                             const at::Tensor& index, const OptTensor& rest, double temperature,
+                             int64_t reduction) {
+  if (records({&z})) return DistillFn::apply(z, teacher, index, rest, temperature, reduction);
+  return distill_run(z, teacher, index, rest, temperature, reduction).loss;
+}
+
+}  // namespace
+
+void bind_lm_ops(pybind11::module& m) {
+  namespace py = pybind11;
+  m.def("window_attention", &window_attention, py::arg("q"), py::arg("k"), py::arg("v"),
+        py::arg("lengths"), py::arg("starts"), py::arg("window"), py::arg("sinks"),
+        py::arg("start"), py::arg("start_given"), py::arg("scale"));
+  m.def("rotary_axes", &rotary_axes, py::arg("q"), py::arg("k"), py::arg("positions"),
+        py::arg("turn"), py::arg("axis"), py::arg("halves"));
+  m.def("topk_distill_loss", &topk_distill_loss, py::arg("logits"), py::arg("teacher"),
+        py::arg("index"), py::arg("rest"), py::arg("temperature"), py::arg("reduction"));
+}

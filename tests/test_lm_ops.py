@@ -1,0 +1,220 @@
+"""Decoder operators on the CPU: what they refuse, the torch formulas against
+64 bits and against differences."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from distributed_kfac_pytorch_amd.ops.attention import window_attention
+from distributed_kfac_pytorch_amd.ops.distill import topk_distill_loss
+from distributed_kfac_pytorch_amd.ops.rotary import rotary_axes
+from tests import lm_reference as ref
+
+
+def rand(*shape, seed=0, dtype=torch.float32):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+# ------------------------------------------------------------- refusals
+def _qkv(b=1, hq=2, hk=1, t=4, d=8, dtype=torch.float32):
+    return rand(b, hq, t, d, dtype=dtype), rand(b, hk, t, d, dtype=dtype), rand(b, hk, t, d, dtype=dtype)
+
+
+@pytest.mark.parametrize('change, error', [
+    (dict(window=0), ValueError),
+    (dict(sinks=-1), ValueError),
+    (dict(scale=0.0), ValueError),
+    (dict(scale=float('nan')), ValueError),
+    (dict(lengths=torch.tensor([4])), ValueError),                       # int64
+    (dict(lengths=torch.tensor([4, 4], dtype=torch.int32)), ValueError),  # two sequences
+    (dict(q_start=torch.tensor([0.0])), ValueError),
+])
+def test_attention_refuses_options(change, error):
+    q, k, v = _qkv()
+    with pytest.raises(error):
+        window_attention(q, k, v, **{'window': 2, **change})
+
+
+@pytest.mark.parametrize('shapes, error', [
+    (((1, 2, 4, 8), (1, 1, 4, 8), (1, 1, 5, 8)), ValueError),     # v unlike k
+    (((1, 3, 4, 8), (1, 2, 4, 8), (1, 2, 4, 8)), ValueError),     # heads do not divide
+    (((2, 2, 4, 8), (1, 1, 4, 8), (1, 1, 4, 8)), ValueError),     # batch
+    (((1, 2, 4, 12), (1, 1, 4, 12), (1, 1, 4, 12)), ValueError),  # head size
+    (((1, 2, 4, 136), (1, 1, 4, 136), (1, 1, 4, 136)), ValueError),
+    (((1, 2, 4, 8), (1, 0, 4, 8), (1, 0, 4, 8)), ValueError),
+    (((2, 4, 8), (1, 4, 8), (1, 4, 8)), ValueError),
+])
+def test_attention_refuses_shapes(shapes, error):
+    q, k, v = (rand(*s) for s in shapes)
+    with pytest.raises(error):
+        window_attention(q, k, v, window=2)
+
+
+def test_attention_refuses_types():
+    q, k, v = _qkv()
+    with pytest.raises(TypeError):
+        window_attention(q.half(), k, v, window=2)
+    with pytest.raises(TypeError):
+        window_attention(q.int(), k.int(), v.int(), window=2)
+
+
+@pytest.mark.parametrize('change, error', [
+    (dict(sections=()), ValueError),
+    (dict(sections=(0, 2)), ValueError),
+    (dict(sections=(5,)), ValueError),
+    (dict(sections=(2, 2)), ValueError),          # positions have one axis
+    (dict(base=0.0), ValueError),
+    (dict(ladder='none'), ValueError),
+    (dict(layout='none'), ValueError),
+])
+def test_rotary_refuses(change, error):
+    q, k, _ = _qkv()
+    with pytest.raises(error):
+        rotary_axes(q, k, torch.arange(4)[:, None], **{'sections': (4,), **change})
+
+
+def test_rotary_refuses_operands():
+    q, k, _ = _qkv()
+    with pytest.raises(TypeError):
+        rotary_axes(q, k, torch.arange(4.0)[:, None], sections=(4,))
+    with pytest.raises(TypeError):
+        rotary_axes(q, k.half(), torch.arange(4)[:, None], sections=(4,))
+    with pytest.raises(ValueError):
+        rotary_axes(q, k[:, :, :3], torch.arange(4)[:, None], sections=(4,))
+    with pytest.raises(ValueError):
+        rotary_axes(q, k, torch.arange(4), sections=(4,))
+    with pytest.raises(ValueError):
+        rotary_axes(q[..., :7], k[..., :7], torch.arange(4)[:, None], sections=(3,))
+
+
+@pytest.mark.parametrize('change, error', [
+    (dict(temperature=0.0), ValueError),
+    (dict(temperature=float('inf')), ValueError),
+    (dict(reduction='avg'), ValueError),
+    (dict(teacher_rest=torch.zeros(2)), ValueError),
+    (dict(teacher_rest=torch.zeros(3, dtype=torch.int64)), ValueError),
+])
+def test_distill_refuses_options(change, error):
+    with pytest.raises(error):
+        topk_distill_loss(rand(3, 9), rand(3, 2), torch.zeros(3, 2, dtype=torch.int64), **change)
+
+
+@pytest.mark.parametrize('z, t, i, error', [
+    (rand(3, 9), rand(3, 2), torch.zeros(3, 3, dtype=torch.int64), ValueError),
+    (rand(3, 9), rand(2, 2), torch.zeros(2, 2, dtype=torch.int64), ValueError),
+    (rand(3, 9), rand(3, 0), torch.zeros(3, 0, dtype=torch.int64), ValueError),
+    (rand(3, 9), rand(3, 1025), torch.zeros(3, 1025, dtype=torch.int64), ValueError),
+    (rand(3, 9), rand(3, 2), torch.zeros(3, 2), TypeError),
+    (rand(3, 9), torch.zeros(3, 2, dtype=torch.int64), torch.zeros(3, 2, dtype=torch.int64), TypeError),
+    (torch.zeros(3, 9, dtype=torch.int32), rand(3, 2), torch.zeros(3, 2, dtype=torch.int64), TypeError),
+    (rand(3, 0), rand(3, 2), torch.zeros(3, 2, dtype=torch.int64), ValueError),
+])
+def test_distill_refuses_operands(z, t, i, error):
+    with pytest.raises(error):
+        topk_distill_loss(z, t, i)
+
+
+# -------------------------------------------------------- against 64 bits
+@pytest.mark.parametrize('hq, hk, tq, tk, window, sinks, lengths, start', [
+    (2, 2, 7, 7, 3, 0, None, None),
+    (4, 2, 9, 9, 2, 3, None, None),
+    (4, 1, 1, 9, 4, 2, [9, 3, 0], None),
+    (3, 3, 6, 6, 2, 1, [6, 4, 0], 0),
+    (2, 1, 5, 8, 20, 0, [8, 2, 5], None),     # fewer tokens than rows
+    (2, 1, 4, 8, 3, 1, None, -2),
+    (2, 1, 3, 0, 3, 1, None, None),           # no keys
+])
+def test_attention_formula(hq, hk, tq, tk, window, sinks, lengths, start):
+    b = 3
+    q, k, v, do = (rand(b, h, t, 8, seed=s) for s, (h, t) in
+                   enumerate([(hq, tq), (hk, tk), (hk, tk), (hq, tq)]))
+    ln = None if lengths is None else torch.tensor(lengths, dtype=torch.int32)
+    if lengths is not None:
+        for i, n in enumerate(lengths):  # what lies behind a sequence is not read
+            k[i, :, n:] = float('nan')
+            v[i, :, n:] = float('inf')
+    conf = dict(window=window, sinks=sinks, lengths=ln, q_start=start)
+    want, tol = ref.attention(q, k, v, do=do, **conf)
+    x = [t.requires_grad_() for t in (q, k, v)]
+    out = window_attention(*x, **conf)
+    got = [out, *torch.autograd.grad(out, x, do)]
+    for name, g, w, t in zip(('out', 'dq', 'dk', 'dv'), got, want, tol):
+        ref.check(name, g, w, t)
+
+
+def test_attention_differences():
+    q, k, v = (t.double().requires_grad_() for t in _qkv(2, 4, 2, 5))
+    ln = torch.tensor([5, 3], dtype=torch.int32)
+    assert torch.autograd.gradcheck(
+        lambda *a: window_attention(*a, window=2, sinks=1, lengths=ln, q_start=0), (q, k, v))
+
+
+@pytest.mark.parametrize('layout', ['interleaved', 'halves'])
+@pytest.mark.parametrize('ladder', ['shared', 'per_axis'])
+def test_rotary_formula_and_differences(layout, ladder):
+    q, k = rand(2, 3, 5, 18), rand(2, 1, 5, 18, seed=1)
+    pos = torch.randint(-9, 10 ** 6, (2, 5, 3), generator=torch.Generator().manual_seed(3))
+    conf = dict(sections=(3, 1, 4), ladder=ladder, layout=layout, base=500.0)
+    for g, x in zip(rotary_axes(q, k, pos, **conf), (q, k)):
+        ref.check('turned', g, *ref.rotary(x, pos, **conf))
+    assert torch.autograd.gradcheck(lambda a, b: rotary_axes(a, b, pos, **conf),
+                                    (q.double().requires_grad_(), k.double().requires_grad_()))
+
+
+def test_rotary_one_axis_is_the_models_rotation():
+    from distributed_kfac_pytorch_amd.models.gpt_neox import _rotary
+
+    q, k = rand(2, 3, 9, 16), rand(2, 3, 9, 16, seed=1)
+    got = rotary_axes(q, k, torch.arange(9)[:, None], sections=(8,))
+    for g, x in zip(got, (q, k)):
+        torch.testing.assert_close(g, _rotary(x), rtol=0, atol=2e-5)
+
+
+def _distill_case(n=4, v=23, k=5, seed=0, rest=False, tau=1.0, dtype=torch.float32):
+    z = rand(n, v, seed=seed) * 3
+    full = z * 0.5 + rand(n, v, seed=seed + 1) * 2
+    t, i = full.topk(k, dim=-1)
+    r = (full / tau).scatter(-1, i, float('-inf')).logsumexp(-1) if rest else None
+    return z.to(dtype), t, i, r
+
+
+@pytest.mark.parametrize('rest', [False, True])
+@pytest.mark.parametrize('reduction', ['mean', 'sum', 'none'])
+@pytest.mark.parametrize('k, twist', [(1, ''), (5, ''), (5, 'padded'), (5, 'twice'), (23, ''),
+                                      (5, 'all padded')])
+def test_distill_formula(rest, reduction, k, twist):
+    z, t, i, r = _distill_case(k=k, rest=rest, tau=1.5)
+    if twist == 'padded':
+        i[1] = -1
+        i[2, 3:] = -7
+    elif twist == 'all padded':
+        i[:] = -1
+    elif twist == 'twice':
+        i[0, 1] = i[0, 3]
+    up = rand(4, seed=9) if reduction == 'none' else torch.tensor(0.3)
+    z.requires_grad_()
+    loss = topk_distill_loss(z, t, i, teacher_rest=r, temperature=1.5, reduction=reduction)
+    want = ref.distill(z, t, i, rest=r, temperature=1.5, reduction=reduction, upstream=up)
+    ref.check('loss', loss, *want[:2])
+    ref.check('dz', *torch.autograd.grad(loss, z, up), *want[2:])
+
+
+def test_distill_differences_and_dense_limit():
+    z, t, i, r = _distill_case(rest=True)
+    z = z.double()
+    assert torch.autograd.gradcheck(
+        lambda a: topk_distill_loss(a, t, i, teacher_rest=r), (z.requires_grad_(),))
+    # every column an entry: the divergence of the whole distributions
+    t = rand(4, 23, seed=5).double()
+    i = torch.argsort(t, dim=-1, descending=True)
+    got = topk_distill_loss(z, t.gather(-1, i), i)
+    dense = torch.nn.functional.kl_div(torch.log_softmax(z, -1), torch.softmax(t, -1),
+                                       reduction='batchmean')
+    torch.testing.assert_close(got, dense)
+
+
+def test_distill_index_behind_the_vocabulary_is_nan():
+    z, t, i, _ = _distill_case()
+    i[2, 1] = 23
+    loss = topk_distill_loss(z, t, i, reduction='none')
+    assert loss.isnan().tolist() == [False, False, True, False]

@@ -1,0 +1,403 @@
+"""Decoder operators on the GPU against 64 bits, at the sizes, masks, strides
+and uses where a kernel can go wrong."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from distributed_kfac_pytorch_amd.ops.attention import window_attention
+from distributed_kfac_pytorch_amd.ops.distill import topk_distill_loss
+from distributed_kfac_pytorch_amd.ops.rotary import rotary_axes
+from tests import lm_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = {'bf16': torch.bfloat16, 'fp16': torch.float16, 'fp32': torch.float32}
+
+
+def rand(dev, *shape, seed=0, dtype=torch.float32):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(dtype).to(dev)
+
+
+# ------------------------------------------------------------- attention
+ATTN = [
+    # b, hq, hk, tq, tk, d, window, sinks, lengths, start
+    (1, 1, 1, 1, 1, 8, 1, 0, None, None),
+    (2, 2, 2, 33, 33, 16, 5, 0, None, None),
+    (1, 2, 1, 64, 64, 64, 64, 0, None, None),
+    (1, 2, 1, 65, 65, 64, 7, 2, None, None),
+    (2, 3, 1, 129, 129, 32, 40, 5, None, None),
+    (1, 4, 2, 200, 200, 40, 1, 1, None, None),
+    (1, 2, 2, 257, 257, 96, 64, 33, None, None),
+    (1, 5, 1, 130, 130, 104, 50, 0, None, None),
+    (1, 2, 1, 191, 191, 128, 500, 3, None, None),
+    (3, 4, 2, 100, 100, 24, 17, 3, [100, 1, 64], 0),
+    (3, 2, 1, 70, 70, 64, 9, 1, [70, 0, 33], 0),
+    (2, 2, 1, 40, 150, 72, 30, 4, None, None),       # a chunk behind a cache
+    (2, 2, 1, 40, 150, 72, 30, 4, [150, 20], None),  # fewer tokens than rows
+    (2, 2, 1, 40, 50, 16, 30, 4, None, -20),
+    (2, 2, 1, 40, 50, 16, 30, 4, None, [30, -1000000000]),
+    (1, 2, 1, 20, 0, 16, 4, 1, None, None),
+    (1, 2, 1, 300, 300, 16, 3, 170, None, None),     # sinks over two key blocks
+    (1, 2, 1, 1500, 1500, 16, 30, 2, None, None),    # far rows in several chunks
+    (1, 4, 1, 700, 700, 64, 20, 140, [650], 0),
+]
+
+
+@pytest.mark.parametrize('dtype', sorted(DTYPES))
+@pytest.mark.parametrize('case', ATTN, ids=lambda c: '-'.join(str(x) for x in c[:8]))
+def test_attention_matches_formula(cuda, case, dtype):
+    b, hq, hk, tq, tk, d, window, sinks, lengths, start = case
+    dt = DTYPES[dtype]
+    q, k, v, do = (rand(cuda, b, h, t, d, seed=s, dtype=dt) for s, (h, t) in
+                   enumerate([(hq, tq), (hk, tk), (hk, tk), (hq, tq)]))
+    ln = None
+    if lengths is not None:
+        ln = torch.tensor(lengths, dtype=torch.int32, device=cuda)
+        for i, n in enumerate(lengths):
+            k[i, :, n:] = float('nan')
+            v[i, :, n:] = float('inf')
+    st = torch.tensor(start, dtype=torch.int32, device=cuda) if isinstance(start, list) else start
+    conf = dict(window=window, sinks=sinks, lengths=ln, q_start=st)
+    want, tol = ref.attention(q, k, v, do=do, **conf)
+    x = [t.requires_grad_() for t in (q, k, v)]
+    out = window_attention(*x, **conf)
+    got = [out, *torch.autograd.grad(out, x, do)]
+    for name, g, w, t in zip(('out', 'dq', 'dk', 'dv'), got, want, tol):
+        ref.check(name, g, w, t)
+    with torch.no_grad():
+        assert torch.equal(window_attention(*x, **conf), out)
+
+
+TOKEN = [
+    # b, hq, hk, tq, tk, d, window, sinks, lengths
+    (1, 2, 2, 1, 1, 64, 1, 0, None),
+    (3, 8, 2, 1, 300, 64, 40, 4, [300, 7, 0]),
+    (2, 8, 1, 1, 2100, 128, 2100, 0, None),
+    (2, 5, 1, 1, 1999, 80, 700, 3, [1999, 640]),
+    (1, 4, 2, 3, 5000, 32, 5000, 0, None),
+    (1, 3, 3, 1, 4097, 16, 64, 200, None),
+    (1, 40, 1, 1, 3001, 64, 3001, 0, None),
+    (1, 40, 1, 7, 3001, 64, 1000, 10, None),
+]
+
+
+@pytest.mark.parametrize('dtype', sorted(DTYPES))
+@pytest.mark.parametrize('case', TOKEN, ids=lambda c: '-'.join(str(x) for x in c[:8]))
+def test_attention_tokens_match_formula(cuda, case, dtype):
+    b, hq, hk, tq, tk, d, window, sinks, lengths = case
+    dt = DTYPES[dtype]
+    q, k, v = (rand(cuda, b, h, t, d, seed=s, dtype=dt) for s, (h, t) in
+               enumerate([(hq, tq), (hk, tk), (hk, tk)]))
+    ln = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=cuda)
+    for i in range(b):
+        n = tk if lengths is None else lengths[i]
+        k[i, :, n:] = float('nan')
+        v[i, :, n:] = float('nan')
+        if tq == 1 and n - window > sinks:  # what no row sees any more
+            k[i, :, sinks:n - window] = float('inf')
+            v[i, :, sinks:n - window] = float('nan')
+    conf = dict(window=window, sinks=sinks, lengths=ln)
+    want, tol = ref.attention(q, k, v, **conf)
+    ref.check('out', window_attention(q, k, v, **conf), want[0], tol[0])
+    # the same rows with a backward pass to follow
+    out = window_attention(q.requires_grad_(), k, v, **conf)
+    ref.check('out', out, want[0], tol[0])
+
+
+@pytest.mark.parametrize('dtype', ['bf16', 'fp32'])
+def test_attention_strides_and_scale(cuda, dtype):
+    dt = DTYPES[dtype]
+    b, h, t, d = 2, 3, 77, 32
+    qkv = rand(cuda, b, t, h, 3 * d, seed=1, dtype=dt).requires_grad_()
+    do = rand(cuda, b, h, d, t, seed=2, dtype=dt).transpose(2, 3)  # rows not contiguous
+    q, k, v = qkv.permute(0, 2, 1, 3).split(d, dim=-1)
+    conf = dict(window=20, sinks=2, scale=0.31)
+    want, tol = ref.attention(q, k, v, do=do, **conf)
+    out = window_attention(q, k, v, **conf)
+    assert out.transpose(1, 2).is_contiguous()
+    (g,) = torch.autograd.grad(out, qkv, do)
+    g = g.permute(0, 2, 1, 3).split(d, dim=-1)
+    for name, x, w, e in zip(('out', 'dq', 'dk', 'dv'), (out, *g), want, tol):
+        ref.check(name, x, w, e)
+    # rows at odd addresses, and one key head shared without a copy
+    odd = torch.empty(b * t * h * d + 3, dtype=dt, device=cuda)[3:].view(b, h, t, d)
+    odd.copy_(q.detach())
+    kk, vv = (x.detach()[:, :1].expand(b, h, t, d) for x in (k, v))
+    want, tol = ref.attention(odd, kk, vv, do=do, **conf)
+    x = [odd.requires_grad_(), kk.requires_grad_(), vv.requires_grad_()]
+    out = window_attention(*x, **conf)
+    for name, g2, w, e in zip(('out', 'dq', 'dk', 'dv'), (out, *torch.autograd.grad(out, x, do)),
+                              want, tol):
+        ref.check(name, g2, w, e)
+
+
+def test_attention_differences(cuda):
+    """The gradient's component along a direction, by central differences of
+    an fp32 call: step e has an error of e^2 / 6 times the third derivative
+    (of order 1 for inputs of order 1) and 2^-24 |f| / e of rounding."""
+    b, h, t, d = 1, 2, 70, 16
+    x = [rand(cuda, b, h, t, d, seed=s) * 0.5 for s in range(3)]
+    do = rand(cuda, b, h, t, d, seed=7)
+    along = [rand(cuda, b, h, t, d, seed=10 + s) for s in range(3)]
+
+    def f(a):
+        return (window_attention(*a, window=9, sinks=2).double() * do.double()).sum()
+
+    leaves = [a.clone().requires_grad_() for a in x]
+    grads = torch.autograd.grad(f(leaves), leaves)
+    for i in range(3):
+        norm = float(along[i].double().norm())
+        step = 1e-2 / norm
+        lo, hi = ([a + s * step * w if j == i else a for j, (a, w) in enumerate(zip(x, along))]
+                  for s in (-1, 1))
+        want = float((f(hi) - f(lo)) / (2 * step)) / norm
+        got = float((grads[i].double() * along[i].double()).sum()) / norm
+        size = float(grads[i].double().norm())
+        assert abs(got - want) <= 1e-2 * size / norm ** 0.5 + 2e-3, (i, got, want)
+
+
+# --------------------------------------------------------------- rotary
+@pytest.mark.parametrize('dtype', sorted(DTYPES))
+@pytest.mark.parametrize('layout', ['interleaved', 'halves'])
+@pytest.mark.parametrize('b, hq, hk, t, d, sections, ladder', [
+    (1, 1, 1, 1, 2, (1,), 'shared'),
+    (2, 3, 3, 17, 64, (32,), 'shared'),
+    (2, 4, 1, 33, 128, (16, 24, 24), 'shared'),
+    (3, 2, 2, 5, 40, (4, 3, 2), 'per_axis'),
+    (1, 2, 1, 300, 18, (5, 4), 'per_axis'),
+    (2, 5, 2, 1, 80, (8, 8), 'shared'),
+    (1, 2, 2, 9, 256, (128,), 'shared'),
+    (2, 2, 1, 0, 16, (8,), 'shared'),
+])
+def test_rotary_matches_formula(cuda, dtype, layout, b, hq, hk, t, d, sections, ladder):
+    dt = DTYPES[dtype]
+    # views whose rows are not next to each other
+    q = rand(cuda, b, t, hq, d, seed=1, dtype=dt).transpose(1, 2).requires_grad_()
+    k = rand(cuda, b, hk, t, d + 2, seed=2, dtype=dt)[..., :d].requires_grad_()
+    gq, gk = rand(cuda, b, hq, t, d, seed=3, dtype=dt), rand(cuda, b, hk, t, d, seed=4, dtype=dt)
+    g = torch.Generator().manual_seed(5)
+    conf = dict(sections=sections, ladder=ladder, layout=layout)
+    for pos in (torch.randint(-5, 4096, (t, len(sections)), generator=g, dtype=torch.int32),
+                torch.randint(2 ** 30, 2 ** 31, (b, t, len(sections)), generator=g)):
+        pos = pos.to(cuda)
+        out = rotary_axes(q, k, pos, **conf)
+        grads = torch.autograd.grad(out, (q, k), (gq, gk))
+        for name, x, got in (('q', q, out[0]), ('k', k, out[1])):
+            ref.check(name, got, *ref.rotary(x, pos, **conf))
+        for name, x, got in (('dq', gq, grads[0]), ('dk', gk, grads[1])):
+            ref.check(name, got, *ref.rotary(x, pos, sign=-1.0, **conf))
+
+
+def test_rotary_passes_the_rest_through(cuda):
+    q = rand(cuda, 1, 2, 3, 32)
+    q[..., 20:] = float('inf')
+    q[0, 0, 0, 31] = float('nan')
+    pos = torch.arange(3, device=cuda)[:, None]
+    for layout in ('interleaved', 'halves'):
+        out, _ = rotary_axes(q, q, pos, sections=(10,), layout=layout)
+        assert torch.equal(out[..., 20:].isnan(), q[..., 20:].isnan())
+        assert torch.equal(out[..., 20:].isinf(), q[..., 20:].isinf())
+        assert bool(out[..., :20].isfinite().all())
+
+
+# -------------------------------------------------------------- distill
+def _teacher(dev, n, v, k, tau, rest, seed):
+    g = torch.Generator().manual_seed(seed)
+    full = torch.randn(n, v, generator=g) * 2.5
+    t, i = full.topk(k, dim=-1)
+    r = (full / tau).scatter(-1, i, float('-inf')).logsumexp(-1) if rest else None
+    return t.to(dev), i.to(dev), None if r is None else r.to(dev)
+
+
+@pytest.mark.parametrize('dtype', sorted(DTYPES))
+@pytest.mark.parametrize('rest', [False, True])
+@pytest.mark.parametrize('n, v, k, tau, reduction', [
+    (1, 1, 1, 1.0, 'mean'),
+    (3, 7, 2, 1.0, 'sum'),
+    (5, 8, 8, 2.0, 'mean'),
+    (4, 255, 5, 0.5, 'none'),
+    (6, 512, 64, 2.0, 'mean'),
+    (9, 1001, 100, 1.0, 'none'),
+    (2, 33278, 20, 1.5, 'mean'),
+    (3, 5003, 1024, 1.0, 'sum'),
+    (2100, 130, 4, 1.0, 'mean'),      # one block a row
+])
+def test_distill_matches_formula(cuda, dtype, rest, n, v, k, tau, reduction):
+    dt = DTYPES[dtype]
+    z = (rand(cuda, n, v, seed=n) * 2).to(dt).requires_grad_()
+    t, i, r = _teacher(cuda, n, v, k, tau, rest, v)
+    if rest and k == v:
+        r = None  # nothing is left
+    up = rand(cuda, n, seed=9) if reduction == 'none' else torch.tensor(0.37, device=cuda)
+    loss = topk_distill_loss(z, t, i, teacher_rest=r, temperature=tau, reduction=reduction)
+    assert loss.dtype == torch.float32
+    want = ref.distill(z, t, i, rest=r, temperature=tau, reduction=reduction, upstream=up)
+    ref.check('loss', loss, *want[:2])
+    ref.check('dz', *torch.autograd.grad(loss, z, up), *want[2:])
+    with torch.no_grad():
+        assert torch.equal(topk_distill_loss(z, t, i, teacher_rest=r, temperature=tau,
+                                             reduction=reduction), loss)
+
+
+@pytest.mark.parametrize('rest', [False, True])
+def test_distill_padding_repeats_views_and_int32(cuda, rest):
+    b, t, v, k = 3, 9, 1037, 6
+    z = rand(cuda, b, t + 1, v + 3, seed=1, dtype=torch.bfloat16).requires_grad_()
+    view = z[:, :-1, 1:v + 1]                    # odd rows and strides
+    tt, ii, rr = _teacher(cuda, b * t, v, k, 1.3, rest, 4)
+    tt, ii = tt.view(b, t, k), ii.view(b, t, k).to(torch.int32)
+    ii[0, 3:] = -1                               # padding rows
+    ii[1, 2, 4:] = -1                            # fewer entries
+    ii[2, 5, 1] = ii[2, 5, 3]                    # an index twice
+    tt[2, 6, 0] = float('-inf')                  # an entry without mass
+    rr = None if rr is None else rr.view(b, t)
+    loss = topk_distill_loss(view, tt, ii, teacher_rest=rr, temperature=1.3)
+    want = ref.distill(view, tt, ii, rest=rr, temperature=1.3)
+    ref.check('loss', loss, *want[:2])
+    (g,) = torch.autograd.grad(loss, z)
+    assert bool((g[:, -1] == 0).all()) and bool((g[..., 0] == 0).all())
+    assert bool((g[0, 3:] == 0).all())
+    ref.check('dz', g[:, :-1, 1:v + 1], *want[2:])
+    # nothing to learn from at all
+    none = topk_distill_loss(view, tt, torch.full_like(ii, -1), teacher_rest=rr)
+    assert float(none.detach()) == 0.0 and bool((torch.autograd.grad(none, z)[0] == 0).all())
+
+
+def test_distill_bad_rows_stay_alone(cuda):
+    n, v, k = 6, 300, 4
+    z = rand(cuda, n, v, seed=3)
+    t, i, r = _teacher(cuda, n, v, k, 1.0, True, 5)
+    good = topk_distill_loss(z, t, i, teacher_rest=r, reduction='none')
+    z2, i2 = z.clone(), i.clone()
+    i2[1, 2] = v                                  # behind the vocabulary
+    i2[2, 0] = 2 ** 40
+    z2[3, 17] = float('nan')
+    z2[4, i[4, 1]] = float('-inf')                # the student excludes an entry
+    z2.requires_grad_()
+    loss = topk_distill_loss(z2, t, i2, teacher_rest=r, reduction='none')
+    assert loss.isnan().tolist() == [False, True, True, True, False, False]
+    assert float(loss[4]) == float('inf')
+    assert torch.equal(loss[[0, 5]], good[[0, 5]])
+    (g,) = torch.autograd.grad(loss, z2, torch.ones_like(loss))
+    assert bool(g[[0, 4, 5]].isfinite().all()) and bool(g[[1, 2, 3]].isnan().any(dim=-1).all())
+    # masked columns (-inf) that no entry names carry no probability
+    z3 = z.clone()
+    z3[:, :100] = float('-inf')
+    keep = (i >= 100).all(dim=-1)
+    z3.requires_grad_()
+    loss = topk_distill_loss(z3, t, i, teacher_rest=r, reduction='none')
+    (g,) = torch.autograd.grad(loss, z3, torch.ones_like(loss))
+    assert bool(g[keep].isfinite().all())
+    assert bool((g[keep][:, :100] == 0).all())
+
+
+# ------------------------------------------------------------ in use
+def _chain(x, conf):
+    """The operators as a decoder's step runs them: qkv and logits from
+    leaves, rotary, attention, a head, the loss; the leaves' gradients."""
+    qkv, head = x
+    q, k, v = qkv.permute(0, 2, 1, 3).split(conf['d'], dim=-1)
+    q, k = rotary_axes(q, k, conf['pos'], sections=conf['sections'])
+    o = window_attention(q, k, v, window=conf['window'], sinks=conf['sinks'])
+    logits = o.transpose(1, 2).flatten(2) @ head
+    loss = topk_distill_loss(logits, conf['teacher'], conf['index'], teacher_rest=conf['rest'],
+                             temperature=2.0)
+    return [loss, *torch.autograd.grad(loss, x)]
+
+
+def _chain_inputs(dev, dtype, seed=0, b=2, t=70, h=4, d=16, v=333):
+    g = torch.Generator().manual_seed(seed)
+    qkv = torch.randn(b, t, h, 3 * d, generator=g)
+    head = torch.randn(h * d, v, generator=g) * 0.3
+    full = torch.randn(b, t, v, generator=g) * 2
+    teacher, index = full.topk(8, dim=-1)
+    rest = (full / 2).scatter(-1, index, float('-inf')).logsumexp(-1)
+    conf = dict(d=d, window=16, sinks=2, sections=(3, 5), teacher=teacher.to(dev),
+                index=index.to(dev), rest=rest.to(dev),
+                pos=torch.randint(0, 900, (t, 2), generator=g).to(dev))
+    return [x.to(dtype).to(dev).requires_grad_() for x in (qkv, head)], conf
+
+
+def test_chain_matches_64_bits(cuda):
+    """fp32 operators against the same chain in 64 bits on the CPU.  Each
+    operator is within 2^-20 of its operands' size (the bounds above at these
+    sizes), the matrix product within 64 roundings of 2^-24; the chain's
+    gradient passes seven of them: 2^-16 of the gradient's largest element."""
+    x, conf = _chain_inputs(cuda, torch.float32)
+    got = _chain(x, conf)
+    want = _chain([t.detach().cpu().double().requires_grad_() for t in x],
+                  {k: v.cpu() if isinstance(v, torch.Tensor) else v for k, v in conf.items()})
+    for g, w in zip(got, want):
+        assert float((g.cpu().double() - w).abs().max()) <= 2.0 ** -16 * float(w.abs().max())
+
+
+def test_chain_repeats_bit_for_bit_on_any_stream(cuda):
+    x, conf = _chain_inputs(cuda, torch.bfloat16, t=300)
+    first = _chain(x, conf)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    answers = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            answers.append(_chain(x, conf))
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    for a in answers:
+        assert all(torch.equal(p, q) for p, q in zip(first, a))
+
+
+def test_chain_in_two_graphs(cuda):
+    """Forward and backward captured twice, replayed with new inputs in turn
+    and with eager work in between: every replay equals the eager answer."""
+    graphs = []
+    for n in range(2):
+        x, conf = _chain_inputs(cuda, torch.bfloat16, seed=n, t=200 + 30 * n)
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            _chain(x, conf)
+        torch.cuda.current_stream().wait_stream(s)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = _chain(x, conf)
+        graphs.append((g, x, conf, out))
+    for rep in range(4):
+        for n, (g, x, conf, out) in enumerate(graphs):
+            new, _ = _chain_inputs(cuda, torch.bfloat16, seed=10 * rep + n + 5, t=200 + 30 * n)
+            with torch.no_grad():
+                for a, b in zip(x, new):
+                    a.copy_(b)
+            g.replay()
+            torch.cuda.synchronize()
+            kept = [t.clone() for t in out]
+            eager = _chain(x, conf)
+            assert all(torch.equal(a, b) for a, b in zip(kept, eager)), (rep, n)
+
+
+def test_gradients_of_gradients_are_refused(cuda):
+    q = rand(cuda, 1, 1, 4, 8).requires_grad_()
+    z = rand(cuda, 2, 9).requires_grad_()
+    pos = torch.arange(4, device=cuda)[:, None]
+    t, i, _ = _teacher(cuda, 2, 9, 2, 1.0, False, 1)
+    for out, leaf in ((window_attention(q, q, q, window=2).sum(), q),
+                      (rotary_axes(q, q, pos, sections=(4,))[0].sum(), q),
+                      (topk_distill_loss(z, t, i), z)):
+        with pytest.raises(RuntimeError, match='gradients of gradients'):
+            torch.autograd.grad(out, leaf, create_graph=True)
+
+
+def test_one_operand_learns(cuda):
+    q, k, v = (rand(cuda, 1, 2, 40, 16, seed=s) for s in range(3))
+    do = rand(cuda, 1, 2, 40, 16, seed=5)
+    want, tol = ref.attention(q, k, v, window=7, do=do)
+    k.requires_grad_()
+    out = window_attention(q, k, v, window=7)
+    ref.check('dk', torch.autograd.grad(out, k, do)[0], want[2], tol[2])
+    pos = torch.arange(40, device=cuda)[:, None]
+    a, b = rotary_axes(q, k, pos, sections=(8,))
+    (g,) = torch.autograd.grad(b, k, do)          # q's output is not used
+    ref.check('dk', g, *ref.rotary(do, pos, sections=(8,), sign=-1.0))
