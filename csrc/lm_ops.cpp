@@ -131,6 +131,7 @@ kfac::AttnArgs attn_args(const at::Tensor& q, const at::Tensor& k, const at::Ten
   strides3(k, a.ks);
   strides3(v, a.vs);
   a.splits = 1;
+  a.Gmagic = a.G > 1 ? (uint32_t)(((uint64_t)1 << 32) / a.G) : 0xffffffffu;
   return a;
 }
 
@@ -149,7 +150,7 @@ std::tuple<at::Tensor, at::Tensor> attn_forward(const at::Tensor& q, const at::T
   strides3(out, a.os);
   a.lse = want_lse ? lse.data_ptr<float>() : nullptr;
   int64_t floats = 0;
-  kfac::attn_plan(a, tag(q), &a.splits, &floats);
+  kfac::attn_plan(a, &a.splits, &floats);
   at::Tensor ws;
   if (floats > 0) {
     ws = at::empty({floats}, q.options().dtype(at::kFloat));
@@ -210,8 +211,8 @@ struct WindowAttnFn : public torch::autograd::Function<WindowAttnFn> {
       strides3(dk, a.dks);
       strides3(dv, a.dvs);
       int64_t floats = 0;
-      kfac::attn_bwd_plan(a, tag(q), &a.sink_blocks, &a.far_chunks, &floats);
-      TORCH_CHECK((int64_t)(a.Tk + 127) / 128 + (int64_t)a.sink_blocks * a.far_chunks <= 65535,
+      kfac::attn_bwd_plan(a, &a.sink_groups, &a.far_chunks, &floats);
+      TORCH_CHECK((int64_t)(a.Tk + 127) / 128 + (int64_t)a.sink_groups * a.far_chunks <= 65535,
                   "window_attention: more than 65535 key blocks");
       at::Tensor ws;
       if (floats > 0) {

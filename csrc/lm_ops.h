@@ -84,17 +84,16 @@ struct AttnArgs {
   int splits;                   // key slices of a row block (forward)
   float* opart;                 // [splits, B * Hkv, rows, D]
   float* lpart;                 // [splits, B * Hkv, rows]
-  int far_chunks;               // row chunks of the sinks' key blocks (backward)
-  int sink_blocks;
-  float* kvpart;                // [B * Hkv, sink_blocks, 1 + far_chunks, 2, keys, D]
+  uint32_t Gmagic;              // floor(2^32 / G)
+  int sink_groups, far_chunks;  // backward: groups of sink keys, chunks of their far rows
+  float* kvpart;                // their shares
 };
 
-// how a forward call is split, and the floats of its partial results
-void attn_plan(const AttnArgs& a, int dtype, int* splits, int64_t* floats);
+// how a forward call is split over the keys, and the floats of its partial
+// results; the same for the backward call's sinks
+void attn_plan(const AttnArgs& a, int* splits, int64_t* floats);
+void attn_bwd_plan(const AttnArgs& a, int* sink_groups, int* far_chunks, int64_t* floats);
 void attn_forward(int dtype, const AttnArgs& a, hipStream_t st);
-// the same for the backward call's sink blocks
-void attn_bwd_plan(const AttnArgs& a, int dtype, int* sink_blocks, int* far_chunks,
-                   int64_t* floats);
 void attn_backward(int dtype, const AttnArgs& a, hipStream_t st);
 
 }  // namespace kfac

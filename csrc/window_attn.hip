@@ -87,8 +87,21 @@ template <typename T> constexpr int kUnit = 16 / (int)sizeof(T);  // elements of
 // 16-byte row reads of neighbouring rows on different banks
 template <typename T, int DP> constexpr int kLd = DP + kUnit<T>;
 
+// waves a SIMD that the row kernels and the key-gradient kernel leave
+// registers for (256 a wave at 2, 512 at 1)
+template <typename T, int DP> constexpr int kRowWaves = sizeof(T) == 2 || DP <= 64 ? 2 : 1;
+template <typename T, int DP> constexpr int kKeyWaves = (sizeof(T) == 2 ? DP <= 64 : DP <= 32) ? 2 : 1;
+
 // accumulator register e of lane half h is tile row (e & 3) + 8 (e >> 2) + 4 h
 __device__ __forceinline__ int acc_row(int e, int h) { return (e & 3) + 8 * (e >> 2) + 4 * h; }
+
+__device__ __forceinline__ v4f quad_of(const v16f& x, int e4) {
+  return v4f{x[e4 * 4], x[e4 * 4 + 1], x[e4 * 4 + 2], x[e4 * 4 + 3]};
+}
+
+__device__ __forceinline__ v4f add4(v4f a, v4f b) {
+  return v4f{a[0] + b[0], a[1] + b[1], a[2] + b[2], a[3] + b[3]};
+}
 
 __device__ __forceinline__ v16f zero16() {
   v16f z;
@@ -204,6 +217,20 @@ struct Seq {
   int len, start;
 };
 
+// row -> (token, head of the group); a.Gmagic = floor(2^32 / G), so the
+// product is the quotient or one less
+struct Row {
+  int t, g;
+  __device__ __forceinline__ Row(int r, const AttnArgs& a) {
+    t = (int)__umulhi((uint32_t)r, a.Gmagic);
+    g = r - t * a.G;
+    if (g >= a.G) {
+      ++t;
+      g -= a.G;
+    }
+  }
+};
+
 __device__ __forceinline__ Seq sequence(const AttnArgs& a, int b) {
   Seq s;
   s.len = a.Tk;
@@ -242,10 +269,11 @@ struct KeyTiles {
 
 // first and last position of rows [r0, r1) that lie in the sequence; false:
 // none does
-__device__ __forceinline__ bool span(int64_t r0, int64_t r1, int G, const Seq& s, int& pmin,
+__device__ __forceinline__ bool span(int r0, int r1, const AttnArgs& args, const Seq& s, int& pmin,
                                      int& pmax) {
-  const int64_t a = r0 / G + s.start, b = (r1 - 1) / G + s.start;
-  if (r1 <= r0 || b < 0 || a >= s.len || s.len <= 0) return false;
+  if (r1 <= r0 || s.len <= 0) return false;
+  const int64_t a = (int64_t)Row(r0, args).t + s.start, b = (int64_t)Row(r1 - 1, args).t + s.start;
+  if (b < 0 || a >= s.len) return false;
   pmin = (int)(a > 0 ? a : 0);
   pmax = (int)(b < s.len - 1 ? b : s.len - 1);
   return true;
@@ -263,50 +291,103 @@ __device__ __forceinline__ int coverage(int pmin, int pmax, int j0, int W, int S
   return 1;
 }
 
+// scores that rows do not see become -inf: their probability is 0
+template <bool KEYS_IN_REGS>
+__device__ __forceinline__ void hide(v16f& s, int fixed, const int* others, int j0, int h, int W,
+                                     int S) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const int p = KEYS_IN_REGS ? fixed : others[acc_row(e, h)];
+    const int j = KEYS_IN_REGS ? j0 + acc_row(e, h) : fixed;
+    if (!sees(p, j, W, S)) s[e] = -kInf;
+  }
+}
+
+// a row's 32 x ND accumulators as T (or fp32), times f
+template <typename T, typename O, int ND>
+__device__ __forceinline__ void put(O* out, const v16f (&x)[ND], float f, bool zero, int D, int h) {
+  typedef O quad __attribute__((ext_vector_type(4)));
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int e4 = 0; e4 < 4; ++e4) {
+      const int dd = d * 32 + acc_row(e4 * 4, h);
+      if (dd < D) {
+        v4f v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = zero ? 0.f : x[d][e4 * 4 + i] * f;
+        *reinterpret_cast<quad*>(out + dd) = __builtin_convertvector(v, quad);
+      }
+    }
+}
+
+// What a block of the row kernels (forward, dq) works on.
+struct RowBlock {
+  int b, hk, bh, r0, r, t, head, p, h, wave;
+  int wmin, wmax, tiles;
+  bool live, wany;
+  Seq seq;
+  __device__ __forceinline__ RowBlock(const AttnArgs& a) {
+    bh = blockIdx.x;
+    b = bh / a.Hkv;
+    hk = bh - b * a.Hkv;
+    const int rows = a.Tq * a.G;
+    r0 = (int)(gridDim.y - 1 - blockIdx.y) * BM;  // longest rows first
+    const int l = threadIdx.x & 63;
+    wave = threadIdx.x >> 6;
+    h = l >> 5;
+    seq = sequence(a, b);
+    r = r0 + wave * 32 + (l & 31);
+    const Row rw(r, a);
+    t = rw.t;
+    head = hk * a.G + rw.g;
+    live = r < rows;
+    p = live ? position(t, seq) : -1;
+    const int w0 = r0 + wave * 32;
+    wmin = 0;
+    wmax = -1;
+    wany = span(w0, w0 + 32 < rows ? w0 + 32 : rows, a, seq, wmin, wmax);
+  }
+  __device__ __forceinline__ KeyTiles keys(const AttnArgs& a) {
+    const int rows = a.Tq * a.G;
+    int pmin = 0, pmax = -1;
+    const bool any = span(r0, r0 + BM < rows ? r0 + BM : rows, a, seq, pmin, pmax);
+    const KeyTiles kt(pmin, pmax, a.W, a.S);
+    tiles = any ? kt.total : 0;
+    return kt;
+  }
+};
+
 // ---------------------------------------------------------------- forward
 template <typename T, int DP, bool SPLIT>
-__global__ void __launch_bounds__(NT) fwd_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(NT, (kRowWaves<T, DP>)) fwd_kernel(AttnArgs a) {
   constexpr int KD = DP / 16, ND = DP / 32, LD = kLd<T, DP>;
   typedef typename Ops<T>::frag frag;
   __shared__ __attribute__((aligned(16))) T Ks[2][BN * LD];
   __shared__ __attribute__((aligned(16))) T Vs[2][BN * LD];
-  const int bh = blockIdx.x, b = bh / a.Hkv, hk = bh % a.Hkv;
-  const int64_t rows = (int64_t)a.Tq * a.G;
-  const int64_t r0 = (int64_t)(gridDim.y - 1 - blockIdx.y) * BM;  // longest rows first
-  const int l = threadIdx.x & 63, wave = threadIdx.x >> 6, h = l >> 5;
-  const Seq seq = sequence(a, b);
-  const int64_t r = r0 + wave * 32 + (l & 31);
-  const int t = (int)(r / a.G), head = hk * a.G + (int)(r % a.G);
-  const bool live = r < rows;
-  const int p = live ? position(t, seq) : -1;
+  RowBlock w(a);
+  const KeyTiles kt = w.keys(a);
+  const int h = w.h;
   const float c = a.scale * kLog2e;
-
-  int pmin = 0, pmax = -1;
-  const int64_t rend = r0 + BM < rows ? r0 + BM : rows;
-  const bool any = span(r0, rend, a.G, seq, pmin, pmax);
-  const int64_t w0 = r0 + wave * 32;
-  int wmin = 0, wmax = -1;
-  const bool wany = span(w0, w0 + 32 < rows ? w0 + 32 : rows, a.G, seq, wmin, wmax);
-  const KeyTiles kt(pmin, pmax, a.W, a.S);
-  int it0 = 0, it1 = any ? kt.total : 0;
+  int it0 = 0, it1 = w.tiles;
   if (SPLIT) {
     const int per = (it1 + a.splits - 1) / a.splits;
     it0 = per * (int)blockIdx.z < it1 ? per * (int)blockIdx.z : it1;
     it1 = it0 + per < it1 ? it0 + per : it1;
   }
 
-  const T* q = reinterpret_cast<const T*>(a.q) + b * a.qs[0] + head * a.qs[1] + t * a.qs[2];
+  const T* q = reinterpret_cast<const T*>(a.q) + w.b * a.qs[0] + w.head * a.qs[1] + w.t * a.qs[2];
   frag qf[KD];
 #pragma unroll
-  for (int k = 0; k < KD; ++k) qf[k] = global_frag<T>(q, k * 16 + 8 * h, a.D, p >= 0);
+  for (int k = 0; k < KD; ++k) qf[k] = global_frag<T>(q, k * 16 + 8 * h, a.D, w.p >= 0);
 
   v16f o[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) o[d] = zero16();
   float m = -kInf, sum = 0.f;
 
-  const T* kb = reinterpret_cast<const T*>(a.k) + b * a.ks[0] + hk * a.ks[1];
-  const T* vb = reinterpret_cast<const T*>(a.v) + b * a.vs[0] + hk * a.vs[1];
+  const T* kb = reinterpret_cast<const T*>(a.k) + w.b * a.ks[0] + w.hk * a.ks[1];
+  const T* vb = reinterpret_cast<const T*>(a.v) + w.b * a.vs[0] + w.hk * a.vs[1];
   Tile<T, DP> tk, tv;
   auto fetch = [&](int it) {
     const int j0 = kt.key0(it);
@@ -325,19 +406,18 @@ __global__ void __launch_bounds__(NT) fwd_kernel(AttnArgs a) {
 #pragma unroll
     for (int sub = 0; sub < BN / 32; ++sub) {
       const int js = j0 + sub * 32;
-      const int cover = wany ? coverage(wmin, wmax, js, a.W, a.S) : 0;
+      const int cover = w.wany ? coverage(w.wmin, w.wmax, js, a.W, a.S) : 0;
       if (cover == 0) continue;
       v16f s = zero16();
 #pragma unroll
       for (int k = 0; k < KD; ++k)
         s = Ops<T>::mma(row_frag<T, DP>(Ks[buf], sub * 32, k * 16), qf[k], s);
-      float mx = -kInf;
+      if (cover == 1) hide<true>(s, w.p, nullptr, js, h, a.W, a.S);
+      float mx = s[0];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        s[e] = cover == 2 || sees(p, js + acc_row(e, h), a.W, a.S) ? s[e] * c : -kInf;
-        mx = fmaxf(mx, s[e]);
-      }
-      mx = fmaxf(mx, other_half(mx));
+      for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
+      // c > 0: the maximum of the products is the product of the maximum
+      mx = fmaxf(mx, other_half(mx)) * c;
       const float mn = fmaxf(m, mx);
       const float base = mn == -kInf ? 0.f : mn;
       const float alpha = ex2(m - base);
@@ -345,7 +425,7 @@ __global__ void __launch_bounds__(NT) fwd_kernel(AttnArgs a) {
       float add = 0.f;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        s[e] = ex2(s[e] - base);
+        s[e] = ex2(__builtin_fmaf(s[e], c, -base));
         add += s[e];
       }
       sum = sum * alpha + add;
@@ -364,77 +444,82 @@ __global__ void __launch_bounds__(NT) fwd_kernel(AttnArgs a) {
   }
 
   sum += other_half(sum);
-  const bool none = p < 0 || sum == 0.f;
+  const bool none = w.p < 0 || sum == 0.f;
   const float inv = none ? 0.f : 1.f / sum;
   const float lse = none ? kInf : m + log2f(sum);
-  if (!live) return;
+  if (!w.live) return;
   if (SPLIT) {
-    const int64_t at = ((int64_t)blockIdx.z * gridDim.x + bh) * rows + r;
+    const int64_t at = ((int64_t)blockIdx.z * gridDim.x + w.bh) * (a.Tq * a.G) + w.r;
     if (h == 0) a.lpart[at] = none ? -kInf : lse;
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-      for (int e4 = 0; e4 < 4; ++e4) {
-        const int dd = d * 32 + acc_row(e4 * 4, h);
-        if (dd < a.D)
-          *reinterpret_cast<float4*>(a.opart + at * a.D + dd) =
-              none ? make_float4(0.f, 0.f, 0.f, 0.f)
-                   : make_float4(o[d][e4 * 4] * inv, o[d][e4 * 4 + 1] * inv,
-                                 o[d][e4 * 4 + 2] * inv, o[d][e4 * 4 + 3] * inv);
-      }
+    put<T, float, ND>(a.opart + at * a.D, o, inv, none, a.D, h);
     return;
   }
-  if (h == 0 && a.lse != nullptr) a.lse[((int64_t)b * a.Hq + head) * a.Tq + t] = lse;
-  T* out = reinterpret_cast<T*>(a.out) + b * a.os[0] + head * a.os[1] + t * a.os[2];
-#pragma unroll
-  for (int d = 0; d < ND; ++d)
-#pragma unroll
-    for (int e4 = 0; e4 < 4; ++e4) {
-      const int dd = d * 32 + acc_row(e4 * 4, h);
-      if (dd < a.D) {
-        v4f f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = none ? 0.f : o[d][e4 * 4 + i] * inv;
-        *reinterpret_cast<typename Ops<T>::quad*>(out + dd) =
-            __builtin_convertvector(f, typename Ops<T>::quad);
-      }
-    }
+  if (h == 0 && a.lse != nullptr) a.lse[((int64_t)w.b * a.Hq + w.head) * a.Tq + w.t] = lse;
+  put<T, T, ND>(reinterpret_cast<T*>(a.out) + w.b * a.os[0] + w.head * a.os[1] + w.t * a.os[2], o,
+                inv, none, a.D, h);
 }
 
-// joins the key slices of a row, in order: one thread per 4 elements of D
+// Joins the key slices of a row: one block a row, 8 lanes groups of 32 (4
+// elements of D a lane) walk every eighth slice, and the groups' sums are
+// added in order.
 template <typename T>
 __global__ void __launch_bounds__(NT) join_kernel(AttnArgs a) {
-  const int64_t rows = (int64_t)a.Tq * a.G, D4 = a.D / 4;
-  const int64_t id = (int64_t)blockIdx.x * NT + threadIdx.x;
-  const int64_t all = (int64_t)a.B * a.Hkv * rows;
-  if (id >= all * D4) return;
-  const int64_t row = id / D4;
-  const int d = (int)(id % D4) * 4;
-  float m = -kInf;
-  for (int z = 0; z < a.splits; ++z) m = fmaxf(m, a.lpart[z * all + row]);
-  const float base = m == -kInf ? 0.f : m;
-  float sum = 0.f;
-  v4f o = {0.f, 0.f, 0.f, 0.f};
-  for (int z = 0; z < a.splits; ++z) {
-    const float lp = a.lpart[z * all + row];
-    // a slice that saw nothing left zeros; one with a NaN has a NaN sum and
-    // must not be skipped
-    const float w = ex2(lp - base);
-    const v4f x = *reinterpret_cast<const v4f*>(a.opart + (z * all + row) * a.D + d);
-    sum += w;
+  __shared__ float wts[256];
+  __shared__ v4f part[8][32];
+  __shared__ float red[NT / 64];
+  const int rows = a.Tq * a.G;
+  const int64_t row = blockIdx.x, all = (int64_t)a.B * a.Hkv * rows;
+  const int tid = threadIdx.x;
+  float lp = tid < a.splits ? a.lpart[tid * all + row] : -kInf;
+  float m = lp;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] += w * x[i];
+  for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+  if ((tid & 63) == 0) red[tid >> 6] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float base = m == -kInf ? 0.f : m;
+  // a slice that saw nothing has weight 0; one with a NaN keeps it
+  wts[tid] = ex2(lp - base);
+  __syncthreads();
+  const int grp = tid >> 5, d = (tid & 31) * 4;
+  v4f o = {0.f, 0.f, 0.f, 0.f};
+  float sum = 0.f;
+  for (int z = grp; z < a.splits; z += 8) {
+    const float wt = wts[z];
+    sum += wt;
+    if (d < a.D) {
+      const v4f x = *reinterpret_cast<const v4f*>(a.opart + (z * all + row) * a.D + d);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] += wt * x[i];
+    }
+  }
+  part[grp][tid & 31] = o;
+  __syncthreads();
+  if (tid < 32) wts[tid] = 0.f;
+  __syncthreads();
+  if ((tid & 31) == 0) wts[grp] = sum;
+  __syncthreads();
+  if (tid >= 32) return;
+  o = part[0][tid];
+  sum = wts[0];
+#pragma unroll
+  for (int g = 1; g < 8; ++g) {
+    sum += wts[g];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] += part[g][tid][i];
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
   for (int i = 0; i < 4; ++i) o[i] *= inv;
-  const int64_t bh = row / rows, r = row % rows;
-  const int64_t b = bh / a.Hkv, t = r / a.G, head = (bh % a.Hkv) * a.G + r % a.G;
-  *reinterpret_cast<typename Ops<T>::quad*>(reinterpret_cast<T*>(a.out) + b * a.os[0] +
-                                            head * a.os[1] + t * a.os[2] + d) =
-      __builtin_convertvector(o, typename Ops<T>::quad);
-  if (d == 0 && a.lse != nullptr)
-    a.lse[(b * a.Hq + head) * a.Tq + t] = sum == 0.f ? kInf : base + log2f(sum);
+  const int bh = (int)(row / rows), b = bh / a.Hkv;
+  const Row rw((int)(row - (int64_t)bh * rows), a);
+  const int head = (bh - b * a.Hkv) * a.G + rw.g;
+  if (d < a.D)
+    *reinterpret_cast<typename Ops<T>::quad*>(reinterpret_cast<T*>(a.out) + b * a.os[0] +
+                                              head * a.os[1] + rw.t * a.os[2] + d) =
+        __builtin_convertvector(o, typename Ops<T>::quad);
+  if (tid == 0 && a.lse != nullptr)
+    a.lse[((int64_t)b * a.Hq + head) * a.Tq + rw.t] = sum == 0.f ? kInf : base + log2f(sum);
 }
 
 // --------------------------------------------------------------- backward
@@ -442,53 +527,40 @@ __global__ void __launch_bounds__(NT) join_kernel(AttnArgs a) {
 // and layout once more: S^T = K Q^T, dP^T = V dO^T, dS^T = P (dP - delta),
 // dQ^T += K^T dS^T.
 template <typename T, int DP>
-__global__ void __launch_bounds__(NT) dq_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(NT, (kRowWaves<T, DP>)) dq_kernel(AttnArgs a) {
   constexpr int KD = DP / 16, ND = DP / 32, LD = kLd<T, DP>;
   typedef typename Ops<T>::frag frag;
   __shared__ __attribute__((aligned(16))) T Ks[2][BN * LD];
   __shared__ __attribute__((aligned(16))) T Vs[2][BN * LD];
-  const int bh = blockIdx.x, b = bh / a.Hkv, hk = bh % a.Hkv;
-  const int64_t rows = (int64_t)a.Tq * a.G;
-  const int64_t r0 = (int64_t)(gridDim.y - 1 - blockIdx.y) * BM;
-  const int l = threadIdx.x & 63, wave = threadIdx.x >> 6, h = l >> 5;
-  const Seq seq = sequence(a, b);
-  const int64_t r = r0 + wave * 32 + (l & 31);
-  const int t = (int)(r / a.G), head = hk * a.G + (int)(r % a.G);
-  const bool live = r < rows;
-  const int p = live ? position(t, seq) : -1;
+  RowBlock w(a);
+  const KeyTiles kt = w.keys(a);
+  const int h = w.h, it1 = w.tiles;
   const float c = a.scale * kLog2e;
 
-  int pmin = 0, pmax = -1;
-  const bool any = span(r0, r0 + BM < rows ? r0 + BM : rows, a.G, seq, pmin, pmax);
-  const int64_t w0 = r0 + wave * 32;
-  int wmin = 0, wmax = -1;
-  const bool wany = span(w0, w0 + 32 < rows ? w0 + 32 : rows, a.G, seq, wmin, wmax);
-  const KeyTiles kt(pmin, pmax, a.W, a.S);
-  const int it1 = any ? kt.total : 0;
-
-  const T* q = reinterpret_cast<const T*>(a.q) + b * a.qs[0] + head * a.qs[1] + t * a.qs[2];
-  const T* g = reinterpret_cast<const T*>(a.dout) + b * a.dos[0] + head * a.dos[1] + t * a.dos[2];
-  const T* o = reinterpret_cast<const T*>(a.out) + b * a.os[0] + head * a.os[1] + t * a.os[2];
+  const T* q = reinterpret_cast<const T*>(a.q) + w.b * a.qs[0] + w.head * a.qs[1] + w.t * a.qs[2];
+  const T* g =
+      reinterpret_cast<const T*>(a.dout) + w.b * a.dos[0] + w.head * a.dos[1] + w.t * a.dos[2];
+  const T* o = reinterpret_cast<const T*>(a.out) + w.b * a.os[0] + w.head * a.os[1] + w.t * a.os[2];
   frag qf[KD], gf[KD];
   float delta = 0.f;
 #pragma unroll
   for (int k = 0; k < KD; ++k) {
-    qf[k] = global_frag<T>(q, k * 16 + 8 * h, a.D, p >= 0);
-    gf[k] = global_frag<T>(g, k * 16 + 8 * h, a.D, p >= 0);
-    const frag of = global_frag<T>(o, k * 16 + 8 * h, a.D, p >= 0);
+    qf[k] = global_frag<T>(q, k * 16 + 8 * h, a.D, w.p >= 0);
+    gf[k] = global_frag<T>(g, k * 16 + 8 * h, a.D, w.p >= 0);
+    const frag of = global_frag<T>(o, k * 16 + 8 * h, a.D, w.p >= 0);
 #pragma unroll
     for (int i = 0; i < 8; ++i) delta += (float)gf[k][i] * (float)of[i];
   }
   delta += other_half(delta);
-  const int64_t at = ((int64_t)b * a.Hq + head) * a.Tq + t;
-  if (live && h == 0) a.delta[at] = delta;
-  const float lse = p >= 0 ? a.lse[at] : kInf;
+  const int64_t at = ((int64_t)w.b * a.Hq + w.head) * a.Tq + w.t;
+  if (w.live && h == 0) a.delta[at] = delta;
+  const float lse = w.p >= 0 ? a.lse[at] : kInf;
 
   v16f dq[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) dq[d] = zero16();
-  const T* kb = reinterpret_cast<const T*>(a.k) + b * a.ks[0] + hk * a.ks[1];
-  const T* vb = reinterpret_cast<const T*>(a.v) + b * a.vs[0] + hk * a.vs[1];
+  const T* kb = reinterpret_cast<const T*>(a.k) + w.b * a.ks[0] + w.hk * a.ks[1];
+  const T* vb = reinterpret_cast<const T*>(a.v) + w.b * a.vs[0] + w.hk * a.vs[1];
   Tile<T, DP> tk, tv;
   auto fetch = [&](int it) {
     const int j0 = kt.key0(it);
@@ -507,7 +579,7 @@ __global__ void __launch_bounds__(NT) dq_kernel(AttnArgs a) {
 #pragma unroll
     for (int sub = 0; sub < BN / 32; ++sub) {
       const int js = j0 + sub * 32;
-      const int cover = wany ? coverage(wmin, wmax, js, a.W, a.S) : 0;
+      const int cover = w.wany ? coverage(w.wmin, w.wmax, js, a.W, a.S) : 0;
       if (cover == 0) continue;
       v16f s = zero16(), dp = zero16();
 #pragma unroll
@@ -515,11 +587,9 @@ __global__ void __launch_bounds__(NT) dq_kernel(AttnArgs a) {
         s = Ops<T>::mma(row_frag<T, DP>(Ks[buf], sub * 32, k * 16), qf[k], s);
         dp = Ops<T>::mma(row_frag<T, DP>(Vs[buf], sub * 32, k * 16), gf[k], dp);
       }
+      if (cover == 1) hide<true>(s, w.p, nullptr, js, h, a.W, a.S);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float pr = ex2(s[e] * c - lse);
-        s[e] = cover == 2 || sees(p, js + acc_row(e, h), a.W, a.S) ? pr * (dp[e] - delta) : 0.f;
-      }
+      for (int e = 0; e < 16; ++e) s[e] = ex2(__builtin_fmaf(s[e], c, -lse)) * (dp[e] - delta);
 #pragma unroll
       for (int ss = 0; ss < 2; ++ss) {
         const frag sf = acc_frag<T>(s, ss);
@@ -529,27 +599,15 @@ __global__ void __launch_bounds__(NT) dq_kernel(AttnArgs a) {
       }
     }
   }
-  if (!live) return;
-  T* out = reinterpret_cast<T*>(a.dq) + b * a.dqs[0] + head * a.dqs[1] + t * a.dqs[2];
-#pragma unroll
-  for (int d = 0; d < ND; ++d)
-#pragma unroll
-    for (int e4 = 0; e4 < 4; ++e4) {
-      const int dd = d * 32 + acc_row(e4 * 4, h);
-      if (dd < a.D) {
-        v4f f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = p < 0 ? 0.f : dq[d][e4 * 4 + i] * a.scale;
-        *reinterpret_cast<typename Ops<T>::quad*>(out + dd) =
-            __builtin_convertvector(f, typename Ops<T>::quad);
-      }
-    }
+  if (!w.live) return;
+  put<T, T, ND>(reinterpret_cast<T*>(a.dq) + w.b * a.dqs[0] + w.head * a.dqs[1] + w.t * a.dqs[2],
+                dq, a.scale, w.p < 0, a.D, h);
 }
 
 // Rows that look at the keys [k0, k0 + BM): the near ones, whose window
 // reaches there, and, where the block holds sinks, the far ones behind them.
 struct RowRange {
-  int64_t n0, n1, f1;  // near [n0, n1), far [n1, f1)
+  int n0, n1, f1;  // near [n0, n1), far [n1, f1)
   __device__ __forceinline__ RowRange(int k0, const AttnArgs& a, const Seq& s) {
     const int64_t last = (int64_t)s.len - 1;        // last position
     const int64_t kend = k0 + BM - 1 < last ? k0 + BM - 1 : last;
@@ -561,206 +619,252 @@ struct RowRange {
     f1 = k0 < a.S && k0 <= last ? clip(last + 1 - s.start, a) * a.G : n1;
     if (f1 < n1) f1 = n1;
   }
-  __device__ __forceinline__ static int64_t clip(int64_t t, const AttnArgs& a) {
-    return t < 0 ? 0 : (t < a.Tq ? t : a.Tq);
+  __device__ __forceinline__ static int clip(int64_t t, const AttnArgs& a) {
+    return (int)(t < 0 ? 0 : (t < a.Tq ? t : a.Tq));
   }
 };
 
-// far rows [f0, f1) of chunk `ch` of `chunks`, in whole tiles
-__device__ __forceinline__ void far_chunk(const RowRange& rr, int ch, int chunks, int64_t& f0,
-                                          int64_t& f1) {
-  const int64_t tiles = (rr.f1 - rr.n1 + BN - 1) / BN;
-  const int64_t per = (tiles + chunks - 1) / chunks;
-  f0 = rr.n1 + per * ch * BN;
-  f1 = f0 + per * BN;
-  if (f1 > rr.f1) f1 = rr.f1;
-  if (f0 > f1) f0 = f1;
+constexpr int kSinkKeys = 32;  // keys of a far item
+
+// fp32 sums of (group of sink keys, share) in AttnArgs::kvpart: share 0 from
+// the near rows, 1 + i from chunk i of the far ones; [dk, dv][key][D]
+__device__ __forceinline__ float* sink_part(const AttnArgs& a, int bh, int group, int share) {
+  return a.kvpart + (((int64_t)bh * a.sink_groups + group) * (1 + a.far_chunks) + share) * 2 *
+                        kSinkKeys * a.D;
 }
 
-// dk and dv: a wave owns 32 keys and the block walks the rows that look at
-// them.  S = Q K^T and dP = dO V^T have a row's scores in register order, so
-// dV^T += dO^T P and dK^T += Q^T dS take P and dS from where they are.
-// blockIdx.y < key blocks: the near rows; above: a chunk of the far rows of
-// a block with sinks, whose sums join_kv_kernel adds up.
+// 64 rows of q and do, and their statistics
 template <typename T, int DP>
-__global__ void __launch_bounds__(NT) dkv_kernel(AttnArgs a, int key_blocks) {
-  constexpr int KD = DP / 16, ND = DP / 32, LD = kLd<T, DP>;
-  typedef typename Ops<T>::frag frag;
-  __shared__ __attribute__((aligned(16))) T Qs[2][BN * LD];
-  __shared__ __attribute__((aligned(16))) T Gs[2][BN * LD];
-  __shared__ float Ls[2][BN], Ds[2][BN];
-  __shared__ int Ps[2][BN];
-  const int bh = blockIdx.x, b = bh / a.Hkv, hk = bh % a.Hkv;
-  const int l = threadIdx.x & 63, wave = threadIdx.x >> 6, h = l >> 5;
-  const Seq seq = sequence(a, b);
-  const bool far = (int)blockIdx.y >= key_blocks;
-  const int item = far ? (int)blockIdx.y - key_blocks : (int)blockIdx.y;
-  const int kblock = far ? item / a.far_chunks : item;
-  const int k0 = kblock * BM;
-  const RowRange rr(k0, a, seq);
-  int64_t ra = rr.n0, rb = rr.n1;
-  if (far) far_chunk(rr, item % a.far_chunks, a.far_chunks, ra, rb);
+struct RowTile {
+  Tile<T, DP> q, g;
+  float lse, delta;
+  int p;
+  __device__ __forceinline__ void load(const AttnArgs& a, const Seq& seq, int b, int hk, int t0,
+                                       int end) {
+    const T* qb = reinterpret_cast<const T*>(a.q) + b * a.qs[0] + hk * a.G * a.qs[1];
+    const T* gb = reinterpret_cast<const T*>(a.dout) + b * a.dos[0] + hk * a.G * a.dos[1];
+    q.load([&](int i) {
+      const Row r(t0 + i, a);
+      return t0 + i < end ? qb + r.g * a.qs[1] + r.t * a.qs[2] : nullptr;
+    }, a.D);
+    g.load([&](int i) {
+      const Row r(t0 + i, a);
+      return t0 + i < end ? gb + r.g * a.dos[1] + r.t * a.dos[2] : nullptr;
+    }, a.D);
+    if (threadIdx.x < BN) {
+      const int r = t0 + threadIdx.x;
+      const Row rw(r, a);
+      // rows outside the sequence have lse = +inf: P = 0
+      p = r < end ? position(rw.t, seq) : -1;
+      lse = kInf;
+      delta = 0.f;
+      if (p >= 0) {
+        const int64_t at = ((int64_t)b * a.Hq + hk * a.G + rw.g) * a.Tq + rw.t;
+        lse = a.lse[at];
+        delta = a.delta[at];
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* Q, T* G, float* L, float* D, int* P) const {
+    q.store(Q);
+    g.store(G);
+    if (threadIdx.x < BN) {
+      L[threadIdx.x] = lse;
+      D[threadIdx.x] = delta;
+      P[threadIdx.x] = p;
+    }
+  }
+};
 
-  const int key = k0 + wave * 32 + (l & 31);
-  const bool kok = key < seq.len;
-  const float c = a.scale * kLog2e;
+// dk and dv: a wave owns 32 keys.  S = Q K^T and dP = dO V^T have a row's
+// scores in register order, so dV^T += dO^T P and dK^T += Q^T dS take P and
+// dS from where they are.
+template <typename T, int DP>
+struct KeyGrad {
+  static constexpr int KD = DP / 16, ND = DP / 32;
+  typedef typename Ops<T>::frag frag;
   frag kf[KD], vf[KD];
-  {
+  v16f dk[ND], dv[ND];
+
+  __device__ __forceinline__ void init(const AttnArgs& a, int b, int hk, int key, bool ok) {
+    const int h = (threadIdx.x & 63) >> 5;
     const T* kp = reinterpret_cast<const T*>(a.k) + b * a.ks[0] + hk * a.ks[1] + key * a.ks[2];
     const T* vp = reinterpret_cast<const T*>(a.v) + b * a.vs[0] + hk * a.vs[1] + key * a.vs[2];
 #pragma unroll
     for (int k = 0; k < KD; ++k) {
-      kf[k] = global_frag<T>(kp, k * 16 + 8 * h, a.D, kok);
-      vf[k] = global_frag<T>(vp, k * 16 + 8 * h, a.D, kok);
+      kf[k] = global_frag<T>(kp, k * 16 + 8 * h, a.D, ok);
+      vf[k] = global_frag<T>(vp, k * 16 + 8 * h, a.D, ok);
     }
-  }
-  v16f dk[ND], dv[ND];
 #pragma unroll
-  for (int d = 0; d < ND; ++d) dk[d] = dv[d] = zero16();
-
-  const T* qb = reinterpret_cast<const T*>(a.q) + b * a.qs[0] + hk * a.G * a.qs[1];
-  const T* gb = reinterpret_cast<const T*>(a.dout) + b * a.dos[0] + hk * a.G * a.dos[1];
-  Tile<T, DP> tq, tg;
-  float nl = 0.f, nd = 0.f;
-  int np = -1;
-  auto fetch = [&](int64_t t0) {
-    tq.load([&](int i) {
-      const int64_t r = t0 + i;
-      return r < rb ? qb + (r % a.G) * a.qs[1] + (r / a.G) * a.qs[2] : nullptr;
-    }, a.D);
-    tg.load([&](int i) {
-      const int64_t r = t0 + i;
-      return r < rb ? gb + (r % a.G) * a.dos[1] + (r / a.G) * a.dos[2] : nullptr;
-    }, a.D);
-    if (threadIdx.x < BN) {
-      const int64_t r = t0 + threadIdx.x;
-      np = r < rb ? position(r / a.G, seq) : -1;
-      nl = kInf;
-      nd = 0.f;
-      if (np >= 0) {
-        const int64_t at = ((int64_t)b * a.Hq + hk * a.G + r % a.G) * a.Tq + r / a.G;
-        nl = a.lse[at];
-        nd = a.delta[at];
-      }
-    }
-  };
-  if (ra < rb) fetch(ra);
-  int buf = 0;
-  for (int64_t t0 = ra; t0 < rb; t0 += BN, buf ^= 1) {
-    tq.store(Qs[buf]);
-    tg.store(Gs[buf]);
-    if (threadIdx.x < BN) {
-      Ls[buf][threadIdx.x] = nl;
-      Ds[buf][threadIdx.x] = nd;
-      Ps[buf][threadIdx.x] = np;
-    }
-    __syncthreads();
-    if (t0 + BN < rb) fetch(t0 + BN);
-#pragma unroll
-    for (int sub = 0; sub < BN / 32; ++sub) {
-      const int64_t s0 = t0 + sub * 32;
-      int pmin, pmax;
-      const bool any = span(s0, s0 + 32 < rb ? s0 + 32 : rb, a.G, seq, pmin, pmax);
-      const int cover = any ? coverage(pmin, pmax, k0 + wave * 32, a.W, a.S) : 0;
-      if (cover == 0) continue;
-      v16f s = zero16(), dp = zero16();
-#pragma unroll
-      for (int k = 0; k < KD; ++k) {
-        s = Ops<T>::mma(row_frag<T, DP>(Qs[buf], sub * 32, k * 16), kf[k], s);
-        dp = Ops<T>::mma(row_frag<T, DP>(Gs[buf], sub * 32, k * 16), vf[k], dp);
-      }
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int i = sub * 32 + acc_row(e, h);
-        const bool see = cover == 2 || sees(Ps[buf][i], key, a.W, a.S);
-        // rows outside the sequence have lse = +inf: P = 0
-        const float pr = see ? ex2(s[e] * c - Ls[buf][i]) : 0.f;
-        dp[e] = see ? pr * (dp[e] - Ds[buf][i]) : 0.f;
-        s[e] = pr;
-      }
-#pragma unroll
-      for (int ss = 0; ss < 2; ++ss) {
-        const frag pf = acc_frag<T>(s, ss), sf = acc_frag<T>(dp, ss);
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          dv[d] = Ops<T>::mma(col_frag<T, DP>(Gs[buf], sub * 32 + ss * 16, d * 32), pf, dv[d]);
-          dk[d] = Ops<T>::mma(col_frag<T, DP>(Qs[buf], sub * 32 + ss * 16, d * 32), sf, dk[d]);
-        }
-      }
-    }
+    for (int d = 0; d < ND; ++d) dk[d] = dv[d] = zero16();
   }
 
-  if (a.far_chunks > 0 && kblock < a.sink_blocks) {
-    // a share of a sink block's sums: [slot][dk, dv][key][D], fp32
-    const int64_t slot = ((int64_t)bh * a.sink_blocks + kblock) * (1 + a.far_chunks) +
-                         (far ? 1 + item % a.far_chunks : 0);
-    float* part = a.kvpart + (slot * 2 * BM + wave * 32 + (l & 31)) * a.D;
+  // 32 rows from tile row i0 on
+  __device__ __forceinline__ void rows(const AttnArgs& a, const T* Q, const T* G, const float* L,
+                                       const float* D, const int* P, int i0, int key, int cover) {
+    const int h = (threadIdx.x & 63) >> 5;
+    const float c = a.scale * kLog2e;
+    v16f s = zero16(), dp = zero16();
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-      for (int e4 = 0; e4 < 4; ++e4) {
-        const int dd = d * 32 + acc_row(e4 * 4, h);
-        if (dd < a.D) {
-          v4f fk, fv;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            fk[i] = dk[d][e4 * 4 + i] * a.scale;
-            fv[i] = dv[d][e4 * 4 + i];
-          }
-          *reinterpret_cast<v4f*>(part + dd) = fk;
-          *reinterpret_cast<v4f*>(part + (int64_t)BM * a.D + dd) = fv;
-        }
-      }
-    return;
-  }
-  if (key >= a.Tk) return;
-  T* ok = reinterpret_cast<T*>(a.dk) + b * a.dks[0] + hk * a.dks[1] + key * a.dks[2];
-  T* ov = reinterpret_cast<T*>(a.dv) + b * a.dvs[0] + hk * a.dvs[1] + key * a.dvs[2];
-#pragma unroll
-  for (int d = 0; d < ND; ++d)
+    for (int k = 0; k < KD; ++k) {
+      s = Ops<T>::mma(row_frag<T, DP>(Q, i0, k * 16), kf[k], s);
+      dp = Ops<T>::mma(row_frag<T, DP>(G, i0, k * 16), vf[k], dp);
+    }
+    if (cover == 1) hide<false>(s, key, P + i0, 0, h, a.W, a.S);
 #pragma unroll
     for (int e4 = 0; e4 < 4; ++e4) {
-      const int dd = d * 32 + acc_row(e4 * 4, h);
-      if (dd < a.D) {
-        v4f fk, fv;
+      const v4f le = *reinterpret_cast<const v4f*>(L + i0 + acc_row(e4 * 4, h));
+      const v4f de = *reinterpret_cast<const v4f*>(D + i0 + acc_row(e4 * 4, h));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          fk[i] = dk[d][e4 * 4 + i] * a.scale;
-          fv[i] = dv[d][e4 * 4 + i];
-        }
-        *reinterpret_cast<typename Ops<T>::quad*>(ok + dd) =
-            __builtin_convertvector(fk, typename Ops<T>::quad);
-        *reinterpret_cast<typename Ops<T>::quad*>(ov + dd) =
-            __builtin_convertvector(fv, typename Ops<T>::quad);
+      for (int i = 0; i < 4; ++i) {
+        const int e = e4 * 4 + i;
+        s[e] = ex2(__builtin_fmaf(s[e], c, -le[i]));
+        dp[e] = s[e] * (dp[e] - de[i]);
       }
     }
+#pragma unroll
+    for (int ss = 0; ss < 2; ++ss) {
+      const frag pf = acc_frag<T>(s, ss), sf = acc_frag<T>(dp, ss);
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        dv[d] = Ops<T>::mma(col_frag<T, DP>(G, i0 + ss * 16, d * 32), pf, dv[d]);
+        dk[d] = Ops<T>::mma(col_frag<T, DP>(Q, i0 + ss * 16, d * 32), sf, dk[d]);
+      }
+    }
+  }
+};
+
+// blockIdx.y < key_blocks: the near rows of 128 keys, 32 a wave, the rows
+// streamed in tiles of 64.  Above: a chunk of the far rows of 32 sink keys,
+// which all waves own together, 32 rows each of a tile of 128; their sums
+// are added in wave order.  Sinks are few and the rows behind the window
+// many, so a far item has its rows spread over the waves and not its keys.
+template <typename T, int DP>
+__global__ void __launch_bounds__(NT, (kKeyWaves<T, DP>)) dkv_kernel(AttnArgs a, int key_blocks) {
+  constexpr int ND = DP / 32, LD = kLd<T, DP>;
+  __shared__ __attribute__((aligned(16))) T Qs[2][BN * LD];
+  __shared__ __attribute__((aligned(16))) T Gs[2][BN * LD];
+  __shared__ __attribute__((aligned(16))) float Ls[2][BN], Ds[2][BN];
+  __shared__ int Ps[2][BN];
+  static_assert(2 * BN * LD * sizeof(T) >= kSinkKeys * DP * sizeof(float), "sums of a far item");
+  const int bh = blockIdx.x, b = bh / a.Hkv, hk = bh - b * a.Hkv;
+  const int l = threadIdx.x & 63, wave = threadIdx.x >> 6, h = l >> 5;
+  const Seq seq = sequence(a, b);
+  RowTile<T, DP> tile;
+  KeyGrad<T, DP> kg;
+
+  if ((int)blockIdx.y >= key_blocks) {
+    const int item = (int)blockIdx.y - key_blocks;
+    const int group = item / a.far_chunks, chunk = item - group * a.far_chunks;
+    const int j0 = group * kSinkKeys, key = j0 + (l & 31);
+    const RowRange rr(j0 / BM * BM, a, seq);
+    const int tiles = (rr.f1 - rr.n1 + BM - 1) / BM;
+    const int per = (tiles + a.far_chunks - 1) / a.far_chunks;
+    int ra = rr.n1 + per * chunk * BM, rb = ra + per * BM;
+    if (rb > rr.f1) rb = rr.f1;
+    kg.init(a, b, hk, key, key < seq.len);
+    for (int t0 = ra; t0 < rb; t0 += BM) {
+      __syncthreads();
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        tile.load(a, seq, b, hk, t0 + half * BN, rb);
+        tile.store(Qs[half], Gs[half], Ls[half], Ds[half], Ps[half]);
+      }
+      __syncthreads();
+      const int s0 = t0 + wave * 32;
+      int pmin, pmax;
+      const int cover = span(s0, s0 + 32 < rb ? s0 + 32 : rb, a, seq, pmin, pmax)
+                            ? coverage(pmin, pmax, j0, a.W, a.S) : 0;
+      if (cover != 0)
+        kg.rows(a, Qs[0], Gs[0], Ls[0], Ds[0], Ps[0], wave * 32, key, cover);
+    }
+    float* sk = reinterpret_cast<float*>(&Qs[0][0]);
+    float* sv = reinterpret_cast<float*>(&Gs[0][0]);
+    for (int turn = 0; turn < NT / 64; ++turn) {
+      __syncthreads();
+      if (wave == turn) {
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int e4 = 0; e4 < 4; ++e4) {
+            const int at = (l & 31) * DP + d * 32 + acc_row(e4 * 4, h);
+            v4f fk = quad_of(kg.dk[d], e4), fv = quad_of(kg.dv[d], e4);
+            if (turn > 0) {
+              fk = add4(fk, *reinterpret_cast<const v4f*>(sk + at));
+              fv = add4(fv, *reinterpret_cast<const v4f*>(sv + at));
+            }
+            *reinterpret_cast<v4f*>(sk + at) = fk;
+            *reinterpret_cast<v4f*>(sv + at) = fv;
+          }
+      }
+    }
+    __syncthreads();
+    float* part = sink_part(a, bh, group, 1 + chunk);
+    for (int i = threadIdx.x; i < kSinkKeys * (DP / 4); i += NT) {
+      const int kk = i / (DP / 4), d = i % (DP / 4) * 4;
+      if (d >= a.D || j0 + kk >= a.S) continue;
+      const v4f fk = *reinterpret_cast<const v4f*>(sk + kk * DP + d);
+      *reinterpret_cast<v4f*>(part + kk * a.D + d) =
+          v4f{fk[0] * a.scale, fk[1] * a.scale, fk[2] * a.scale, fk[3] * a.scale};
+      *reinterpret_cast<v4f*>(part + (kSinkKeys + kk) * a.D + d) =
+          *reinterpret_cast<const v4f*>(sv + kk * DP + d);
+    }
+    return;
+  }
+
+  const int k0 = (int)blockIdx.y * BM;
+  const RowRange rr(k0, a, seq);
+  const int key = k0 + wave * 32 + (l & 31);
+  kg.init(a, b, hk, key, key < seq.len);
+  if (rr.n0 < rr.n1) tile.load(a, seq, b, hk, rr.n0, rr.n1);
+  int buf = 0;
+  for (int t0 = rr.n0; t0 < rr.n1; t0 += BN, buf ^= 1) {
+    tile.store(Qs[buf], Gs[buf], Ls[buf], Ds[buf], Ps[buf]);
+    __syncthreads();
+    if (t0 + BN < rr.n1) tile.load(a, seq, b, hk, t0 + BN, rr.n1);
+#pragma unroll
+    for (int sub = 0; sub < BN / 32; ++sub) {
+      const int s0 = t0 + sub * 32;
+      int pmin, pmax;
+      const int cover = span(s0, s0 + 32 < rr.n1 ? s0 + 32 : rr.n1, a, seq, pmin, pmax)
+                            ? coverage(pmin, pmax, k0 + wave * 32, a.W, a.S) : 0;
+      if (cover != 0)
+        kg.rows(a, Qs[buf], Gs[buf], Ls[buf], Ds[buf], Ps[buf], sub * 32, key, cover);
+    }
+  }
+  if (a.far_chunks > 0 && key < a.S) {
+    float* part = sink_part(a, bh, key / kSinkKeys, 0) + key % kSinkKeys * a.D;
+    put<T, float, ND>(part, kg.dk, a.scale, false, a.D, h);
+    put<T, float, ND>(part + kSinkKeys * a.D, kg.dv, 1.f, false, a.D, h);
+  } else if (key < a.Tk) {
+    put<T, T, ND>(reinterpret_cast<T*>(a.dk) + b * a.dks[0] + hk * a.dks[1] + key * a.dks[2],
+                  kg.dk, a.scale, false, a.D, h);
+    put<T, T, ND>(reinterpret_cast<T*>(a.dv) + b * a.dvs[0] + hk * a.dvs[1] + key * a.dvs[2],
+                  kg.dv, 1.f, false, a.D, h);
+  }
 }
 
-// the shares of the sink blocks' keys, summed in order
+// the shares of the sinks' gradients, summed in order
 template <typename T>
 __global__ void __launch_bounds__(NT) join_kv_kernel(AttnArgs a) {
-  const int64_t D4 = a.D / 4;
-  const int64_t per = (int64_t)BM * D4;
+  const int D4 = a.D / 4;
   const int64_t id = (int64_t)blockIdx.x * NT + threadIdx.x;
-  if (id >= (int64_t)a.B * a.Hkv * a.sink_blocks * per) return;
-  const int64_t blk = id / per;                       // (b, head, sink block)
-  const int i = (int)(id % per / D4), d = (int)(id % D4) * 4;
-  const int64_t bh = blk / a.sink_blocks, b = bh / a.Hkv, hk = bh % a.Hkv;
-  const int64_t key = (blk % a.sink_blocks) * BM + i;
-  if (key >= a.Tk) return;
-  v4f fk = {0.f, 0.f, 0.f, 0.f}, fv = fk;
-  for (int ch = 0; ch <= a.far_chunks; ++ch) {
-    const float* part =
-        a.kvpart + (((blk * (1 + a.far_chunks) + ch) * 2) * BM + i) * (int64_t)a.D + d;
-    fk += *reinterpret_cast<const v4f*>(part);
-    fv += *reinterpret_cast<const v4f*>(part + (int64_t)BM * a.D);
-  }
-  *reinterpret_cast<typename Ops<T>::quad*>(reinterpret_cast<T*>(a.dk) + b * a.dks[0] +
-                                            hk * a.dks[1] + key * a.dks[2] + d) =
-      __builtin_convertvector(fk, typename Ops<T>::quad);
-  *reinterpret_cast<typename Ops<T>::quad*>(reinterpret_cast<T*>(a.dv) + b * a.dvs[0] +
-                                            hk * a.dvs[1] + key * a.dvs[2] + d) =
-      __builtin_convertvector(fv, typename Ops<T>::quad);
+  if (id >= (int64_t)a.B * a.Hkv * a.S * 2 * D4) return;
+  const int d = (int)(id % D4) * 4;
+  const int64_t rest = id / D4;
+  const int which = (int)(rest & 1), key = (int)((rest >> 1) % a.S);
+  const int bh = (int)((rest >> 1) / a.S), b = bh / a.Hkv, hk = bh - b * a.Hkv;
+  const float* part = sink_part(a, bh, key / kSinkKeys, 0) +
+                      (which * kSinkKeys + key % kSinkKeys) * a.D + d;
+  const int64_t step = (int64_t)2 * kSinkKeys * a.D;
+  v4f f = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int ch = 0; ch <= a.far_chunks; ++ch) f = add4(f, *reinterpret_cast<const v4f*>(part + ch * step));
+  T* out = which == 0
+               ? reinterpret_cast<T*>(a.dk) + b * a.dks[0] + hk * a.dks[1] + key * a.dks[2]
+               : reinterpret_cast<T*>(a.dv) + b * a.dvs[0] + hk * a.dvs[1] + key * a.dvs[2];
+  *reinterpret_cast<typename Ops<T>::quad*>(out + d) =
+      __builtin_convertvector(f, typename Ops<T>::quad);
 }
 
 unsigned row_blocks(const AttnArgs& a) {
@@ -772,8 +876,7 @@ void forward_dp(const AttnArgs& a, hipStream_t st) {
   const dim3 grid((unsigned)(a.B * a.Hkv), row_blocks(a), (unsigned)a.splits);
   if (a.splits > 1) {
     fwd_kernel<T, DP, true><<<grid, NT, 0, st>>>(a);
-    const int64_t n = (int64_t)a.B * a.Hq * a.Tq * (a.D / 4);
-    join_kernel<T><<<(unsigned)ceil_div(n, NT), NT, 0, st>>>(a);
+    join_kernel<T><<<(unsigned)(a.B * a.Hq * a.Tq), NT, 0, st>>>(a);
   } else {
     fwd_kernel<T, DP, false><<<grid, NT, 0, st>>>(a);
   }
@@ -784,9 +887,9 @@ void backward_dp(const AttnArgs& a, hipStream_t st) {
   const unsigned bh = (unsigned)(a.B * a.Hkv);
   dq_kernel<T, DP><<<dim3(bh, row_blocks(a)), NT, 0, st>>>(a);
   const int kb = (int)ceil_div(a.Tk, BM);
-  dkv_kernel<T, DP><<<dim3(bh, (unsigned)(kb + a.sink_blocks * a.far_chunks)), NT, 0, st>>>(a, kb);
+  dkv_kernel<T, DP><<<dim3(bh, (unsigned)(kb + a.sink_groups * a.far_chunks)), NT, 0, st>>>(a, kb);
   if (a.far_chunks > 0) {
-    const int64_t n = (int64_t)bh * a.sink_blocks * BM * (a.D / 4);
+    const int64_t n = (int64_t)bh * a.S * 2 * (a.D / 4);
     join_kv_kernel<T><<<(unsigned)ceil_div(n, NT), NT, 0, st>>>(a);
   }
 }
@@ -809,7 +912,7 @@ void backward_type(const AttnArgs& a, hipStream_t st) {
 
 }  // namespace
 
-void attn_plan(const AttnArgs& a, int, int* splits, int64_t* floats) {
+void attn_plan(const AttnArgs& a, int* splits, int64_t* floats) {
   const int64_t rows = (int64_t)a.Tq * a.G;
   const int64_t blocks = (int64_t)a.B * a.Hkv * ceil_div(rows, BM);
   // tiles that the longest row block can see
@@ -832,19 +935,19 @@ void attn_forward(int dtype, const AttnArgs& a, hipStream_t st) {
   else forward_type<float>(a, st);
 }
 
-void attn_bwd_plan(const AttnArgs& a, int, int* sink_blocks, int* far_chunks, int64_t* floats) {
-  *sink_blocks = *far_chunks = 0;
+void attn_bwd_plan(const AttnArgs& a, int* sink_groups, int* far_chunks, int64_t* floats) {
+  *sink_groups = *far_chunks = 0;
   *floats = 0;
   // far rows exist only behind the window of a sink's key
-  if (a.S <= 0 || a.W >= a.Tk || a.Tk == 0) return;
-  const int64_t sb = ceil_div(std::min<int64_t>(a.S, a.Tk), BM);
-  const int64_t tiles = ceil_div((int64_t)a.Tq * a.G, BN);
-  int64_t ch = ceil_div(tiles, 16);
-  if (ch > 64) ch = 64;
-  if (ch < 1) ch = 1;
-  *sink_blocks = (int)sb;
+  if (a.S <= 0 || a.W >= a.Tk) return;
+  const int64_t groups = ceil_div(a.S, kSinkKeys), bh = (int64_t)a.B * a.Hkv;
+  // chunks of at least two tiles until there are items for 4 blocks a CU
+  int64_t ch = ceil_div(1024, bh * groups);
+  ch = std::min(ch, ceil_div((int64_t)a.Tq * a.G, 2 * BM));
+  ch = std::max<int64_t>(1, std::min<int64_t>(ch, 32));
+  *sink_groups = (int)groups;
   *far_chunks = (int)ch;
-  *floats = (int64_t)a.B * a.Hkv * sb * (1 + ch) * 2 * BM * a.D;
+  *floats = bh * groups * (1 + ch) * 2 * kSinkKeys * a.D;
 }
 
 void attn_backward(int dtype, const AttnArgs& a, hipStream_t st) {
