@@ -48,9 +48,16 @@ bool rows16(const at::Tensor& t) {
   return true;
 }
 
-// t, or a copy whose rows can be read in 16-byte accesses
-at::Tensor readable(const at::Tensor& t) {
-  return rows16(t) ? t : t.clone(at::MemoryFormat::Contiguous);
+// An attention operand [B, H, T, D]: rows that 16-byte accesses can read, a
+// token's row no longer than the stride to the next (an expanded one is
+// not), and 64 rows of `group` heads within 2^31 bytes of the first, which
+// is what the kernels' 32-bit offsets reach.  Else a copy laid out
+// [B, T, H, D].
+at::Tensor operand(const at::Tensor& t, int64_t group) {
+  const int64_t reach = ((group - 1) * t.stride(1) + 64 * t.stride(2)) * (int64_t)t.element_size();
+  if (rows16(t) && (t.size(2) <= 1 || t.stride(2) >= t.size(3)) && reach < ((int64_t)1 << 31) - 1024)
+    return t;
+  return t.transpose(1, 2).clone(at::MemoryFormat::Contiguous).transpose(1, 2);
 }
 
 void strides3(const at::Tensor& t, int64_t* s) {  // batch, head, token of [B, H, T, D]
@@ -136,7 +143,7 @@ kfac::AttnArgs attn_args(const at::Tensor& q, const at::Tensor& k, const at::Ten
 }
 
 // out [B, Hq, Tq, D] over memory laid out [B, Tq, Hq, D] (what the output
-// projection reads), and lse [B, Hq, Tq] where a backward pass may follow
+// projection reads), and the rows' lse where a backward pass may follow
 std::tuple<at::Tensor, at::Tensor> attn_forward(const at::Tensor& q, const at::Tensor& k,
                                                 const at::Tensor& v, const OptTensor& lengths,
                                                 const OptTensor& starts, const AttnConf& c,
@@ -145,7 +152,7 @@ std::tuple<at::Tensor, at::Tensor> attn_forward(const at::Tensor& q, const at::T
   kfac::AttnArgs a = attn_args(q, k, v, lengths, starts, c);
   at::Tensor out = at::empty({a.B, a.Tq, a.Hq, a.D}, q.options()).transpose(1, 2);
   at::Tensor lse;
-  if (want_lse) lse = at::empty({a.B, a.Hq, a.Tq}, q.options().dtype(at::kFloat));
+  if (want_lse) lse = at::empty({a.B * a.Hkv, (int64_t)a.Tq * a.G}, q.options().dtype(at::kFloat));
   a.out = out.data_ptr();
   strides3(out, a.os);
   a.lse = want_lse ? lse.data_ptr<float>() : nullptr;
@@ -163,13 +170,20 @@ std::tuple<at::Tensor, at::Tensor> attn_forward(const at::Tensor& q, const at::T
   return {out, lse};
 }
 
+int64_t groups(const at::Tensor& q, const at::Tensor& k) {
+  TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && k.size(1) > 0,
+              "window_attention: q, k, v must be 4-D");
+  return q.size(1) / k.size(1);
+}
+
 struct WindowAttnFn : public torch::autograd::Function<WindowAttnFn> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& q_, const at::Tensor& k_,
                             const at::Tensor& v_, const OptTensor& lengths,
                             const OptTensor& starts, int64_t window, int64_t sinks, int64_t start,
                             bool start_given, double scale) {
     const AttnConf c{window, sinks, start, start_given, scale};
-    const at::Tensor q = readable(q_), k = readable(k_), v = readable(v_);
+    const int64_t G = groups(q_, k_);
+    const at::Tensor q = operand(q_, G), k = operand(k_, 1), v = operand(v_, 1);
     auto [out, lse] = attn_forward(q, k, v, lengths, starts, c, true);
     ctx->save_for_backward({q, k, v, out, lse, lengths.has_value() ? *lengths : at::Tensor(),
                             starts.has_value() ? *starts : at::Tensor()});
@@ -191,7 +205,7 @@ struct WindowAttnFn : public torch::autograd::Function<WindowAttnFn> {
     const OptTensor starts = sv[6].defined() ? OptTensor(sv[6]) : c10::nullopt;
     c10::hip::HIPGuardMasqueradingAsCUDA g(q.device());
     kfac::AttnArgs a = attn_args(q, k, v, lengths, starts, c);
-    const at::Tensor go = readable(grads[0]);
+    const at::Tensor go = operand(grads[0], a.G);
     at::Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v);
     if (a.Tq == 0 || q.numel() == 0) {
       dk.zero_();
@@ -235,7 +249,8 @@ at::Tensor window_attention(const at::Tensor& q, const at::Tensor& k, const at::
     return WindowAttnFn::apply(q, k, v, lengths, starts, window, sinks, start, start_given, scale);
   const AttnConf c{window, sinks, start, start_given, scale};
   return std::get<0>(
-      attn_forward(readable(q), readable(k), readable(v), lengths, starts, c, false));
+      attn_forward(operand(q, groups(q, k)), operand(k, 1), operand(v, 1), lengths, starts, c,
+                   false));
 }
 
 // -------------------------------------------------------------- rotary

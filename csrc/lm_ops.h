@@ -71,8 +71,8 @@ struct AttnArgs {
   int64_t dos[3];
   void* out;                    // [B, Hq, Tq, D] with strides os
   int64_t os[3];
-  float* lse;                   // [B, Hq, Tq], log2 units; +inf: sees nothing
-  float* delta;                 // [B, Hq, Tq]
+  float* lse;                   // [B * Hkv, Tq * G] (rows), log2 units; +inf: sees nothing
+  float* delta;                 // the same
   void *dq, *dk, *dv;
   int64_t dqs[3], dks[3], dvs[3];
   const int* lengths;           // [B] or null

@@ -53,8 +53,24 @@ typedef __attribute__((address_space(3))) v4i16 lds_v4i16;
 
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// x of lane l ^ 32
-__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
+// (x of lane l & 31, x of lane l | 32)
+__device__ __forceinline__ void halves(float x, float& lo, float& hi) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x),
+                                                  __builtin_bit_cast(uint32_t, x), false, false);
+  const uint32_t a = r[0], b = r[1];
+  lo = __uint_as_float(a);
+  hi = __uint_as_float(b);
+}
+__device__ __forceinline__ float halves_sum(float x) {
+  float lo, hi;
+  halves(x, lo, hi);
+  return lo + hi;
+}
+__device__ __forceinline__ float halves_max(float x) {
+  float lo, hi;
+  halves(x, lo, hi);
+  return fmaxf(lo, hi);
+}
 
 template <typename T> struct Ops;
 template <> struct Ops<__bf16> {
@@ -83,9 +99,21 @@ template <> struct Ops<float> {
 
 template <typename T> constexpr int kUnit = 16 / (int)sizeof(T);  // elements of 16 bytes
 
-// LDS row stride: rows 16 bytes past a multiple of 256 (or of 128) keep the
-// 16-byte row reads of neighbouring rows on different banks
-template <typename T, int DP> constexpr int kLd = DP + kUnit<T>;
+// An LDS tile is BN rows of CR 16-byte chunks (a power of two), chunk c of
+// row r at place c ^ place_of(r).  Row reads (16 bytes of 32 rows) and
+// transposed reads (64 bytes of 4 rows) then both meet every bank once; a
+// padded row stride can serve only one of the two.
+template <typename T, int DP> constexpr int kChunks = DP * (int)sizeof(T) <= 64 ? 4
+                                                   : DP * (int)sizeof(T) <= 128 ? 8
+                                                   : DP * (int)sizeof(T) <= 256 ? 16 : 32;
+template <typename T, int DP> constexpr int kLd = kChunks<T, DP> * kUnit<T>;  // elements of a row
+
+template <int CR>
+__device__ __forceinline__ int place_of(int r) {
+  if constexpr (CR >= 16) return ((r & 3) << 2) | ((r >> 2) & 3);
+  else if constexpr (CR == 8) return ((r & 2) << 1) | ((r >> 2) & 3);
+  else return (r >> 2) & 3;
+}
 
 // waves a SIMD that the row kernels and the key-gradient kernel leave
 // registers for (256 a wave at 2, 512 at 1)
@@ -111,19 +139,19 @@ __device__ __forceinline__ v16f zero16() {
 }
 
 // Left operand from rows: lane l holds row r0 + (l & 31), elements
-// k0 + 8 (l >> 5) .. + 7 of a row-major LDS tile
+// 16 k + 8 (l >> 5) .. + 7 (r0 a multiple of 16)
 template <typename T, int DP>
-__device__ __forceinline__ typename Ops<T>::frag row_frag(const T* L, int r0, int k0) {
-  const int l = threadIdx.x & 63;
-  const T* p = L + (r0 + (l & 31)) * kLd<T, DP> + k0 + 8 * (l >> 5);
-  typename Ops<T>::frag f;
+__device__ __forceinline__ typename Ops<T>::frag row_frag(const T* L, int r0, int k) {
+  const int l = threadIdx.x & 63, f = place_of<kChunks<T, DP>>(l & 31);
+  const T* p = L + (r0 + (l & 31)) * kLd<T, DP>;
   if constexpr (sizeof(T) == 2) {
-    f = *reinterpret_cast<const typename Ops<T>::frag*>(p);
+    return *reinterpret_cast<const typename Ops<T>::frag*>(p + ((2 * k + (l >> 5)) ^ f) * 8);
   } else {
-    const v4f a = *reinterpret_cast<const v4f*>(p), b = *reinterpret_cast<const v4f*>(p + 4);
-    f = v8f{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    const int c = 4 * k + 2 * (l >> 5);
+    const v4f a = *reinterpret_cast<const v4f*>(p + (c ^ f) * 4);
+    const v4f b = *reinterpret_cast<const v4f*>(p + ((c + 1) ^ f) * 4);
+    return v8f{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
   }
-  return f;
 }
 
 // Left operand from columns: lane l holds column c0 + (l & 31) of tile rows
@@ -131,23 +159,26 @@ __device__ __forceinline__ typename Ops<T>::frag row_frag(const T* L, int r0, in
 // 8s .. 8s + 7 of an accumulator hold its rows (r0 = 16 s)
 template <typename T, int DP>
 __device__ __forceinline__ typename Ops<T>::frag col_frag(const T* L, int r0, int c0) {
+  constexpr int CR = kChunks<T, DP>, LD = kLd<T, DP>;
   const int l = threadIdx.x & 63;
   if constexpr (sizeof(T) == 2) {
     // ds_read_b64_tr_b16: 16 lanes read 4 rows x 16 columns (lane 4q + p row
     // q, columns 4p ..) and get a column's 4 rows each
-    const int i = l & 15, g = l >> 4;
-    const T* p = L + (r0 + 4 * (g >> 1) + (i >> 2)) * kLd<T, DP> + c0 + 16 * (g & 1) + 4 * (i & 3);
-    const v4i16 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)p);
-    const v4i16 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(p + 8 * kLd<T, DP>));
+    const int i = l & 15, g = l >> 4, r = 4 * (g >> 1) + (i >> 2);
+    const int c = c0 / 8 + 2 * (g & 1) + ((i & 3) >> 1);
+    const T* lp = L + (r0 + r) * LD + (c ^ place_of<CR>(r)) * 8 + 4 * (i & 1);
+    const T* hp = L + (r0 + r + 8) * LD + (c ^ place_of<CR>(r + 8)) * 8 + 4 * (i & 1);
+    const v4i16 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)lp);
+    const v4i16 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)hp);
     const v8i16 f = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     return __builtin_bit_cast(typename Ops<T>::frag, f);
   } else {
-    const T* p = L + (r0 + 4 * (l >> 5)) * kLd<T, DP> + c0 + (l & 31);
+    const int c = (c0 + (l & 31)) / 4, r = 4 * (l >> 5);
     v8f f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[i] = p[i * kLd<T, DP>];
-      f[4 + i] = p[(8 + i) * kLd<T, DP>];
+    for (int i = 0; i < 8; ++i) {
+      const int rr = r + (i & 3) + 8 * (i >> 2);
+      f[i] = L[(r0 + rr) * LD + (c ^ place_of<CR>(rr)) * 4 + (l & 3)];
     }
     return f;
   }
@@ -184,34 +215,42 @@ __device__ __forceinline__ typename Ops<T>::frag global_frag(const T* row, int d
   return f;
 }
 
-// a BN-row tile on its way from global memory through registers into LDS
-template <typename T, int DP>
-struct Tile {
-  static constexpr int CR = DP / kUnit<T>;          // 16-byte chunks of a row
-  static constexpr int CH = BN * CR / NT;           // chunks a thread
-  static_assert(BN * CR % NT == 0, "tile");
-  uint4 r[CH];
+constexpr uint32_t kNowhere = 0x80000000u;  // an offset that no buffer reaches: reads 0
 
-  // row_ptr(i): row i's address, or null where it is to be zeros
-  template <typename F>
-  __device__ __forceinline__ void load(F row_ptr, int D) {
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      const int id = threadIdx.x + c * NT;
-      const int d = (id % CR) * kUnit<T>;
-      const T* p = row_ptr(id / CR);
-      r[c] = p != nullptr && d < D ? *reinterpret_cast<const uint4*>(p + d)
-                                   : make_uint4(0, 0, 0, 0);
-    }
+// One wave's share of a BN-row tile, straight from global memory into LDS
+// (16 bytes a lane, no registers in between).  The places in LDS follow the
+// lanes; which chunk belongs there is in the offsets, which a tile of rows
+// at a constant stride keeps for its whole life.  Offsets behind the
+// buffer's last byte read zeros.
+template <typename T, int DP>
+struct Dma {
+  static constexpr int CR = kChunks<T, DP>, CH = BN * CR / NT;
+  __device__ __forceinline__ static int row(int n) { return (n * NT + (int)threadIdx.x) / CR; }
+  __device__ __forceinline__ static int chunk(int n) {
+    return ((n * NT + (int)threadIdx.x) % CR) ^ place_of<CR>(row(n));
   }
-  __device__ __forceinline__ void store(T* L) const {
+  // byte offset of this lane's chunk n in a row at `at` bytes
+  __device__ __forceinline__ static uint32_t offset(int n, uint32_t at, int D) {
+    return chunk(n) * kUnit<T> < D ? at + chunk(n) * 16 : kNowhere;
+  }
+  template <typename F>
+  __device__ __forceinline__ static void run(T* L, const T* base, uint32_t bytes, int wave,
+                                             F offset_of) {
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<T*>(base), (short)0, (int)bytes, 0x00020000);
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      const int id = threadIdx.x + c * NT;
-      *reinterpret_cast<uint4*>(L + (id / CR) * kLd<T, DP> + (id % CR) * kUnit<T>) = r[c];
-    }
+    for (int n = 0; n < CH; ++n)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rs, (__attribute__((address_space(3))) void*)(L + (n * NT + wave * 64) * kUnit<T>), 16,
+          offset_of(n), 0, 0, 0);
   }
 };
+
+// this wave's loads into LDS have arrived, then everybody's
+__device__ __forceinline__ void arrived() {
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  __syncthreads();
+}
 
 struct Seq {
   int len, start;
@@ -334,7 +373,7 @@ struct RowBlock {
     const int rows = a.Tq * a.G;
     r0 = (int)(gridDim.y - 1 - blockIdx.y) * BM;  // longest rows first
     const int l = threadIdx.x & 63;
-    wave = threadIdx.x >> 6;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     h = l >> 5;
     seq = sequence(a, b);
     r = r0 + wave * 32 + (l & 31);
@@ -358,13 +397,72 @@ struct RowBlock {
   }
 };
 
+// The K and V tiles of a row block, one after the other.
+template <typename T, int DP>
+struct KeyStream {
+  typedef Dma<T, DP> D;
+  const T *k, *v;
+  uint32_t ko[D::CH], vo[D::CH];
+  int64_t ks, vs;
+  int wave;
+  __device__ __forceinline__ KeyStream(const AttnArgs& a, const RowBlock& w) {
+    k = reinterpret_cast<const T*>(a.k) + w.b * a.ks[0] + w.hk * a.ks[1];
+    v = reinterpret_cast<const T*>(a.v) + w.b * a.vs[0] + w.hk * a.vs[1];
+    ks = a.ks[2];
+    vs = a.vs[2];
+    wave = w.wave;
+#pragma unroll
+    for (int n = 0; n < D::CH; ++n) {
+      ko[n] = D::offset(n, D::row(n) * (uint32_t)(ks * sizeof(T)), a.D);
+      vo[n] = D::offset(n, D::row(n) * (uint32_t)(vs * sizeof(T)), a.D);
+    }
+  }
+  // keys behind kt.hi, and those before the window that are no sinks, read
+  // as zeros: nobody sees them, and they may hold anything
+  __device__ __forceinline__ void fetch(const AttnArgs& a, const KeyTiles& kt, int j0, T* K,
+                                        T* V) const {
+    const int n = kt.hi - j0 < BN ? kt.hi - j0 : BN;
+    const uint32_t kb = (uint32_t)(((n - 1) * ks + a.D) * sizeof(T));
+    const uint32_t vb = (uint32_t)(((n - 1) * vs + a.D) * sizeof(T));
+    if (j0 >= kt.lo) {
+      D::run(K, k + j0 * ks, kb, wave, [&](int i) { return ko[i]; });
+      D::run(V, v + j0 * vs, vb, wave, [&](int i) { return vo[i]; });
+    } else {
+      auto seen = [&](int i) { return j0 + D::row(i) >= kt.lo || j0 + D::row(i) < a.S; };
+      D::run(K, k + j0 * ks, kb, wave, [&](int i) { return seen(i) ? ko[i] : kNowhere; });
+      D::run(V, v + j0 * vs, vb, wave, [&](int i) { return seen(i) ? vo[i] : kNowhere; });
+    }
+  }
+};
+
+// Runs step(K tile, V tile, first key) over key tiles [it0, it1), the next
+// tile on its way while one is worked on.  Two buffers that the compiler can
+// tell apart: it would otherwise wait for the loads before every LDS read.
+template <typename T, int DP, typename F>
+__device__ __forceinline__ void stream_keys(const AttnArgs& a, const RowBlock& w,
+                                            const KeyTiles& kt, int it0, int it1, F step) {
+  __shared__ __attribute__((aligned(16))) T K0[BN * kLd<T, DP>];
+  __shared__ __attribute__((aligned(16))) T K1[BN * kLd<T, DP>];
+  __shared__ __attribute__((aligned(16))) T V0[BN * kLd<T, DP>];
+  __shared__ __attribute__((aligned(16))) T V1[BN * kLd<T, DP>];
+  const KeyStream<T, DP> ks(a, w);
+  if (it0 < it1) ks.fetch(a, kt, kt.key0(it0), K0, V0);
+  for (int it = it0; it < it1; it += 2) {
+    arrived();
+    if (it + 1 < it1) ks.fetch(a, kt, kt.key0(it + 1), K1, V1);
+    step(K0, V0, kt.key0(it));
+    if (it + 1 >= it1) break;
+    arrived();
+    if (it + 2 < it1) ks.fetch(a, kt, kt.key0(it + 2), K0, V0);
+    step(K1, V1, kt.key0(it + 1));
+  }
+}
+
 // ---------------------------------------------------------------- forward
 template <typename T, int DP, bool SPLIT>
 __global__ void __launch_bounds__(NT, (kRowWaves<T, DP>)) fwd_kernel(AttnArgs a) {
-  constexpr int KD = DP / 16, ND = DP / 32, LD = kLd<T, DP>;
+  constexpr int KD = DP / 16, ND = DP / 32;
   typedef typename Ops<T>::frag frag;
-  __shared__ __attribute__((aligned(16))) T Ks[2][BN * LD];
-  __shared__ __attribute__((aligned(16))) T Vs[2][BN * LD];
   RowBlock w(a);
   const KeyTiles kt = w.keys(a);
   const int h = w.h;
@@ -386,23 +484,7 @@ __global__ void __launch_bounds__(NT, (kRowWaves<T, DP>)) fwd_kernel(AttnArgs a)
   for (int d = 0; d < ND; ++d) o[d] = zero16();
   float m = -kInf, sum = 0.f;
 
-  const T* kb = reinterpret_cast<const T*>(a.k) + w.b * a.ks[0] + w.hk * a.ks[1];
-  const T* vb = reinterpret_cast<const T*>(a.v) + w.b * a.vs[0] + w.hk * a.vs[1];
-  Tile<T, DP> tk, tv;
-  auto fetch = [&](int it) {
-    const int j0 = kt.key0(it);
-    auto ok = [&](int i) { return j0 + i < kt.hi && (j0 + i >= kt.lo || j0 + i < a.S); };
-    tk.load([&](int i) { return ok(i) ? kb + (int64_t)(j0 + i) * a.ks[2] : nullptr; }, a.D);
-    tv.load([&](int i) { return ok(i) ? vb + (int64_t)(j0 + i) * a.vs[2] : nullptr; }, a.D);
-  };
-  if (it0 < it1) fetch(it0);
-  for (int it = it0; it < it1; ++it) {
-    const int buf = (it - it0) & 1;
-    tk.store(Ks[buf]);
-    tv.store(Vs[buf]);
-    __syncthreads();
-    if (it + 1 < it1) fetch(it + 1);
-    const int j0 = kt.key0(it);
+  stream_keys<T, DP>(a, w, kt, it0, it1, [&](const T* K, const T* V, int j0) {
 #pragma unroll
     for (int sub = 0; sub < BN / 32; ++sub) {
       const int js = j0 + sub * 32;
@@ -410,40 +492,43 @@ __global__ void __launch_bounds__(NT, (kRowWaves<T, DP>)) fwd_kernel(AttnArgs a)
       if (cover == 0) continue;
       v16f s = zero16();
 #pragma unroll
-      for (int k = 0; k < KD; ++k)
-        s = Ops<T>::mma(row_frag<T, DP>(Ks[buf], sub * 32, k * 16), qf[k], s);
+      for (int k = 0; k < KD; ++k) s = Ops<T>::mma(row_frag<T, DP>(K, sub * 32, k), qf[k], s);
       if (cover == 1) hide<true>(s, w.p, nullptr, js, h, a.W, a.S);
       float mx = s[0];
 #pragma unroll
       for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
       // c > 0: the maximum of the products is the product of the maximum
-      mx = fmaxf(mx, other_half(mx)) * c;
-      const float mn = fmaxf(m, mx);
-      const float base = mn == -kInf ? 0.f : mn;
-      const float alpha = ex2(m - base);
-      m = mn;
+      mx = halves_max(mx) * c;
+      // the accumulators are rescaled only where a row's maximum grew
+      if (__any(mx > m)) {
+        const float mn = fmaxf(m, mx);
+        const float alpha = ex2(m - (mn == -kInf ? 0.f : mn));
+        m = mn;
+        sum *= alpha;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
+      }
+      const float base = m == -kInf ? 0.f : m;
       float add = 0.f;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         s[e] = ex2(__builtin_fmaf(s[e], c, -base));
         add += s[e];
       }
-      sum = sum * alpha + add;
-#pragma unroll
-      for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
+      sum += add;
 #pragma unroll
       for (int ss = 0; ss < 2; ++ss) {
         const frag pf = acc_frag<T>(s, ss);
 #pragma unroll
         for (int d = 0; d < ND; ++d)
-          o[d] = Ops<T>::mma(col_frag<T, DP>(Vs[buf], sub * 32 + ss * 16, d * 32), pf, o[d]);
+          o[d] = Ops<T>::mma(col_frag<T, DP>(V, sub * 32 + ss * 16, d * 32), pf, o[d]);
       }
     }
-  }
+  });
 
-  sum += other_half(sum);
+  sum = halves_sum(sum);
   const bool none = w.p < 0 || sum == 0.f;
   const float inv = none ? 0.f : 1.f / sum;
   const float lse = none ? kInf : m + log2f(sum);
@@ -454,7 +539,7 @@ __global__ void __launch_bounds__(NT, (kRowWaves<T, DP>)) fwd_kernel(AttnArgs a)
     put<T, float, ND>(a.opart + at * a.D, o, inv, none, a.D, h);
     return;
   }
-  if (h == 0 && a.lse != nullptr) a.lse[((int64_t)w.b * a.Hq + w.head) * a.Tq + w.t] = lse;
+  if (h == 0 && a.lse != nullptr) a.lse[(int64_t)w.bh * (a.Tq * a.G) + w.r] = lse;
   put<T, T, ND>(reinterpret_cast<T*>(a.out) + w.b * a.os[0] + w.head * a.os[1] + w.t * a.os[2], o,
                 inv, none, a.D, h);
 }
@@ -519,7 +604,7 @@ __global__ void __launch_bounds__(NT) join_kernel(AttnArgs a) {
                                               head * a.os[1] + rw.t * a.os[2] + d) =
         __builtin_convertvector(o, typename Ops<T>::quad);
   if (tid == 0 && a.lse != nullptr)
-    a.lse[((int64_t)b * a.Hq + head) * a.Tq + rw.t] = sum == 0.f ? kInf : base + log2f(sum);
+    a.lse[row] = sum == 0.f ? kInf : base + log2f(sum);
 }
 
 // --------------------------------------------------------------- backward
@@ -528,13 +613,11 @@ __global__ void __launch_bounds__(NT) join_kernel(AttnArgs a) {
 // dQ^T += K^T dS^T.
 template <typename T, int DP>
 __global__ void __launch_bounds__(NT, (kRowWaves<T, DP>)) dq_kernel(AttnArgs a) {
-  constexpr int KD = DP / 16, ND = DP / 32, LD = kLd<T, DP>;
+  constexpr int KD = DP / 16, ND = DP / 32;
   typedef typename Ops<T>::frag frag;
-  __shared__ __attribute__((aligned(16))) T Ks[2][BN * LD];
-  __shared__ __attribute__((aligned(16))) T Vs[2][BN * LD];
   RowBlock w(a);
   const KeyTiles kt = w.keys(a);
-  const int h = w.h, it1 = w.tiles;
+  const int h = w.h;
   const float c = a.scale * kLog2e;
 
   const T* q = reinterpret_cast<const T*>(a.q) + w.b * a.qs[0] + w.head * a.qs[1] + w.t * a.qs[2];
@@ -551,31 +634,15 @@ __global__ void __launch_bounds__(NT, (kRowWaves<T, DP>)) dq_kernel(AttnArgs a) 
 #pragma unroll
     for (int i = 0; i < 8; ++i) delta += (float)gf[k][i] * (float)of[i];
   }
-  delta += other_half(delta);
-  const int64_t at = ((int64_t)w.b * a.Hq + w.head) * a.Tq + w.t;
+  delta = halves_sum(delta);
+  const int64_t at = (int64_t)w.bh * (a.Tq * a.G) + w.r;
   if (w.live && h == 0) a.delta[at] = delta;
   const float lse = w.p >= 0 ? a.lse[at] : kInf;
 
   v16f dq[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) dq[d] = zero16();
-  const T* kb = reinterpret_cast<const T*>(a.k) + w.b * a.ks[0] + w.hk * a.ks[1];
-  const T* vb = reinterpret_cast<const T*>(a.v) + w.b * a.vs[0] + w.hk * a.vs[1];
-  Tile<T, DP> tk, tv;
-  auto fetch = [&](int it) {
-    const int j0 = kt.key0(it);
-    auto ok = [&](int i) { return j0 + i < kt.hi && (j0 + i >= kt.lo || j0 + i < a.S); };
-    tk.load([&](int i) { return ok(i) ? kb + (int64_t)(j0 + i) * a.ks[2] : nullptr; }, a.D);
-    tv.load([&](int i) { return ok(i) ? vb + (int64_t)(j0 + i) * a.vs[2] : nullptr; }, a.D);
-  };
-  if (it1 > 0) fetch(0);
-  for (int it = 0; it < it1; ++it) {
-    const int buf = it & 1;
-    tk.store(Ks[buf]);
-    tv.store(Vs[buf]);
-    __syncthreads();
-    if (it + 1 < it1) fetch(it + 1);
-    const int j0 = kt.key0(it);
+  stream_keys<T, DP>(a, w, kt, 0, w.tiles, [&](const T* K, const T* V, int j0) {
 #pragma unroll
     for (int sub = 0; sub < BN / 32; ++sub) {
       const int js = j0 + sub * 32;
@@ -584,8 +651,8 @@ __global__ void __launch_bounds__(NT, (kRowWaves<T, DP>)) dq_kernel(AttnArgs a) 
       v16f s = zero16(), dp = zero16();
 #pragma unroll
       for (int k = 0; k < KD; ++k) {
-        s = Ops<T>::mma(row_frag<T, DP>(Ks[buf], sub * 32, k * 16), qf[k], s);
-        dp = Ops<T>::mma(row_frag<T, DP>(Vs[buf], sub * 32, k * 16), gf[k], dp);
+        s = Ops<T>::mma(row_frag<T, DP>(K, sub * 32, k), qf[k], s);
+        dp = Ops<T>::mma(row_frag<T, DP>(V, sub * 32, k), gf[k], dp);
       }
       if (cover == 1) hide<true>(s, w.p, nullptr, js, h, a.W, a.S);
 #pragma unroll
@@ -595,10 +662,10 @@ __global__ void __launch_bounds__(NT, (kRowWaves<T, DP>)) dq_kernel(AttnArgs a) 
         const frag sf = acc_frag<T>(s, ss);
 #pragma unroll
         for (int d = 0; d < ND; ++d)
-          dq[d] = Ops<T>::mma(col_frag<T, DP>(Ks[buf], sub * 32 + ss * 16, d * 32), sf, dq[d]);
+          dq[d] = Ops<T>::mma(col_frag<T, DP>(K, sub * 32 + ss * 16, d * 32), sf, dq[d]);
       }
     }
-  }
+  });
   if (!w.live) return;
   put<T, T, ND>(reinterpret_cast<T*>(a.dq) + w.b * a.dqs[0] + w.head * a.dqs[1] + w.t * a.dqs[2],
                 dq, a.scale, w.p < 0, a.D, h);
@@ -633,45 +700,72 @@ __device__ __forceinline__ float* sink_part(const AttnArgs& a, int bh, int group
                         kSinkKeys * a.D;
 }
 
-// 64 rows of q and do, and their statistics
+// 64 rows of q and do with their statistics, and the positions of the rows
+template <typename T>
+struct RowBuf {
+  T *q, *g;
+  float *lse, *delta;
+  int* p;
+};
+
 template <typename T, int DP>
-struct RowTile {
-  Tile<T, DP> q, g;
-  float lse, delta;
-  int p;
-  __device__ __forceinline__ void load(const AttnArgs& a, const Seq& seq, int b, int hk, int t0,
-                                       int end) {
-    const T* qb = reinterpret_cast<const T*>(a.q) + b * a.qs[0] + hk * a.G * a.qs[1];
-    const T* gb = reinterpret_cast<const T*>(a.dout) + b * a.dos[0] + hk * a.G * a.dos[1];
-    q.load([&](int i) {
-      const Row r(t0 + i, a);
-      return t0 + i < end ? qb + r.g * a.qs[1] + r.t * a.qs[2] : nullptr;
-    }, a.D);
-    g.load([&](int i) {
-      const Row r(t0 + i, a);
-      return t0 + i < end ? gb + r.g * a.dos[1] + r.t * a.dos[2] : nullptr;
-    }, a.D);
-    if (threadIdx.x < BN) {
-      const int r = t0 + threadIdx.x;
-      const Row rw(r, a);
-      // rows outside the sequence have lse = +inf: P = 0
-      p = r < end ? position(rw.t, seq) : -1;
-      lse = kInf;
-      delta = 0.f;
-      if (p >= 0) {
-        const int64_t at = ((int64_t)b * a.Hq + hk * a.G + rw.g) * a.Tq + rw.t;
-        lse = a.lse[at];
-        delta = a.delta[at];
-      }
+struct RowStream {
+  typedef Dma<T, DP> D;
+  const T *q, *g;
+  const float *lse, *delta;
+  uint32_t qo[D::CH], go[D::CH];
+  int wave, start;
+  bool repeats;  // every tile begins with a token's first head
+  __device__ __forceinline__ RowStream(const AttnArgs& a, const Seq& seq, int b, int hk, int wv) {
+    wave = wv;
+    start = seq.start;
+    q = reinterpret_cast<const T*>(a.q) + b * a.qs[0] + hk * a.G * a.qs[1];
+    g = reinterpret_cast<const T*>(a.dout) + b * a.dos[0] + hk * a.G * a.dos[1];
+    const int64_t at = ((int64_t)b * a.Hkv + hk) * (a.Tq * a.G);
+    lse = a.lse + at;
+    delta = a.delta + at;
+    repeats = BN % a.G == 0;
+    if (repeats) offsets(a, 0, BN, qo, go);
+  }
+  // of the tile's rows r0 .. r0 + BN - 1, from r0's token on
+  __device__ __forceinline__ void offsets(const AttnArgs& a, int r0, int count, uint32_t (&x)[D::CH],
+                                          uint32_t (&y)[D::CH]) const {
+    const int t0 = Row(r0, a).t;
+#pragma unroll
+    for (int n = 0; n < D::CH; ++n) {
+      const Row r(r0 + D::row(n), a);
+      const bool in = D::row(n) < count;
+      x[n] = in ? D::offset(n, (uint32_t)((r.g * a.qs[1] + (r.t - t0) * a.qs[2]) * sizeof(T)), a.D)
+                : kNowhere;
+      y[n] = in ? D::offset(n, (uint32_t)((r.g * a.dos[1] + (r.t - t0) * a.dos[2]) * sizeof(T)), a.D)
+                : kNowhere;
     }
   }
-  __device__ __forceinline__ void store(T* Q, T* G, float* L, float* D, int* P) const {
-    q.store(Q);
-    g.store(G);
-    if (threadIdx.x < BN) {
-      L[threadIdx.x] = lse;
-      D[threadIdx.x] = delta;
-      P[threadIdx.x] = p;
+  // rows [r0, r0 + BN) that lie before `end`; the others read as zeros (q
+  // and do of 0 add nothing, whatever the statistics)
+  __device__ __forceinline__ void fetch(const AttnArgs& a, int r0, int end, const RowBuf<T>& to) const {
+    const int count = end - r0 < BN ? end - r0 : BN;
+    const int t0 = Row(r0, a).t;
+    const T *qb = q + t0 * a.qs[2], *gb = g + t0 * a.dos[2];
+    if (repeats && count == BN) {
+      D::run(to.q, qb, kNowhere - 1, wave, [&](int n) { return qo[n]; });
+      D::run(to.g, gb, kNowhere - 1, wave, [&](int n) { return go[n]; });
+    } else {
+      uint32_t x[D::CH], y[D::CH];
+      offsets(a, r0, count, x, y);
+      D::run(to.q, qb, kNowhere - 1, wave, [&](int n) { return x[n]; });
+      D::run(to.g, gb, kNowhere - 1, wave, [&](int n) { return y[n]; });
+    }
+    const int l = threadIdx.x & 63;
+    if (wave < 2) {
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<float*>((wave == 0 ? lse : delta) + r0), (short)0, (count > 0 ? count : 0) * 4,
+          0x00020000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rs, (__attribute__((address_space(3))) void*)(wave == 0 ? to.lse : to.delta), 4, l * 4,
+          0, 0, 0);
+    } else if (wave == 2) {
+      to.p[l] = Row(r0 + l, a).t + start;
     }
   }
 };
@@ -700,21 +794,21 @@ struct KeyGrad {
   }
 
   // 32 rows from tile row i0 on
-  __device__ __forceinline__ void rows(const AttnArgs& a, const T* Q, const T* G, const float* L,
-                                       const float* D, const int* P, int i0, int key, int cover) {
+  __device__ __forceinline__ void rows(const AttnArgs& a, const RowBuf<T>& b, int i0, int key,
+                                       int cover) {
     const int h = (threadIdx.x & 63) >> 5;
     const float c = a.scale * kLog2e;
     v16f s = zero16(), dp = zero16();
 #pragma unroll
     for (int k = 0; k < KD; ++k) {
-      s = Ops<T>::mma(row_frag<T, DP>(Q, i0, k * 16), kf[k], s);
-      dp = Ops<T>::mma(row_frag<T, DP>(G, i0, k * 16), vf[k], dp);
+      s = Ops<T>::mma(row_frag<T, DP>(b.q, i0, k), kf[k], s);
+      dp = Ops<T>::mma(row_frag<T, DP>(b.g, i0, k), vf[k], dp);
     }
-    if (cover == 1) hide<false>(s, key, P + i0, 0, h, a.W, a.S);
+    if (cover == 1) hide<false>(s, key, b.p + i0, 0, h, a.W, a.S);
 #pragma unroll
     for (int e4 = 0; e4 < 4; ++e4) {
-      const v4f le = *reinterpret_cast<const v4f*>(L + i0 + acc_row(e4 * 4, h));
-      const v4f de = *reinterpret_cast<const v4f*>(D + i0 + acc_row(e4 * 4, h));
+      const v4f le = *reinterpret_cast<const v4f*>(b.lse + i0 + acc_row(e4 * 4, h));
+      const v4f de = *reinterpret_cast<const v4f*>(b.delta + i0 + acc_row(e4 * 4, h));
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int e = e4 * 4 + i;
@@ -727,8 +821,8 @@ struct KeyGrad {
       const frag pf = acc_frag<T>(s, ss), sf = acc_frag<T>(dp, ss);
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
-        dv[d] = Ops<T>::mma(col_frag<T, DP>(G, i0 + ss * 16, d * 32), pf, dv[d]);
-        dk[d] = Ops<T>::mma(col_frag<T, DP>(Q, i0 + ss * 16, d * 32), sf, dk[d]);
+        dv[d] = Ops<T>::mma(col_frag<T, DP>(b.g, i0 + ss * 16, d * 32), pf, dv[d]);
+        dk[d] = Ops<T>::mma(col_frag<T, DP>(b.q, i0 + ss * 16, d * 32), sf, dk[d]);
       }
     }
   }
@@ -742,15 +836,19 @@ struct KeyGrad {
 template <typename T, int DP>
 __global__ void __launch_bounds__(NT, (kKeyWaves<T, DP>)) dkv_kernel(AttnArgs a, int key_blocks) {
   constexpr int ND = DP / 32, LD = kLd<T, DP>;
-  __shared__ __attribute__((aligned(16))) T Qs[2][BN * LD];
-  __shared__ __attribute__((aligned(16))) T Gs[2][BN * LD];
-  __shared__ __attribute__((aligned(16))) float Ls[2][BN], Ds[2][BN];
-  __shared__ int Ps[2][BN];
-  static_assert(2 * BN * LD * sizeof(T) >= kSinkKeys * DP * sizeof(float), "sums of a far item");
+  __shared__ __attribute__((aligned(16))) T Q0[BN * LD];
+  __shared__ __attribute__((aligned(16))) T Q1[BN * LD];
+  __shared__ __attribute__((aligned(16))) T G0[BN * LD];
+  __shared__ __attribute__((aligned(16))) T G1[BN * LD];
+  __shared__ __attribute__((aligned(16))) float L0[BN], L1[BN], D0[BN], D1[BN];
+  __shared__ int P0[BN], P1[BN];
+  static_assert(BN * LD * sizeof(T) >= kSinkKeys * DP * sizeof(float), "sums of a far item");
+  const RowBuf<T> b0{Q0, G0, L0, D0, P0}, b1{Q1, G1, L1, D1, P1};
   const int bh = blockIdx.x, b = bh / a.Hkv, hk = bh - b * a.Hkv;
-  const int l = threadIdx.x & 63, wave = threadIdx.x >> 6, h = l >> 5;
+  const int l = threadIdx.x & 63, h = l >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Seq seq = sequence(a, b);
-  RowTile<T, DP> tile;
+  const RowStream<T, DP> rs(a, seq, b, hk, wave);
   KeyGrad<T, DP> kg;
 
   if ((int)blockIdx.y >= key_blocks) {
@@ -758,28 +856,24 @@ __global__ void __launch_bounds__(NT, (kKeyWaves<T, DP>)) dkv_kernel(AttnArgs a,
     const int group = item / a.far_chunks, chunk = item - group * a.far_chunks;
     const int j0 = group * kSinkKeys, key = j0 + (l & 31);
     const RowRange rr(j0 / BM * BM, a, seq);
-    const int tiles = (rr.f1 - rr.n1 + BM - 1) / BM;
-    const int per = (tiles + a.far_chunks - 1) / a.far_chunks;
-    int ra = rr.n1 + per * chunk * BM, rb = ra + per * BM;
-    if (rb > rr.f1) rb = rr.f1;
+    const int tokens = (rr.f1 - rr.n1) / a.G;
+    const int per = (tokens + a.far_chunks - 1) / a.far_chunks * a.G;
+    const int ra = rr.n1 + per * chunk < rr.f1 ? rr.n1 + per * chunk : rr.f1;
+    const int rb = ra + per < rr.f1 ? ra + per : rr.f1;
     kg.init(a, b, hk, key, key < seq.len);
     for (int t0 = ra; t0 < rb; t0 += BM) {
       __syncthreads();
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        tile.load(a, seq, b, hk, t0 + half * BN, rb);
-        tile.store(Qs[half], Gs[half], Ls[half], Ds[half], Ps[half]);
-      }
-      __syncthreads();
+      rs.fetch(a, t0, rb, b0);
+      rs.fetch(a, t0 + BN, rb, b1);
+      arrived();
       const int s0 = t0 + wave * 32;
       int pmin, pmax;
       const int cover = span(s0, s0 + 32 < rb ? s0 + 32 : rb, a, seq, pmin, pmax)
                             ? coverage(pmin, pmax, j0, a.W, a.S) : 0;
-      if (cover != 0)
-        kg.rows(a, Qs[0], Gs[0], Ls[0], Ds[0], Ps[0], wave * 32, key, cover);
+      if (cover != 0) kg.rows(a, wave < 2 ? b0 : b1, (wave & 1) * 32, key, cover);
     }
-    float* sk = reinterpret_cast<float*>(&Qs[0][0]);
-    float* sv = reinterpret_cast<float*>(&Gs[0][0]);
+    float* sk = reinterpret_cast<float*>(Q0);
+    float* sv = reinterpret_cast<float*>(G0);
     for (int turn = 0; turn < NT / 64; ++turn) {
       __syncthreads();
       if (wave == turn) {
@@ -816,21 +910,25 @@ __global__ void __launch_bounds__(NT, (kKeyWaves<T, DP>)) dkv_kernel(AttnArgs a,
   const RowRange rr(k0, a, seq);
   const int key = k0 + wave * 32 + (l & 31);
   kg.init(a, b, hk, key, key < seq.len);
-  if (rr.n0 < rr.n1) tile.load(a, seq, b, hk, rr.n0, rr.n1);
-  int buf = 0;
-  for (int t0 = rr.n0; t0 < rr.n1; t0 += BN, buf ^= 1) {
-    tile.store(Qs[buf], Gs[buf], Ls[buf], Ds[buf], Ps[buf]);
-    __syncthreads();
-    if (t0 + BN < rr.n1) tile.load(a, seq, b, hk, t0 + BN, rr.n1);
+  auto step = [&](const RowBuf<T>& buf, int t0) {
 #pragma unroll
     for (int sub = 0; sub < BN / 32; ++sub) {
       const int s0 = t0 + sub * 32;
       int pmin, pmax;
       const int cover = span(s0, s0 + 32 < rr.n1 ? s0 + 32 : rr.n1, a, seq, pmin, pmax)
                             ? coverage(pmin, pmax, k0 + wave * 32, a.W, a.S) : 0;
-      if (cover != 0)
-        kg.rows(a, Qs[buf], Gs[buf], Ls[buf], Ds[buf], Ps[buf], sub * 32, key, cover);
+      if (cover != 0) kg.rows(a, buf, sub * 32, key, cover);
     }
+  };
+  if (rr.n0 < rr.n1) rs.fetch(a, rr.n0, rr.n1, b0);
+  for (int t0 = rr.n0; t0 < rr.n1; t0 += 2 * BN) {
+    arrived();
+    if (t0 + BN < rr.n1) rs.fetch(a, t0 + BN, rr.n1, b1);
+    step(b0, t0);
+    if (t0 + BN >= rr.n1) break;
+    arrived();
+    if (t0 + 2 * BN < rr.n1) rs.fetch(a, t0 + 2 * BN, rr.n1, b0);
+    step(b1, t0 + BN);
   }
   if (a.far_chunks > 0 && key < a.S) {
     float* part = sink_part(a, bh, key / kSinkKeys, 0) + key % kSinkKeys * a.D;
