@@ -318,27 +318,18 @@ __device__ __forceinline__ bool span(int r0, int r1, const AttnArgs& args, const
   return true;
 }
 
-__device__ __forceinline__ bool sees(int p, int j, int W, int S) {
-  return j <= p && (p - j < W || j < S);
+// bits below n set, n clamped to [0, 32]
+__device__ __forceinline__ uint32_t below(int n) {
+  return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1u);
 }
 
-// what a run of rows sees of 32 keys from j0 on: 0 nothing, 2 all, 1 mixed
-__device__ __forceinline__ int coverage(int pmin, int pmax, int j0, int W, int S) {
-  const int j1 = j0 + 31;
-  if (j0 > pmax || (pmin - j1 >= W && j0 >= S)) return 0;
-  if (j1 <= pmin && (pmax - j0 < W || j1 < S)) return 2;
-  return 1;
-}
-
-// scores that rows do not see become -inf: their probability is 0
-template <bool KEYS_IN_REGS>
-__device__ __forceinline__ void hide(v16f& s, int fixed, const int* others, int j0, int h, int W,
-                                     int S) {
+// Scores become -inf where bit acc_row(e, 0) of `keep` is clear: their
+// probability is 0.  Two instructions an element (sign-extended bit, select).
+__device__ __forceinline__ void hide(v16f& s, uint32_t keep) {
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
-    const int p = KEYS_IN_REGS ? fixed : others[acc_row(e, h)];
-    const int j = KEYS_IN_REGS ? j0 + acc_row(e, h) : fixed;
-    if (!sees(p, j, W, S)) s[e] = -kInf;
+    const uint32_t m = (uint32_t)((int)(keep << (31 - acc_row(e, 0))) >> 31);
+    s[e] = __uint_as_float((__float_as_uint(s[e]) & m) | (0xff800000u & ~m));
   }
 }
 
@@ -363,8 +354,11 @@ __device__ __forceinline__ void put(O* out, const v16f (&x)[ND], float f, bool z
 // What a block of the row kernels (forward, dq) works on.
 struct RowBlock {
   int b, hk, bh, r0, r, t, head, p, h, wave;
-  int wmin, wmax, tiles;
-  bool live, wany;
+  int tiles;
+  // keys that some row of this wave sees, and those that all rows see:
+  // [0, S) or [any0, any1), and [full0, full1) or [0, fulls)
+  int any0, any1, full0, full1, fulls;
+  bool live;
   Seq seq;
   __device__ __forceinline__ RowBlock(const AttnArgs& a) {
     bh = blockIdx.x;
@@ -383,9 +377,24 @@ struct RowBlock {
     live = r < rows;
     p = live ? position(t, seq) : -1;
     const int w0 = r0 + wave * 32;
-    wmin = 0;
-    wmax = -1;
-    wany = span(w0, w0 + 32 < rows ? w0 + 32 : rows, a, seq, wmin, wmax);
+    int wmin = 0, wmax = -1;  // no rows: no keys
+    span(w0, w0 + 32 < rows ? w0 + 32 : rows, a, seq, wmin, wmax);
+    any0 = wmin - a.W + 1;
+    any1 = wmax + 1;
+    full0 = wmax - a.W + 1;
+    full1 = wmin + 1;
+    fulls = a.S < full1 ? a.S : full1;
+  }
+  // what the wave's rows see of 32 keys from j0 on: 0 nothing, 2 all, 1 mixed
+  __device__ __forceinline__ int coverage(int j0, int S) const {
+    if (j0 >= any1 || (j0 + 32 <= any0 && j0 >= S)) return 0;
+    return (j0 >= full0 && j0 + 32 <= full1) || j0 + 32 <= fulls ? 2 : 1;
+  }
+  // which of the 32 keys from j0 on this lane's row sees: bit o is key
+  // j0 + 4h + o
+  __device__ __forceinline__ uint32_t seen(int j0, const AttnArgs& a) const {
+    const int first = j0 + 4 * h;
+    return below(p - first + 1) & (~below(p - a.W + 1 - first) | below(a.S - first));
   }
   __device__ __forceinline__ KeyTiles keys(const AttnArgs& a) {
     const int rows = a.Tq * a.G;
@@ -488,12 +497,12 @@ __global__ void __launch_bounds__(NT, (kRowWaves<T, DP>)) fwd_kernel(AttnArgs a)
 #pragma unroll
     for (int sub = 0; sub < BN / 32; ++sub) {
       const int js = j0 + sub * 32;
-      const int cover = w.wany ? coverage(w.wmin, w.wmax, js, a.W, a.S) : 0;
+      const int cover = w.coverage(js, a.S);
       if (cover == 0) continue;
       v16f s = zero16();
 #pragma unroll
       for (int k = 0; k < KD; ++k) s = Ops<T>::mma(row_frag<T, DP>(K, sub * 32, k), qf[k], s);
-      if (cover == 1) hide<true>(s, w.p, nullptr, js, h, a.W, a.S);
+      if (cover == 1) hide(s, w.seen(js, a));
       float mx = s[0];
 #pragma unroll
       for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
@@ -646,7 +655,7 @@ __global__ void __launch_bounds__(NT, (kRowWaves<T, DP>)) dq_kernel(AttnArgs a) 
 #pragma unroll
     for (int sub = 0; sub < BN / 32; ++sub) {
       const int js = j0 + sub * 32;
-      const int cover = w.wany ? coverage(w.wmin, w.wmax, js, a.W, a.S) : 0;
+      const int cover = w.coverage(js, a.S);
       if (cover == 0) continue;
       v16f s = zero16(), dp = zero16();
 #pragma unroll
@@ -654,7 +663,7 @@ __global__ void __launch_bounds__(NT, (kRowWaves<T, DP>)) dq_kernel(AttnArgs a) 
         s = Ops<T>::mma(row_frag<T, DP>(K, sub * 32, k), qf[k], s);
         dp = Ops<T>::mma(row_frag<T, DP>(V, sub * 32, k), gf[k], dp);
       }
-      if (cover == 1) hide<true>(s, w.p, nullptr, js, h, a.W, a.S);
+      if (cover == 1) hide(s, w.seen(js, a));
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = ex2(__builtin_fmaf(s[e], c, -lse)) * (dp[e] - delta);
 #pragma unroll
@@ -700,12 +709,11 @@ __device__ __forceinline__ float* sink_part(const AttnArgs& a, int bh, int group
                         kSinkKeys * a.D;
 }
 
-// 64 rows of q and do with their statistics, and the positions of the rows
+// 64 rows of q and do with their statistics
 template <typename T>
 struct RowBuf {
   T *q, *g;
   float *lse, *delta;
-  int* p;
 };
 
 template <typename T, int DP>
@@ -714,11 +722,10 @@ struct RowStream {
   const T *q, *g;
   const float *lse, *delta;
   uint32_t qo[D::CH], go[D::CH];
-  int wave, start;
+  int wave;
   bool repeats;  // every tile begins with a token's first head
-  __device__ __forceinline__ RowStream(const AttnArgs& a, const Seq& seq, int b, int hk, int wv) {
+  __device__ __forceinline__ RowStream(const AttnArgs& a, int b, int hk, int wv) {
     wave = wv;
-    start = seq.start;
     q = reinterpret_cast<const T*>(a.q) + b * a.qs[0] + hk * a.G * a.qs[1];
     g = reinterpret_cast<const T*>(a.dout) + b * a.dos[0] + hk * a.G * a.dos[1];
     const int64_t at = ((int64_t)b * a.Hkv + hk) * (a.Tq * a.G);
@@ -764,9 +771,33 @@ struct RowStream {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
           rs, (__attribute__((address_space(3))) void*)(wave == 0 ? to.lse : to.delta), 4, l * 4,
           0, 0, 0);
-    } else if (wave == 2) {
-      to.p[l] = Row(r0 + l, a).t + start;
     }
+  }
+};
+
+// The rows that see a wave's 32 keys, as rows: first and behind the last
+// that see some of them, that see all of them, and that see this lane's.
+struct KeyRows {
+  int any0, any1, full0, full1, mine0, mine1;
+  __device__ __forceinline__ KeyRows(int j0, int key, const AttnArgs& a, const Seq& s) {
+    // row of the first token at position p or later
+    auto row = [&](int64_t p) { return RowRange::clip(p - s.start, a) * a.G; };
+    const int64_t last = s.len, w = a.W;
+    any0 = row(j0);
+    any1 = row(j0 < a.S || j0 + 31 + w > last ? last : j0 + 31 + w);
+    full0 = row((int64_t)j0 + 31);
+    full1 = row(j0 + 31 < a.S || j0 + w > last ? last : j0 + w);
+    mine0 = row(key);
+    mine1 = row(key < a.S || key + w > last ? last : key + w);
+  }
+  __device__ __forceinline__ int coverage(int r0) const {
+    if (r0 + 32 <= any0 || r0 >= any1) return 0;
+    return r0 >= full0 && r0 + 32 <= full1 ? 2 : 1;
+  }
+  // bit o is row r0 + 4h + o
+  __device__ __forceinline__ uint32_t seen(int r0, int h) const {
+    const int first = r0 + 4 * h;
+    return below(mine1 - first) & ~below(mine0 - first);
   }
 };
 
@@ -793,9 +824,11 @@ struct KeyGrad {
     for (int d = 0; d < ND; ++d) dk[d] = dv[d] = zero16();
   }
 
-  // 32 rows from tile row i0 on
-  __device__ __forceinline__ void rows(const AttnArgs& a, const RowBuf<T>& b, int i0, int key,
-                                       int cover) {
+  // 32 rows, r0 on, that lie in the tile from its row i0 on
+  __device__ __forceinline__ void rows(const AttnArgs& a, const RowBuf<T>& b, int i0, int r0,
+                                       const KeyRows& kr) {
+    const int cover = kr.coverage(r0);
+    if (cover == 0) return;
     const int h = (threadIdx.x & 63) >> 5;
     const float c = a.scale * kLog2e;
     v16f s = zero16(), dp = zero16();
@@ -804,7 +837,7 @@ struct KeyGrad {
       s = Ops<T>::mma(row_frag<T, DP>(b.q, i0, k), kf[k], s);
       dp = Ops<T>::mma(row_frag<T, DP>(b.g, i0, k), vf[k], dp);
     }
-    if (cover == 1) hide<false>(s, key, b.p + i0, 0, h, a.W, a.S);
+    if (cover == 1) hide(s, kr.seen(r0, h));
 #pragma unroll
     for (int e4 = 0; e4 < 4; ++e4) {
       const v4f le = *reinterpret_cast<const v4f*>(b.lse + i0 + acc_row(e4 * 4, h));
@@ -841,14 +874,13 @@ __global__ void __launch_bounds__(NT, (kKeyWaves<T, DP>)) dkv_kernel(AttnArgs a,
   __shared__ __attribute__((aligned(16))) T G0[BN * LD];
   __shared__ __attribute__((aligned(16))) T G1[BN * LD];
   __shared__ __attribute__((aligned(16))) float L0[BN], L1[BN], D0[BN], D1[BN];
-  __shared__ int P0[BN], P1[BN];
   static_assert(BN * LD * sizeof(T) >= kSinkKeys * DP * sizeof(float), "sums of a far item");
-  const RowBuf<T> b0{Q0, G0, L0, D0, P0}, b1{Q1, G1, L1, D1, P1};
+  const RowBuf<T> b0{Q0, G0, L0, D0}, b1{Q1, G1, L1, D1};
   const int bh = blockIdx.x, b = bh / a.Hkv, hk = bh - b * a.Hkv;
   const int l = threadIdx.x & 63, h = l >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Seq seq = sequence(a, b);
-  const RowStream<T, DP> rs(a, seq, b, hk, wave);
+  const RowStream<T, DP> rs(a, b, hk, wave);
   KeyGrad<T, DP> kg;
 
   if ((int)blockIdx.y >= key_blocks) {
@@ -860,17 +892,15 @@ __global__ void __launch_bounds__(NT, (kKeyWaves<T, DP>)) dkv_kernel(AttnArgs a,
     const int per = (tokens + a.far_chunks - 1) / a.far_chunks * a.G;
     const int ra = rr.n1 + per * chunk < rr.f1 ? rr.n1 + per * chunk : rr.f1;
     const int rb = ra + per < rr.f1 ? ra + per : rr.f1;
+    const KeyRows kr(j0, key, a, seq);
     kg.init(a, b, hk, key, key < seq.len);
     for (int t0 = ra; t0 < rb; t0 += BM) {
       __syncthreads();
       rs.fetch(a, t0, rb, b0);
       rs.fetch(a, t0 + BN, rb, b1);
       arrived();
-      const int s0 = t0 + wave * 32;
-      int pmin, pmax;
-      const int cover = span(s0, s0 + 32 < rb ? s0 + 32 : rb, a, seq, pmin, pmax)
-                            ? coverage(pmin, pmax, j0, a.W, a.S) : 0;
-      if (cover != 0) kg.rows(a, wave < 2 ? b0 : b1, (wave & 1) * 32, key, cover);
+      if (t0 + wave * 32 < rb)
+        kg.rows(a, wave < 2 ? b0 : b1, (wave & 1) * 32, t0 + wave * 32, kr);
     }
     float* sk = reinterpret_cast<float*>(Q0);
     float* sv = reinterpret_cast<float*>(G0);
@@ -909,16 +939,11 @@ __global__ void __launch_bounds__(NT, (kKeyWaves<T, DP>)) dkv_kernel(AttnArgs a,
   const int k0 = (int)blockIdx.y * BM;
   const RowRange rr(k0, a, seq);
   const int key = k0 + wave * 32 + (l & 31);
+  const KeyRows kr(k0 + wave * 32, key, a, seq);
   kg.init(a, b, hk, key, key < seq.len);
   auto step = [&](const RowBuf<T>& buf, int t0) {
 #pragma unroll
-    for (int sub = 0; sub < BN / 32; ++sub) {
-      const int s0 = t0 + sub * 32;
-      int pmin, pmax;
-      const int cover = span(s0, s0 + 32 < rr.n1 ? s0 + 32 : rr.n1, a, seq, pmin, pmax)
-                            ? coverage(pmin, pmax, k0 + wave * 32, a.W, a.S) : 0;
-      if (cover != 0) kg.rows(a, buf, sub * 32, key, cover);
-    }
+    for (int sub = 0; sub < BN / 32; ++sub) kg.rows(a, buf, sub * 32, t0 + sub * 32, kr);
   };
   if (rr.n0 < rr.n1) rs.fetch(a, rr.n0, rr.n1, b0);
   for (int t0 = rr.n0; t0 < rr.n1; t0 += 2 * BN) {
