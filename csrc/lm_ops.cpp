@@ -356,7 +356,7 @@ std::tuple<at::Tensor, at::Tensor> rotary_axes(const at::Tensor& q, const at::Te
 // ------------------------------------------------------------- distill
 kfac::DistillArgs distill_args(const at::Tensor& z, const at::Tensor& teacher,
                                const at::Tensor& index, const OptTensor& rest,
-                               double temperature) {
+                               double temperature, double weight) {
   TORCH_CHECK(z.is_cuda() && z.dim() == 3 && (z.stride(2) == 1 || z.size(2) == 1),
               "topk_distill_loss: logits must be a GPU tensor [.., .., V] with unit last stride");
   on_device(teacher, z, "teacher_logits");
@@ -388,6 +388,7 @@ kfac::DistillArgs distill_args(const at::Tensor& z, const at::Tensor& teacher,
   a.index = index.data_ptr();
   a.index64 = index.scalar_type() == at::kLong;
   a.temperature = (float)temperature;
+  a.weight = (float)weight;
   a.aligned = rows16(z);
   kfac::distill_split(a.N, a.V, rest.has_value(), &a.slice, &a.splits);
   TORCH_CHECK(a.N * a.splits < (1LL << 31), "topk_distill_loss: too many rows");
@@ -395,31 +396,43 @@ kfac::DistillArgs distill_args(const at::Tensor& z, const at::Tensor& teacher,
 }
 
 struct DistillOut {
-  at::Tensor loss, info, mean;
+  at::Tensor loss, info, mean, dz;
 };
 
-// reduction: 0 none, 1 sum, 2 mean
+// reduction: 0 none, 1 sum, 2 mean; grad: a backward pass will follow
 DistillOut distill_run(const at::Tensor& z, const at::Tensor& teacher, const at::Tensor& index,
-                       const OptTensor& rest, double temperature, int64_t reduction) {
+                       const OptTensor& rest, double temperature, double weight,
+                       int64_t reduction, bool grad) {
   c10::hip::HIPGuardMasqueradingAsCUDA g(z.device());
-  kfac::DistillArgs a = distill_args(z, teacher, index, rest, temperature);
+  kfac::DistillArgs a = distill_args(z, teacher, index, rest, temperature, weight);
   const auto f32 = z.options().dtype(at::kFloat);
   DistillOut o;
   o.info = at::empty({a.N, 4}, f32);
   at::Tensor rows = at::empty({a.N}, f32);
-  at::Tensor part;
-  if (a.splits > 1) part = at::empty({a.N * a.splits, 4}, f32);
   a.info = reinterpret_cast<float4*>(o.info.data_ptr<float>());
   a.row_loss = rows.data_ptr<float>();
-  a.part = a.splits > 1 ? reinterpret_cast<float4*>(part.data_ptr<float>()) : nullptr;
   o.loss = rows;
+  float *loss = nullptr, *mean = nullptr;
   if (reduction != 0) {
     o.loss = at::empty({}, f32);
     o.mean = at::empty({1}, f32);
+    loss = o.loss.data_ptr<float>();
+    mean = o.mean.data_ptr<float>();
   }
-  kfac::distill_forward(tag(z), a, reduction != 0 ? o.loss.data_ptr<float>() : nullptr,
-                        reduction != 0 ? o.mean.data_ptr<float>() : nullptr, (int)reduction,
-                        stream());
+  if (grad && reduction != 0 && kfac::distill_fuses(tag(z), a.N, a.V)) {
+    o.dz = at::empty(z.sizes(), z.options());
+    a.dz = o.dz.data_ptr();
+    a.dz_aligned = rows16(o.dz);
+    a.mean = mean;
+    kfac::distill_forward_grad(tag(z), a, loss, (int)reduction, stream());
+  } else {
+    at::Tensor part;
+    if (a.splits > 1) {
+      part = at::empty({a.N * a.splits, 4}, f32);
+      a.part = reinterpret_cast<float4*>(part.data_ptr<float>());
+    }
+    kfac::distill_forward(tag(z), a, loss, mean, (int)reduction, stream());
+  }
   C10_HIP_KERNEL_LAUNCH_CHECK();
   return o;
 }
@@ -427,25 +440,41 @@ DistillOut distill_run(const at::Tensor& z, const at::Tensor& teacher, const at:
 struct DistillFn : public torch::autograd::Function<DistillFn> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& z, const at::Tensor& teacher,
                             const at::Tensor& index, const OptTensor& rest, double temperature,
-                            int64_t reduction) {
-    auto o = distill_run(z, teacher, index, rest, temperature, reduction);
+                            double weight, int64_t reduction) {
+    auto o = distill_run(z, teacher, index, rest, temperature, weight, reduction, true);
     ctx->save_for_backward({z, teacher, index, rest.has_value() ? *rest : at::Tensor(), o.info,
                             o.mean});
     ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["weight"] = weight;
     ctx->saved_data["reduction"] = reduction;
+    if (o.dz.defined()) ctx->saved_data["dz"] = o.dz;
     return o.loss;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once_only("topk_distill_loss");
     auto sv = ctx->get_saved_variables();
     const at::Tensor& z = sv[0];
-    const OptTensor rest = sv[3].defined() ? OptTensor(sv[3]) : c10::nullopt;
     c10::hip::HIPGuardMasqueradingAsCUDA g(z.device());
-    kfac::DistillArgs a =
-        distill_args(z, sv[1], sv[2], rest, ctx->saved_data["temperature"].toDouble());
-    const bool rows = ctx->saved_data["reduction"].toInt() == 0;
     const at::Tensor up = grads[0].to(at::kFloat).contiguous();
-    at::Tensor dz = at::empty(z.sizes(), z.options());
+    at::Tensor dz, u;
+    auto kept = ctx->saved_data.find("dz");
+    if (kept != ctx->saved_data.end()) {
+      // the gradient that the forward wrote is given away and scaled in
+      // place, so it serves one backward pass; another one of the same graph
+      // (retain_graph) computes its own below
+      dz = kept->second.toTensor();
+      ctx->saved_data.erase(kept);
+      if (dz.numel() > 0)
+        kfac::distill_scale(tag(z), dz.data_ptr(), dz.numel(), up.data_ptr<float>(), stream());
+      C10_HIP_KERNEL_LAUNCH_CHECK();
+      return {dz, u, u, u, u, u, u};
+    }
+    const OptTensor rest = sv[3].defined() ? OptTensor(sv[3]) : c10::nullopt;
+    kfac::DistillArgs a =
+        distill_args(z, sv[1], sv[2], rest, ctx->saved_data["temperature"].toDouble(),
+                     ctx->saved_data["weight"].toDouble());
+    const bool rows = ctx->saved_data["reduction"].toInt() == 0;
+    dz = at::empty(z.sizes(), z.options());
     a.info = reinterpret_cast<float4*>(sv[4].data_ptr<float>());
     a.upstream = up.data_ptr<float>();
     a.upstream_rows = rows;
@@ -454,16 +483,16 @@ struct DistillFn : public torch::autograd::Function<DistillFn> {
     a.dz_aligned = rows16(dz);
     kfac::distill_backward(tag(z), a, stream());
     C10_HIP_KERNEL_LAUNCH_CHECK();
-    at::Tensor u;
-    return {dz, u, u, u, u, u};
+    return {dz, u, u, u, u, u, u};
   }
 };
 
 at::Tensor topk_distill_loss(const at::Tensor& z, const at::Tensor& teacher,
                              const at::Tensor& index, const OptTensor& rest, double temperature,
-                             int64_t reduction) {
-  if (records({&z})) return DistillFn::apply(z, teacher, index, rest, temperature, reduction);
-  return distill_run(z, teacher, index, rest, temperature, reduction).loss;
+                             double weight, int64_t reduction) {
+  if (records({&z}))
+    return DistillFn::apply(z, teacher, index, rest, temperature, weight, reduction);
+  return distill_run(z, teacher, index, rest, temperature, weight, reduction, false).loss;
 }
 
 }  // namespace
@@ -476,5 +505,6 @@ void bind_lm_ops(pybind11::module& m) {
   m.def("rotary_axes", &rotary_axes, py::arg("q"), py::arg("k"), py::arg("positions"),
         py::arg("turn"), py::arg("axis"), py::arg("halves"));
   m.def("topk_distill_loss", &topk_distill_loss, py::arg("logits"), py::arg("teacher"),
-        py::arg("index"), py::arg("rest"), py::arg("temperature"), py::arg("reduction"));
+        py::arg("index"), py::arg("rest"), py::arg("temperature"),
+        py::arg("weight"), py::arg("reduction"));
 }

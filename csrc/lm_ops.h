@@ -41,7 +41,7 @@ struct DistillArgs {
   const float* rest;     // [N] or null
   int64_t N, V;
   int K, index64, aligned;
-  float temperature;
+  float temperature, weight;
   float4* part;          // [N, splits]: running statistics of a slice of a row
   float4* info;          // [N]: see distill.hip
   float* row_loss;       // [N]
@@ -60,6 +60,13 @@ struct DistillArgs {
 void distill_forward(int dtype, const DistillArgs& a, float* loss, float* factor, int reduction,
                      hipStream_t st);
 void distill_backward(int dtype, const DistillArgs& a, hipStream_t st);
+// loss and gradient in one pass over the logits (a.dz, a.mean to be written;
+// reduction 1 or 2), where distill_fuses says so
+bool distill_fuses(int dtype, int64_t N, int64_t V);
+void distill_forward_grad(int dtype, const DistillArgs& a, float* loss, int reduction,
+                          hipStream_t st);
+// dz *= *factor in place (16-byte aligned)
+void distill_scale(int dtype, void* dz, int64_t n, const float* factor, hipStream_t st);
 // columns of a split for N rows of V columns, and how many there are
 void distill_split(int64_t N, int64_t V, bool bitmap, int64_t* slice, int* splits);
 

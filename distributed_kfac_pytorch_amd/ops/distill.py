@@ -11,10 +11,12 @@ divided by the temperature): ``r`` is the share of the rest, ``R`` what the
 student gives to the columns outside the row's entries.  Without it the
 entries are renormalised and ``r = 0``.
 
-GPU tensors run the native kernels: one pass over the logits forward, one
-pass backward that writes the gradient; no copy of the logits in fp32, sums
-in 32 bits or more, bit-reproducible.  CPU tensors run the same formula in
-torch.  ``utils.training.TopKDistillLoss`` is the module form.
+GPU tensors run the native kernels, which make no copy of the logits in fp32,
+sum in 32 bits or more and are bit-reproducible.  With 256 rows or more in
+bf16 or fp32 the forward reads the logits once and writes their gradient in
+the same pass; otherwise the backward reads them once more.  CPU tensors run
+the same formula in torch.  ``utils.training.TopKDistillLoss`` is the module
+form.
 """
 from __future__ import annotations
 
@@ -75,6 +77,7 @@ def topk_distill_loss(
     *,
     teacher_rest: torch.Tensor | None = None,
     temperature: float = 1.0,
+    weight: float = 1.0,
     reduction: str = 'mean',
 ) -> torch.Tensor:
     """Divergence of the student's ``logits`` ``[..., V]`` from a teacher of
@@ -92,6 +95,10 @@ def topk_distill_loss(
         teacher_rest: ``[...]``, log-sum-exp of the teacher's other logits
             divided by the temperature; constant.
         temperature: positive; the loss carries its square.
+        weight: factor of the loss.  Give a known factor (a mixing weight, one
+            over the accumulation steps) here rather than multiply the result:
+            in bf16 and fp32 the forward already writes the gradient, and a
+            factor put on later costs another pass over it.
         reduction: ``'mean'`` over the rows that have entries, ``'sum'`` or
             ``'none'`` (``[...]``).
 
@@ -123,12 +130,16 @@ def topk_distill_loss(
     temperature = float(temperature)
     if not (temperature > 0.0 and math.isfinite(temperature)):
         raise ValueError(f'temperature must be positive, got {temperature}')
+    weight = float(weight)
+    if not math.isfinite(weight):
+        raise ValueError(f'weight must be finite, got {weight}')
     if reduction not in _REDUCTIONS:
         raise ValueError(f'reduction must be one of {_REDUCTIONS}, got {reduction!r}')
     teacher_logits = teacher_logits.detach()
     rest = None if teacher_rest is None else teacher_rest.detach()
     if not _nat.use_native(logits):
-        return _reference(logits, teacher_logits, teacher_index, rest, temperature, reduction)
+        loss = _reference(logits, teacher_logits, teacher_index, rest, temperature, reduction)
+        return loss if weight == 1.0 else loss * weight
     z = logits
     if z.stride(-1) != 1 and z.shape[-1] > 1:
         z = z.contiguous()
@@ -139,5 +150,5 @@ def topk_distill_loss(
     loss = _nat.native().topk_distill_loss(  # type: ignore[union-attr]
         z, teacher_logits.float().contiguous(), teacher_index.contiguous(),
         None if rest is None else rest.float().contiguous(), temperature,
-        _REDUCTIONS.index(reduction))
+        weight, _REDUCTIONS.index(reduction))
     return loss.view(lead) if reduction == 'none' else loss

@@ -91,6 +91,7 @@ def test_rotary_refuses_operands():
     (dict(temperature=0.0), ValueError),
     (dict(temperature=float('inf')), ValueError),
     (dict(reduction='avg'), ValueError),
+    (dict(weight=float('nan')), ValueError),
     (dict(teacher_rest=torch.zeros(2)), ValueError),
     (dict(teacher_rest=torch.zeros(3, dtype=torch.int64)), ValueError),
 ])
