@@ -90,6 +90,14 @@ struct AttnConf {
   double scale;
 };
 
+// what a node keeps besides tensors, as one entry (each is exact in a double)
+std::vector<double> pack(const AttnConf& c) {
+  return {(double)c.window, (double)c.sinks, (double)c.start, c.start_given ? 1.0 : 0.0, c.scale};
+}
+AttnConf unpack(const std::vector<double>& v) {
+  return {(int64_t)v[0], (int64_t)v[1], (int64_t)v[2], v[3] != 0.0, v[4]};
+}
+
 kfac::AttnArgs attn_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                          const OptTensor& lengths, const OptTensor& starts, const AttnConf& c) {
   TORCH_CHECK(q.is_cuda() && q.dim() == 4 && k.dim() == 4 && v.sizes() == k.sizes(),
@@ -187,20 +195,14 @@ struct WindowAttnFn : public torch::autograd::Function<WindowAttnFn> {
     auto [out, lse] = attn_forward(q, k, v, lengths, starts, c, true);
     ctx->save_for_backward({q, k, v, out, lse, lengths.has_value() ? *lengths : at::Tensor(),
                             starts.has_value() ? *starts : at::Tensor()});
-    ctx->saved_data["window"] = window;
-    ctx->saved_data["sinks"] = sinks;
-    ctx->saved_data["start"] = start;
-    ctx->saved_data["start_given"] = start_given;
-    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["conf"] = pack(c);
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once_only("window_attention");
     auto sv = ctx->get_saved_variables();
     const at::Tensor &q = sv[0], &k = sv[1], &v = sv[2], &out = sv[3], &lse = sv[4];
-    const AttnConf c{ctx->saved_data["window"].toInt(), ctx->saved_data["sinks"].toInt(),
-                     ctx->saved_data["start"].toInt(), ctx->saved_data["start_given"].toBool(),
-                     ctx->saved_data["scale"].toDouble()};
+    const AttnConf c = unpack(ctx->saved_data["conf"].toDoubleVector());
     const OptTensor lengths = sv[5].defined() ? OptTensor(sv[5]) : c10::nullopt;
     const OptTensor starts = sv[6].defined() ? OptTensor(sv[6]) : c10::nullopt;
     c10::hip::HIPGuardMasqueradingAsCUDA g(q.device());
@@ -211,13 +213,10 @@ struct WindowAttnFn : public torch::autograd::Function<WindowAttnFn> {
       dk.zero_();
       dv.zero_();
     } else {
-      at::Tensor delta = at::empty_like(lse);
       a.out = out.data_ptr();
       strides3(out, a.os);
       a.dout = go.data_ptr();
       strides3(go, a.dos);
-      a.lse = lse.data_ptr<float>();
-      a.delta = delta.data_ptr<float>();
       a.dq = dq.data_ptr();
       a.dk = dk.data_ptr();
       a.dv = dv.data_ptr();
@@ -228,11 +227,11 @@ struct WindowAttnFn : public torch::autograd::Function<WindowAttnFn> {
       kfac::attn_bwd_plan(a, &a.sink_groups, &a.far_chunks, &floats);
       TORCH_CHECK((int64_t)(a.Tk + 127) / 128 + (int64_t)a.sink_groups * a.far_chunks <= 65535,
                   "window_attention: more than 65535 key blocks");
-      at::Tensor ws;
-      if (floats > 0) {
-        ws = at::empty({floats}, lse.options());
-        a.kvpart = ws.data_ptr<float>();
-      }
+      // the sinks' shares (16-byte aligned), then delta
+      const at::Tensor ws = at::empty({floats + lse.numel()}, lse.options());
+      a.lse = lse.data_ptr<float>();
+      a.kvpart = ws.data_ptr<float>();
+      a.delta = a.kvpart + floats;
       if (a.Tk == 0) dq.zero_();
       kfac::attn_backward(tag(q), a, stream());
       C10_HIP_KERNEL_LAUNCH_CHECK();
@@ -254,9 +253,10 @@ at::Tensor window_attention(const at::Tensor& q, const at::Tensor& k, const at::
 }
 
 // -------------------------------------------------------------- rotary
+// a pair's frequency in turns per position, and its axis: fp64 [pairs, 2] on
+// the CPU
 struct RotaryConf {
-  std::vector<double> turn;    // of each pair
-  std::vector<int64_t> axis;
+  at::Tensor table;
   bool halves;
 };
 
@@ -270,9 +270,11 @@ std::tuple<at::Tensor, at::Tensor> rotary_run(const at::Tensor& q, const at::Ten
   on_device(k, q, "k");
   on_device(pos, q, "positions");
   const int64_t B = q.size(0), T = q.size(2), D = q.size(3);
-  const int64_t pairs = (int64_t)c.turn.size();
-  TORCH_CHECK(pairs >= 1 && pairs <= kfac::kMaxRotaryPairs && 2 * pairs <= D && D % 2 == 0 &&
-                  c.axis.size() == c.turn.size(),
+  TORCH_CHECK(c.table.device().is_cpu() && c.table.scalar_type() == at::kDouble &&
+                  c.table.dim() == 2 && c.table.size(1) == 2 && c.table.is_contiguous(),
+              "rotary_axes: table must be a contiguous fp64 CPU tensor [pairs, 2]");
+  const int64_t pairs = c.table.size(0);
+  TORCH_CHECK(pairs >= 1 && pairs <= kfac::kMaxRotaryPairs && 2 * pairs <= D && D % 2 == 0,
               "rotary_axes: pairs do not fit the head");
   TORCH_CHECK((pos.scalar_type() == at::kLong || pos.scalar_type() == at::kInt) &&
                   (pos.dim() == 2 || (pos.dim() == 3 && pos.size(0) == B)) &&
@@ -282,10 +284,11 @@ std::tuple<at::Tensor, at::Tensor> rotary_run(const at::Tensor& q, const at::Ten
               "rotary_axes: too large");
   c10::hip::HIPGuardMasqueradingAsCUDA g(q.device());
   kfac::RotaryArgs a{};
-  for (int64_t i = 0; i < pairs; ++i) {
-    TORCH_CHECK(c.axis[i] >= 0 && c.axis[i] < pos.size(-1), "rotary_axes: axis of a pair");
-    a.tab.turn[i] = c.turn[i];
-    a.tab.axis[i] = (uint8_t)c.axis[i];
+  const double* entry = c.table.data_ptr<double>();
+  for (int64_t i = 0; i < pairs; ++i, entry += 2) {
+    TORCH_CHECK(entry[1] >= 0 && entry[1] < pos.size(-1), "rotary_axes: axis of a pair");
+    a.tab.turn[i] = entry[0];
+    a.tab.axis[i] = (uint8_t)entry[1];
   }
   at::Tensor qo = at::empty({B, q.size(1), T, D}, q.options());
   at::Tensor ko = at::empty({B, k.size(1), T, D}, k.options());
@@ -321,36 +324,32 @@ at::Tensor unit_last(const at::Tensor& t) {
 
 struct RotaryFn : public torch::autograd::Function<RotaryFn> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k,
-                               const at::Tensor& pos, const std::vector<double>& turn,
-                               const std::vector<int64_t>& axis, bool halves) {
-    const RotaryConf c{turn, axis, halves};
+                               const at::Tensor& pos, const at::Tensor& table, bool halves) {
+    const RotaryConf c{table, halves};
     auto [qo, ko] = rotary_run(unit_last(q), unit_last(k), pos, c, 1.0);
     ctx->save_for_backward({pos});
-    ctx->saved_data["turn"] = turn;
-    ctx->saved_data["axis"] = axis;
-    ctx->saved_data["halves"] = halves;
+    ctx->saved_data[halves ? "halves" : "interleaved"] = table;
     return {qo, ko};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once_only("rotary_axes");
-    const RotaryConf c{ctx->saved_data["turn"].toDoubleVector(),
-                       ctx->saved_data["axis"].toIntVector(), ctx->saved_data["halves"].toBool()};
+    const auto kept = ctx->saved_data.begin();
+    const RotaryConf c{kept->second.toTensor(), kept->first == "halves"};
     auto [dq, dk] = rotary_run(unit_last(grads[0]), unit_last(grads[1]),
                                ctx->get_saved_variables()[0], c, -1.0);
     at::Tensor u;
-    return {dq, dk, u, u, u, u};
+    return {dq, dk, u, u, u};
   }
 };
 
 std::tuple<at::Tensor, at::Tensor> rotary_axes(const at::Tensor& q, const at::Tensor& k,
-                                               const at::Tensor& pos,
-                                               const std::vector<double>& turn,
-                                               const std::vector<int64_t>& axis, bool halves) {
+                                               const at::Tensor& pos, const at::Tensor& table,
+                                               bool halves) {
   if (records({&q, &k})) {
-    auto r = RotaryFn::apply(q, k, pos, turn, axis, halves);
+    auto r = RotaryFn::apply(q, k, pos, table, halves);
     return {r[0], r[1]};
   }
-  return rotary_run(unit_last(q), unit_last(k), pos, RotaryConf{turn, axis, halves}, 1.0);
+  return rotary_run(unit_last(q), unit_last(k), pos, RotaryConf{table, halves}, 1.0);
 }
 
 // ------------------------------------------------------------- distill
@@ -503,7 +502,7 @@ void bind_lm_ops(pybind11::module& m) {
         py::arg("lengths"), py::arg("starts"), py::arg("window"), py::arg("sinks"),
         py::arg("start"), py::arg("start_given"), py::arg("scale"));
   m.def("rotary_axes", &rotary_axes, py::arg("q"), py::arg("k"), py::arg("positions"),
-        py::arg("turn"), py::arg("axis"), py::arg("halves"));
+        py::arg("table"), py::arg("halves"));
   m.def("topk_distill_loss", &topk_distill_loss, py::arg("logits"), py::arg("teacher"),
         py::arg("index"), py::arg("rest"), py::arg("temperature"),
         py::arg("weight"), py::arg("reduction"));

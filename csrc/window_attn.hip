@@ -578,14 +578,15 @@ __global__ void __launch_bounds__(NT) join_kernel(AttnArgs a) {
   const int grp = tid >> 5, d = (tid & 31) * 4;
   v4f o = {0.f, 0.f, 0.f, 0.f};
   float sum = 0.f;
+#pragma unroll 8
   for (int z = grp; z < a.splits; z += 8) {
     const float wt = wts[z];
     sum += wt;
-    if (d < a.D) {
-      const v4f x = *reinterpret_cast<const v4f*>(a.opart + (z * all + row) * a.D + d);
+    // lanes behind D read its last elements again and are not stored
+    const v4f x = *reinterpret_cast<const v4f*>(a.opart + (z * all + row) * a.D +
+                                                (d < a.D ? d : a.D - 4));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] += wt * x[i];
-    }
+    for (int i = 0; i < 4; ++i) o[i] += wt * x[i];
   }
   part[grp][tid & 31] = o;
   __syncthreads();
@@ -694,6 +695,7 @@ struct RowRange {
     if (n1 < n0) n1 = n0;
     f1 = k0 < a.S && k0 <= last ? clip(last + 1 - s.start, a) * a.G : n1;
     if (f1 < n1) f1 = n1;
+    if (a.far_chunks == 0) n1 = f1;  // no far items: the block takes all rows
   }
   __device__ __forceinline__ static int clip(int64_t t, const AttnArgs& a) {
     return (int)(t < 0 ? 0 : (t < a.Tq ? t : a.Tq));
@@ -1061,8 +1063,11 @@ void attn_forward(int dtype, const AttnArgs& a, hipStream_t st) {
 void attn_bwd_plan(const AttnArgs& a, int* sink_groups, int* far_chunks, int64_t* floats) {
   *sink_groups = *far_chunks = 0;
   *floats = 0;
-  // far rows exist only behind the window of a sink's key
-  if (a.S <= 0 || a.W >= a.Tk) return;
+  // far rows exist only behind the window of a sink's key; up to 512 rows
+  // (8 tiles) the block of keys takes them itself: a launch that adds up the
+  // shares costs more (2 x 64 tokens, 4 heads of 16: 17 us for the pass
+  // against 20)
+  if (a.S <= 0 || a.W >= a.Tk || (int64_t)a.Tq * a.G <= 512) return;
   const int64_t groups = ceil_div(a.S, kSinkKeys), bh = (int64_t)a.B * a.Hkv;
   // chunks of at least two tiles until there are items for 4 blocks a CU
   int64_t ch = ceil_div(1024, bh * groups);

@@ -31,23 +31,22 @@ _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
 @functools.lru_cache(maxsize=64)
-def _table(sections: tuple[int, ...], base: float, ladder: str) -> tuple[list[float], list[int]]:
-    """Per pair: frequency in turns per position, axis."""
+def _table(sections: tuple[int, ...], base: float, ladder: str) -> torch.Tensor:
+    """fp64 [pairs, 2] on the CPU: frequency in turns per position, axis."""
     pairs = sum(sections)
-    turn, axis = [], []
+    rows: list[tuple[float, float]] = []
     for a, n in enumerate(sections):
         for i in range(n):
-            e = i / n if ladder == 'per_axis' else len(turn) / pairs
-            turn.append(base ** -e / (2.0 * math.pi))
-            axis.append(a)
-    return turn, axis
+            e = i / n if ladder == 'per_axis' else len(rows) / pairs
+            rows.append((base ** -e / (2.0 * math.pi), float(a)))
+    return torch.tensor(rows, dtype=torch.float64, device='cpu')
 
 
-def _reference(x: torch.Tensor, positions: torch.Tensor, turn: list[float], axis: list[int],
+def _reference(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor,
                halves: bool) -> torch.Tensor:
-    n = len(turn)
+    n = table.shape[0]
     pos = positions if positions.dim() == 3 else positions[None]
-    freq = torch.tensor(turn, dtype=torch.float64, device=x.device) * (2.0 * math.pi)
+    freq, axis = (table[:, 0] * (2.0 * math.pi)).to(x.device), table[:, 1].long().to(x.device)
     ang = pos.double()[..., axis] * freq
     # a 64-bit input keeps its bits; the others are turned in 32
     work = torch.float64 if x.dtype == torch.float64 else torch.float32
@@ -115,9 +114,9 @@ def rotary_axes(
         raise ValueError(f'base must be positive, got {base}')
     if ladder not in ('shared', 'per_axis') or layout not in ('interleaved', 'halves'):
         raise ValueError(f'unknown ladder {ladder!r} or layout {layout!r}')
-    turn, axis = _table(sections, float(base), ladder)
+    table = _table(sections, float(base), ladder)
     if _nat.use_native(q, k):
         return _nat.native().rotary_axes(  # type: ignore[union-attr]
-            q, k, positions, turn, axis, layout == 'halves')
-    return (_reference(q, positions, turn, axis, layout == 'halves'),
-            _reference(k, positions, turn, axis, layout == 'halves'))
+            q, k, positions, table, layout == 'halves')
+    return (_reference(q, positions, table, layout == 'halves'),
+            _reference(k, positions, table, layout == 'halves'))
