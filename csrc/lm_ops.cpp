@@ -225,7 +225,7 @@ struct WindowAttnFn : public torch::autograd::Function<WindowAttnFn> {
       strides3(dv, a.dvs);
       int64_t floats = 0;
       kfac::attn_bwd_plan(a, &a.sink_groups, &a.far_chunks, &floats);
-      TORCH_CHECK((int64_t)(a.Tk + 127) / 128 + (int64_t)a.sink_groups * a.far_chunks <= 65535,
+      TORCH_CHECK((int64_t)(a.Tk + 63) / 64 + (int64_t)a.sink_groups * a.far_chunks <= 65535,
                   "window_attention: more than 65535 key blocks");
       // the sinks' shares (16-byte aligned), then delta
       const at::Tensor ws = at::empty({floats + lse.numel()}, lse.options());

@@ -34,8 +34,7 @@ namespace kfac {
 
 namespace {
 
-constexpr int NT = 256;      // 4 waves
-constexpr int BM = 128;      // rows (or keys) of a block, 32 a wave
+constexpr int NT = 256;      // threads of the joining kernels
 constexpr int BN = 64;       // streamed tile
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kInf = __builtin_inff();
@@ -115,10 +114,18 @@ __device__ __forceinline__ int place_of(int r) {
   else return (r >> 2) & 3;
 }
 
-// waves a SIMD that the row kernels and the key-gradient kernel leave
-// registers for (256 a wave at 2, 512 at 1)
-template <typename T, int DP> constexpr int kRowWaves = sizeof(T) == 2 || DP <= 64 ? 2 : 1;
-template <typename T, int DP> constexpr int kKeyWaves = (sizeof(T) == 2 ? DP <= 64 : DP <= 32) ? 2 : 1;
+// Waves a SIMD that the row kernels and the key-gradient kernel leave
+// registers for (256 a wave at 2, 512 at 1).
+template <typename T, int DP> constexpr int kRowFit = sizeof(T) == 2 || DP <= 64 ? 2 : 1;
+template <typename T, int DP> constexpr int kKeyFit = (sizeof(T) == 2 ? DP <= 64 : DP <= 32) ? 2 : 1;
+
+// Waves of a block.  Rows: 4 (GPT-NeoX batch: forward 39 us, 44 with 2 and 42
+// with 8; 8192 tokens with heads of 128: 94, 148, 115).  Keys: 2 up to heads
+// of 64, where the shorter blocks even out the load (67 us, 74 with 4; fp32
+// padded batch 60, 78), 4 above, where the traffic of the rows weighs more
+// (228 us, 243 with 2).
+constexpr int kRowWaves = 4;
+template <int DP> constexpr int kKeyWaves = DP <= 64 ? 2 : 4;
 
 // accumulator register e of lane half h is tile row (e & 3) + 8 (e >> 2) + 4 h
 __device__ __forceinline__ int acc_row(int e, int h) { return (e & 3) + 8 * (e >> 2) + 4 * h; }
@@ -222,9 +229,9 @@ constexpr uint32_t kNowhere = 0x80000000u;  // an offset that no buffer reaches:
 // lanes; which chunk belongs there is in the offsets, which a tile of rows
 // at a constant stride keeps for its whole life.  Offsets behind the
 // buffer's last byte read zeros.
-template <typename T, int DP>
+template <typename T, int DP, int NW>
 struct Dma {
-  static constexpr int CR = kChunks<T, DP>, CH = BN * CR / NT;
+  static constexpr int NT = 64 * NW, CR = kChunks<T, DP>, CH = BN * CR / NT;
   __device__ __forceinline__ static int row(int n) { return (n * NT + (int)threadIdx.x) / CR; }
   __device__ __forceinline__ static int chunk(int n) {
     return ((n * NT + (int)threadIdx.x) % CR) ^ place_of<CR>(row(n));
@@ -234,10 +241,10 @@ struct Dma {
     return chunk(n) * kUnit<T> < D ? at + chunk(n) * 16 : kNowhere;
   }
   template <typename F>
-  __device__ __forceinline__ static void run(T* L, const T* base, uint32_t bytes, int wave,
+  __device__ __forceinline__ static void run(T* L, const void* base, uint32_t bytes, int wave,
                                              F offset_of) {
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<T*>(base), (short)0, (int)bytes, 0x00020000);
+        const_cast<void*>(base), (short)0, (int)bytes, 0x00020000);
 #pragma unroll
     for (int n = 0; n < CH; ++n)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
@@ -352,7 +359,9 @@ __device__ __forceinline__ void put(O* out, const v16f (&x)[ND], float f, bool z
 }
 
 // What a block of the row kernels (forward, dq) works on.
+template <int NW>
 struct RowBlock {
+  static constexpr int BM = 32 * NW;
   int b, hk, bh, r0, r, t, head, p, h, wave;
   int tiles;
   // keys that some row of this wave sees, and those that all rows see:
@@ -407,39 +416,42 @@ struct RowBlock {
 };
 
 // The K and V tiles of a row block, one after the other.
-template <typename T, int DP>
+template <typename T, int DP, int NW>
 struct KeyStream {
-  typedef Dma<T, DP> D;
-  const T *k, *v;
+  typedef Dma<T, DP, NW> D;
+  const char *k, *v;
   uint32_t ko[D::CH], vo[D::CH];
-  int64_t ks, vs;
+  uint32_t ks, vs;  // bytes from a key to the next
   int wave;
-  __device__ __forceinline__ KeyStream(const AttnArgs& a, const RowBlock& w) {
-    k = reinterpret_cast<const T*>(a.k) + w.b * a.ks[0] + w.hk * a.ks[1];
-    v = reinterpret_cast<const T*>(a.v) + w.b * a.vs[0] + w.hk * a.vs[1];
-    ks = a.ks[2];
-    vs = a.vs[2];
+  __device__ __forceinline__ KeyStream(const AttnArgs& a, const RowBlock<NW>& w) {
+    k = reinterpret_cast<const char*>(reinterpret_cast<const T*>(a.k) + w.b * a.ks[0] +
+                                      w.hk * a.ks[1]);
+    v = reinterpret_cast<const char*>(reinterpret_cast<const T*>(a.v) + w.b * a.vs[0] +
+                                      w.hk * a.vs[1]);
+    ks = (uint32_t)(a.ks[2] * sizeof(T));
+    vs = (uint32_t)(a.vs[2] * sizeof(T));
     wave = w.wave;
 #pragma unroll
     for (int n = 0; n < D::CH; ++n) {
-      ko[n] = D::offset(n, D::row(n) * (uint32_t)(ks * sizeof(T)), a.D);
-      vo[n] = D::offset(n, D::row(n) * (uint32_t)(vs * sizeof(T)), a.D);
+      ko[n] = D::offset(n, D::row(n) * ks, a.D);
+      vo[n] = D::offset(n, D::row(n) * vs, a.D);
     }
   }
   // keys behind kt.hi, and those before the window that are no sinks, read
   // as zeros: nobody sees them, and they may hold anything
   __device__ __forceinline__ void fetch(const AttnArgs& a, const KeyTiles& kt, int j0, T* K,
                                         T* V) const {
-    const int n = kt.hi - j0 < BN ? kt.hi - j0 : BN;
-    const uint32_t kb = (uint32_t)(((n - 1) * ks + a.D) * sizeof(T));
-    const uint32_t vb = (uint32_t)(((n - 1) * vs + a.D) * sizeof(T));
+    const uint32_t last = kt.hi - j0 < BN ? kt.hi - j0 - 1 : BN - 1, row = a.D * sizeof(T);
+    const uint32_t kb = last * ks + row, vb = last * vs + row;
+    const char* kp = k + (uint64_t)(uint32_t)j0 * ks;
+    const char* vp = v + (uint64_t)(uint32_t)j0 * vs;
     if (j0 >= kt.lo) {
-      D::run(K, k + j0 * ks, kb, wave, [&](int i) { return ko[i]; });
-      D::run(V, v + j0 * vs, vb, wave, [&](int i) { return vo[i]; });
+      D::run(K, kp, kb, wave, [&](int i) { return ko[i]; });
+      D::run(V, vp, vb, wave, [&](int i) { return vo[i]; });
     } else {
       auto seen = [&](int i) { return j0 + D::row(i) >= kt.lo || j0 + D::row(i) < a.S; };
-      D::run(K, k + j0 * ks, kb, wave, [&](int i) { return seen(i) ? ko[i] : kNowhere; });
-      D::run(V, v + j0 * vs, vb, wave, [&](int i) { return seen(i) ? vo[i] : kNowhere; });
+      D::run(K, kp, kb, wave, [&](int i) { return seen(i) ? ko[i] : kNowhere; });
+      D::run(V, vp, vb, wave, [&](int i) { return seen(i) ? vo[i] : kNowhere; });
     }
   }
 };
@@ -447,14 +459,14 @@ struct KeyStream {
 // Runs step(K tile, V tile, first key) over key tiles [it0, it1), the next
 // tile on its way while one is worked on.  Two buffers that the compiler can
 // tell apart: it would otherwise wait for the loads before every LDS read.
-template <typename T, int DP, typename F>
-__device__ __forceinline__ void stream_keys(const AttnArgs& a, const RowBlock& w,
+template <typename T, int DP, int NW, typename F>
+__device__ __forceinline__ void stream_keys(const AttnArgs& a, const RowBlock<NW>& w,
                                             const KeyTiles& kt, int it0, int it1, F step) {
   __shared__ __attribute__((aligned(16))) T K0[BN * kLd<T, DP>];
   __shared__ __attribute__((aligned(16))) T K1[BN * kLd<T, DP>];
   __shared__ __attribute__((aligned(16))) T V0[BN * kLd<T, DP>];
   __shared__ __attribute__((aligned(16))) T V1[BN * kLd<T, DP>];
-  const KeyStream<T, DP> ks(a, w);
+  const KeyStream<T, DP, NW> ks(a, w);
   if (it0 < it1) ks.fetch(a, kt, kt.key0(it0), K0, V0);
   for (int it = it0; it < it1; it += 2) {
     arrived();
@@ -468,11 +480,11 @@ __device__ __forceinline__ void stream_keys(const AttnArgs& a, const RowBlock& w
 }
 
 // ---------------------------------------------------------------- forward
-template <typename T, int DP, bool SPLIT>
-__global__ void __launch_bounds__(NT, (kRowWaves<T, DP>)) fwd_kernel(AttnArgs a) {
+template <typename T, int DP, int NW, bool SPLIT>
+__global__ void __launch_bounds__(64 * NW, (kRowFit<T, DP>)) fwd_kernel(AttnArgs a) {
   constexpr int KD = DP / 16, ND = DP / 32;
   typedef typename Ops<T>::frag frag;
-  RowBlock w(a);
+  RowBlock<NW> w(a);
   const KeyTiles kt = w.keys(a);
   const int h = w.h;
   const float c = a.scale * kLog2e;
@@ -493,7 +505,7 @@ __global__ void __launch_bounds__(NT, (kRowWaves<T, DP>)) fwd_kernel(AttnArgs a)
   for (int d = 0; d < ND; ++d) o[d] = zero16();
   float m = -kInf, sum = 0.f;
 
-  stream_keys<T, DP>(a, w, kt, it0, it1, [&](const T* K, const T* V, int j0) {
+  stream_keys<T, DP, NW>(a, w, kt, it0, it1, [&](const T* K, const T* V, int j0) {
 #pragma unroll
     for (int sub = 0; sub < BN / 32; ++sub) {
       const int js = j0 + sub * 32;
@@ -508,8 +520,11 @@ __global__ void __launch_bounds__(NT, (kRowWaves<T, DP>)) fwd_kernel(AttnArgs a)
       for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
       // c > 0: the maximum of the products is the product of the maximum
       mx = halves_max(mx) * c;
-      // the accumulators are rescaled only where a row's maximum grew
-      if (__any(mx > m)) {
+      // The base of a row's powers may lie up to 2^8 below its maximum: sums
+      // and accumulators have the exponents for that (fp16 probabilities end
+      // at 2^16), the quotient at the end does not change, and most tiles of
+      // a row leave its accumulators alone.
+      if (__any(mx > m + 8.f)) {
         const float mn = fmaxf(m, mx);
         const float alpha = ex2(m - (mn == -kInf ? 0.f : mn));
         m = mn;
@@ -621,11 +636,11 @@ __global__ void __launch_bounds__(NT) join_kernel(AttnArgs a) {
 // dq, and delta = do . o for the key-gradient kernel.  The forward's tiles
 // and layout once more: S^T = K Q^T, dP^T = V dO^T, dS^T = P (dP - delta),
 // dQ^T += K^T dS^T.
-template <typename T, int DP>
-__global__ void __launch_bounds__(NT, (kRowWaves<T, DP>)) dq_kernel(AttnArgs a) {
+template <typename T, int DP, int NW>
+__global__ void __launch_bounds__(64 * NW, (kRowFit<T, DP>)) dq_kernel(AttnArgs a) {
   constexpr int KD = DP / 16, ND = DP / 32;
   typedef typename Ops<T>::frag frag;
-  RowBlock w(a);
+  RowBlock<NW> w(a);
   const KeyTiles kt = w.keys(a);
   const int h = w.h;
   const float c = a.scale * kLog2e;
@@ -652,7 +667,7 @@ __global__ void __launch_bounds__(NT, (kRowWaves<T, DP>)) dq_kernel(AttnArgs a) 
   v16f dq[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) dq[d] = zero16();
-  stream_keys<T, DP>(a, w, kt, 0, w.tiles, [&](const T* K, const T* V, int j0) {
+  stream_keys<T, DP, NW>(a, w, kt, 0, w.tiles, [&](const T* K, const T* V, int j0) {
 #pragma unroll
     for (int sub = 0; sub < BN / 32; ++sub) {
       const int js = j0 + sub * 32;
@@ -681,9 +696,15 @@ __global__ void __launch_bounds__(NT, (kRowWaves<T, DP>)) dq_kernel(AttnArgs a) 
                 dq, a.scale, w.p < 0, a.D, h);
 }
 
+__device__ __forceinline__ int clip(int64_t t, const AttnArgs& a) {
+  return (int)(t < 0 ? 0 : (t < a.Tq ? t : a.Tq));
+}
+
 // Rows that look at the keys [k0, k0 + BM): the near ones, whose window
 // reaches there, and, where the block holds sinks, the far ones behind them.
+template <int NW>
 struct RowRange {
+  static constexpr int BM = 32 * NW;
   int n0, n1, f1;  // near [n0, n1), far [n1, f1)
   __device__ __forceinline__ RowRange(int k0, const AttnArgs& a, const Seq& s) {
     const int64_t last = (int64_t)s.len - 1;        // last position
@@ -696,9 +717,6 @@ struct RowRange {
     f1 = k0 < a.S && k0 <= last ? clip(last + 1 - s.start, a) * a.G : n1;
     if (f1 < n1) f1 = n1;
     if (a.far_chunks == 0) n1 = f1;  // no far items: the block takes all rows
-  }
-  __device__ __forceinline__ static int clip(int64_t t, const AttnArgs& a) {
-    return (int)(t < 0 ? 0 : (t < a.Tq ? t : a.Tq));
   }
 };
 
@@ -718,9 +736,9 @@ struct RowBuf {
   float *lse, *delta;
 };
 
-template <typename T, int DP>
+template <typename T, int DP, int NW>
 struct RowStream {
-  typedef Dma<T, DP> D;
+  typedef Dma<T, DP, NW> D;
   const T *q, *g;
   const float *lse, *delta;
   uint32_t qo[D::CH], go[D::CH];
@@ -783,7 +801,7 @@ struct KeyRows {
   int any0, any1, full0, full1, mine0, mine1;
   __device__ __forceinline__ KeyRows(int j0, int key, const AttnArgs& a, const Seq& s) {
     // row of the first token at position p or later
-    auto row = [&](int64_t p) { return RowRange::clip(p - s.start, a) * a.G; };
+    auto row = [&](int64_t p) { return clip(p - s.start, a) * a.G; };
     const int64_t last = s.len, w = a.W;
     any0 = row(j0);
     any1 = row(j0 < a.S || j0 + 31 + w > last ? last : j0 + 31 + w);
@@ -868,28 +886,29 @@ struct KeyGrad {
 // which all waves own together, 32 rows each of a tile of 128; their sums
 // are added in wave order.  Sinks are few and the rows behind the window
 // many, so a far item has its rows spread over the waves and not its keys.
-template <typename T, int DP>
-__global__ void __launch_bounds__(NT, (kKeyWaves<T, DP>)) dkv_kernel(AttnArgs a, int key_blocks) {
-  constexpr int ND = DP / 32, LD = kLd<T, DP>;
+template <typename T, int DP, int NW>
+__global__ void __launch_bounds__(64 * NW, (kKeyFit<T, DP>)) dkv_kernel(AttnArgs a, int key_blocks) {
+  constexpr int ND = DP / 32, LD = kLd<T, DP>, NT = 64 * NW, BM = 32 * NW;
   __shared__ __attribute__((aligned(16))) T Q0[BN * LD];
   __shared__ __attribute__((aligned(16))) T Q1[BN * LD];
   __shared__ __attribute__((aligned(16))) T G0[BN * LD];
   __shared__ __attribute__((aligned(16))) T G1[BN * LD];
   __shared__ __attribute__((aligned(16))) float L0[BN], L1[BN], D0[BN], D1[BN];
   static_assert(BN * LD * sizeof(T) >= kSinkKeys * DP * sizeof(float), "sums of a far item");
+  static_assert(NW == 2 || NW == 4, "two waves or four");
   const RowBuf<T> b0{Q0, G0, L0, D0}, b1{Q1, G1, L1, D1};
   const int bh = blockIdx.x, b = bh / a.Hkv, hk = bh - b * a.Hkv;
   const int l = threadIdx.x & 63, h = l >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Seq seq = sequence(a, b);
-  const RowStream<T, DP> rs(a, b, hk, wave);
+  const RowStream<T, DP, NW> rs(a, b, hk, wave);
   KeyGrad<T, DP> kg;
 
   if ((int)blockIdx.y >= key_blocks) {
     const int item = (int)blockIdx.y - key_blocks;
     const int group = item / a.far_chunks, chunk = item - group * a.far_chunks;
     const int j0 = group * kSinkKeys, key = j0 + (l & 31);
-    const RowRange rr(j0 / BM * BM, a, seq);
+    const RowRange<NW> rr(j0 / BM * BM, a, seq);
     const int tokens = (rr.f1 - rr.n1) / a.G;
     const int per = (tokens + a.far_chunks - 1) / a.far_chunks * a.G;
     const int ra = rr.n1 + per * chunk < rr.f1 ? rr.n1 + per * chunk : rr.f1;
@@ -899,14 +918,14 @@ __global__ void __launch_bounds__(NT, (kKeyWaves<T, DP>)) dkv_kernel(AttnArgs a,
     for (int t0 = ra; t0 < rb; t0 += BM) {
       __syncthreads();
       rs.fetch(a, t0, rb, b0);
-      rs.fetch(a, t0 + BN, rb, b1);
+      if (NW > 2) rs.fetch(a, t0 + BN, rb, b1);
       arrived();
       if (t0 + wave * 32 < rb)
-        kg.rows(a, wave < 2 ? b0 : b1, (wave & 1) * 32, t0 + wave * 32, kr);
+        kg.rows(a, NW <= 2 || wave < 2 ? b0 : b1, (wave & 1) * 32, t0 + wave * 32, kr);
     }
     float* sk = reinterpret_cast<float*>(Q0);
     float* sv = reinterpret_cast<float*>(G0);
-    for (int turn = 0; turn < NT / 64; ++turn) {
+    for (int turn = 0; turn < NW; ++turn) {
       __syncthreads();
       if (wave == turn) {
 #pragma unroll
@@ -939,7 +958,7 @@ __global__ void __launch_bounds__(NT, (kKeyWaves<T, DP>)) dkv_kernel(AttnArgs a,
   }
 
   const int k0 = (int)blockIdx.y * BM;
-  const RowRange rr(k0, a, seq);
+  const RowRange<NW> rr(k0, a, seq);
   const int key = k0 + wave * 32 + (l & 31);
   const KeyRows kr(k0 + wave * 32, key, a, seq);
   kg.init(a, b, hk, key, key < seq.len);
@@ -992,27 +1011,28 @@ __global__ void __launch_bounds__(NT) join_kv_kernel(AttnArgs a) {
       __builtin_convertvector(f, typename Ops<T>::quad);
 }
 
-unsigned row_blocks(const AttnArgs& a) {
-  return (unsigned)ceil_div((int64_t)a.Tq * a.G, BM);
-}
-
 template <typename T, int DP>
 void forward_dp(const AttnArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)(a.B * a.Hkv), row_blocks(a), (unsigned)a.splits);
+  constexpr int NW = kRowWaves;
+  const dim3 grid((unsigned)(a.B * a.Hkv), (unsigned)ceil_div((int64_t)a.Tq * a.G, 32 * NW),
+                  (unsigned)a.splits);
   if (a.splits > 1) {
-    fwd_kernel<T, DP, true><<<grid, NT, 0, st>>>(a);
+    fwd_kernel<T, DP, NW, true><<<grid, 64 * NW, 0, st>>>(a);
     join_kernel<T><<<(unsigned)(a.B * a.Hq * a.Tq), NT, 0, st>>>(a);
   } else {
-    fwd_kernel<T, DP, false><<<grid, NT, 0, st>>>(a);
+    fwd_kernel<T, DP, NW, false><<<grid, 64 * NW, 0, st>>>(a);
   }
 }
 
 template <typename T, int DP>
 void backward_dp(const AttnArgs& a, hipStream_t st) {
+  constexpr int QN = kRowWaves, KN = kKeyWaves<DP>;
   const unsigned bh = (unsigned)(a.B * a.Hkv);
-  dq_kernel<T, DP><<<dim3(bh, row_blocks(a)), NT, 0, st>>>(a);
-  const int kb = (int)ceil_div(a.Tk, BM);
-  dkv_kernel<T, DP><<<dim3(bh, (unsigned)(kb + a.sink_groups * a.far_chunks)), NT, 0, st>>>(a, kb);
+  dq_kernel<T, DP, QN><<<dim3(bh, (unsigned)ceil_div((int64_t)a.Tq * a.G, 32 * QN)), 64 * QN, 0,
+                         st>>>(a);
+  const int kb = (int)ceil_div(a.Tk, 32 * KN);
+  dkv_kernel<T, DP, KN><<<dim3(bh, (unsigned)(kb + a.sink_groups * a.far_chunks)), 64 * KN, 0,
+                          st>>>(a, kb);
   if (a.far_chunks > 0) {
     const int64_t n = (int64_t)bh * a.S * 2 * (a.D / 4);
     join_kv_kernel<T><<<(unsigned)ceil_div(n, NT), NT, 0, st>>>(a);
@@ -1039,9 +1059,9 @@ void backward_type(const AttnArgs& a, hipStream_t st) {
 
 void attn_plan(const AttnArgs& a, int* splits, int64_t* floats) {
   const int64_t rows = (int64_t)a.Tq * a.G;
-  const int64_t blocks = (int64_t)a.B * a.Hkv * ceil_div(rows, BM);
+  const int64_t blocks = (int64_t)a.B * a.Hkv * ceil_div(rows, 32 * kRowWaves);
   // tiles that the longest row block can see
-  const int64_t most = ceil_div(std::min<int64_t>((int64_t)a.W + BM, a.Tk), BN) +
+  const int64_t most = ceil_div(std::min<int64_t>((int64_t)a.W + 128, a.Tk), BN) +
                        ceil_div(std::min<int64_t>(a.S, a.Tk), BN) + 1;
   int64_t s = 1;
   if (blocks > 0 && blocks < 256) {
@@ -1071,7 +1091,7 @@ void attn_bwd_plan(const AttnArgs& a, int* sink_groups, int* far_chunks, int64_t
   const int64_t groups = ceil_div(a.S, kSinkKeys), bh = (int64_t)a.B * a.Hkv;
   // chunks of at least two tiles until there are items for 4 blocks a CU
   int64_t ch = ceil_div(1024, bh * groups);
-  ch = std::min(ch, ceil_div((int64_t)a.Tq * a.G, 2 * BM));
+  ch = std::min(ch, ceil_div((int64_t)a.Tq * a.G, 256));
   ch = std::max<int64_t>(1, std::min<int64_t>(ch, 32));
   *sink_groups = (int)groups;
   *far_chunks = (int)ch;
