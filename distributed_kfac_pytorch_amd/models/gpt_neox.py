@@ -10,8 +10,11 @@ factors) and the TP/PP tests.  Per block (NeoX "parallel residual"):
     MLP:  h_to_4h = ColumnParallelLinear(h, 4h, gather_output=False) -> GELU
           -> 4h_to_h = RowParallelLinear(4h, h, input_is_parallel=True)
 
-Rotary position embeddings on the full head dim; token embedding and LM
-head replicated (the reference registers only the parallel linears).
+Rotary position embeddings on the full head dim; with ``attention_window`` /
+``attention_sinks`` or ``rotary_sections`` the block rotates and attends
+through the native operators (``ops.rotary``, ``ops.attention``): a sliding
+window with a few first tokens that stay visible, positions with several axes.
+Token embedding and LM head replicated (the reference registers only the parallel linears).
 ``gpt_neox_125m()`` = hidden 768, 12 layers, 12 heads, seq 2048, which gives
 48 K-FAC layers with factor dims up to 3073.
 """
@@ -23,6 +26,8 @@ import torch.nn.functional as F
 
 from distributed_kfac_pytorch_amd.neox.tp_layers import ColumnParallelLinear
 from distributed_kfac_pytorch_amd.neox.tp_layers import RowParallelLinear
+from distributed_kfac_pytorch_amd.ops.attention import window_attention
+from distributed_kfac_pytorch_amd.ops.rotary import rotary_axes
 from distributed_kfac_pytorch_amd.parallel.comm import get_world_size
 
 
@@ -38,13 +43,42 @@ def _rotary(x: torch.Tensor, base: float = 10000.0) -> torch.Tensor:
 
 
 class ParallelAttention(torch.nn.Module):
-    def __init__(self, hidden: int, heads: int, group: dist.ProcessGroup | None, seed: int) -> None:
+    """Self-attention of a block.
+
+    ``window``: tokens a token sees, itself included, plus the first ``sinks``
+    tokens (default: all before it).  ``rotary_sections``: pairs of a head
+    that each position axis turns (default: all pairs by one axis).  Either
+    selects the native rotary and attention operators; without them the block
+    runs ``scaled_dot_product_attention`` over the whole prefix.
+    """
+
+    def __init__(
+        self,
+        hidden: int,
+        heads: int,
+        group: dist.ProcessGroup | None,
+        seed: int,
+        window: int | None = None,
+        sinks: int = 0,
+        rotary_sections: tuple[int, ...] | None = None,
+    ) -> None:
         super().__init__()
         mp = get_world_size(group)
         if heads % mp != 0:
             raise ValueError('heads must be divisible by the MP size')
         self.local_heads = heads // mp
         self.head_dim = hidden // heads
+        if window is None and sinks != 0:
+            raise ValueError('attention sinks need an attention window')
+        if window is not None and (window < 1 or sinks < 0):
+            raise ValueError(f'window must be at least 1 and sinks at least 0, got {window}, {sinks}')
+        self.native = window is not None or rotary_sections is not None
+        if self.native and (self.head_dim % 8 != 0 or self.head_dim > 128):
+            raise ValueError('windowed attention and position axes need a head size that is a '
+                             f'multiple of 8, at most 128, got {self.head_dim}')
+        self.window = window
+        self.sinks = sinks
+        self.rotary_sections = tuple(rotary_sections or (self.head_dim // 2,))
         self.query_key_value = ColumnParallelLinear(
             hidden, 3 * hidden, gather_output=False, group=group, init_seed=seed,
         )
@@ -52,12 +86,21 @@ class ParallelAttention(torch.nn.Module):
             hidden, hidden, input_is_parallel=True, group=group, init_seed=seed + 1,
         )
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, positions: torch.Tensor | None = None) -> torch.Tensor:
         b, t, _ = x.shape
         qkv = self.query_key_value(x).view(b, t, self.local_heads, 3 * self.head_dim)
         q, k, v = qkv.permute(0, 2, 1, 3).split(self.head_dim, dim=-1)
-        q, k = _rotary(q), _rotary(k)
-        o = F.scaled_dot_product_attention(q, k, v, is_causal=True)
+        if self.native:
+            if positions is None:
+                positions = torch.arange(t, device=x.device)[:, None].expand(
+                    t, len(self.rotary_sections))
+            q, k = rotary_axes(q, k, positions, sections=self.rotary_sections)
+            o = window_attention(q, k, v, window=self.window or max(t, 1), sinks=self.sinks)
+        else:
+            if positions is not None:
+                raise ValueError('positions need rotary_sections (or attention_window)')
+            q, k = _rotary(q), _rotary(k)
+            o = F.scaled_dot_product_attention(q, k, v, is_causal=True)
         o = o.permute(0, 2, 1, 3).reshape(b, t, self.local_heads * self.head_dim)
         return self.dense(o)
 
@@ -77,15 +120,25 @@ class ParallelMLP(torch.nn.Module):
 
 
 class GPTNeoXBlock(torch.nn.Module):
-    def __init__(self, hidden: int, heads: int, group: dist.ProcessGroup | None, seed: int) -> None:
+    def __init__(
+        self,
+        hidden: int,
+        heads: int,
+        group: dist.ProcessGroup | None,
+        seed: int,
+        window: int | None = None,
+        sinks: int = 0,
+        rotary_sections: tuple[int, ...] | None = None,
+    ) -> None:
         super().__init__()
         self.input_layernorm = torch.nn.LayerNorm(hidden)
         self.post_attention_layernorm = torch.nn.LayerNorm(hidden)
-        self.attention = ParallelAttention(hidden, heads, group, seed)
+        self.attention = ParallelAttention(hidden, heads, group, seed, window, sinks,
+                                           rotary_sections)
         self.mlp = ParallelMLP(hidden, group, seed + 2)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
-        return x + self.attention(self.input_layernorm(x)) + self.mlp(
+    def forward(self, x: torch.Tensor, positions: torch.Tensor | None = None) -> torch.Tensor:
+        return x + self.attention(self.input_layernorm(x), positions) + self.mlp(
             self.post_attention_layernorm(x),
         )
 
@@ -142,19 +195,26 @@ class GPTNeoX(torch.nn.Module):
         layers: int = 12,
         heads: int = 12,
         group: dist.ProcessGroup | None = None,
+        attention_window: int | None = None,
+        attention_sinks: int = 0,
+        rotary_sections: tuple[int, ...] | None = None,
     ) -> None:
         super().__init__()
         self.embed_in = _seeded_embedding(vocab, hidden, EMBED_SEED)
         self.layers = torch.nn.ModuleList(
-            [GPTNeoXBlock(hidden, heads, group, seed=100 * i) for i in range(layers)],
+            [GPTNeoXBlock(hidden, heads, group, 100 * i, attention_window, attention_sinks,
+                          rotary_sections) for i in range(layers)],
         )
         self.final_layer_norm = torch.nn.LayerNorm(hidden)
         self.embed_out = _seeded_head(hidden, vocab, HEAD_SEED)
 
-    def forward(self, tokens: torch.Tensor) -> torch.Tensor:
+    def forward(self, tokens: torch.Tensor, positions: torch.Tensor | None = None) -> torch.Tensor:
+        """Logits ``[B, T, vocab]``.  ``positions``: integer ``[T, axes]`` or
+        ``[B, T, axes]`` with one axis per entry of ``rotary_sections``
+        (default: a token's index on every axis)."""
         x = self.embed_in(tokens)
         for blk in self.layers:
-            x = blk(x)
+            x = blk(x, positions)
         return self.embed_out(self.final_layer_norm(x))
 
 
@@ -164,13 +224,16 @@ def gpt_neox_pipeline_layers(
     layers: int = 12,
     heads: int = 12,
     group: dist.ProcessGroup | None = None,
+    attention_window: int | None = None,
+    attention_sinks: int = 0,
 ) -> list:
     """Layer constructors for ``neox.pipeline.PipelineModule``: embedding,
     the blocks, the head -- weight for weight the layers of ``GPTNeoX`` with
     the same arguments, whatever the stage partition."""
     out: list = [lambda: GPTNeoXEmbedding(vocab, hidden)]
     for i in range(layers):
-        out.append(lambda i=i: GPTNeoXBlock(hidden, heads, group, seed=100 * i))
+        out.append(lambda i=i: GPTNeoXBlock(hidden, heads, group, 100 * i, attention_window,
+                                            attention_sinks))
     out.append(lambda: GPTNeoXHead(hidden, vocab))
     return out
 

@@ -19,6 +19,8 @@ from typing import Callable
 import torch
 import torch.distributed as dist
 
+from distributed_kfac_pytorch_amd.ops.distill import topk_distill_loss
+
 
 def save_checkpoint(
     model: torch.nn.Module,
@@ -78,6 +80,28 @@ class LabelSmoothLoss(torch.nn.Module):
         weight = torch.full_like(log_prob, self.smoothing / (k - 1))
         weight.scatter_(-1, target.unsqueeze(-1), 1.0 - self.smoothing)
         return (-weight * log_prob).sum(dim=-1).mean()
+
+
+class TopKDistillLoss(torch.nn.Module):
+    """Distillation from a teacher's top logits (``ops.distill``): the
+    divergence from the teacher's distribution over its ``K`` best entries
+    (and, with ``teacher_rest``, the rest of the vocabulary) to the student's.
+    ``weight`` is a factor of the loss, cheaper here than multiplied on later."""
+
+    def __init__(self, temperature: float = 1.0, weight: float = 1.0,
+                 reduction: str = 'mean') -> None:
+        super().__init__()
+        self.temperature = temperature
+        self.weight = weight
+        self.reduction = reduction
+
+    def forward(self, input: torch.Tensor, teacher_logits: torch.Tensor,
+                teacher_index: torch.Tensor,
+                teacher_rest: torch.Tensor | None = None) -> torch.Tensor:
+        return topk_distill_loss(
+            input, teacher_logits, teacher_index, teacher_rest=teacher_rest,
+            temperature=self.temperature, weight=self.weight, reduction=self.reduction,
+        )
 
 
 class Metric:

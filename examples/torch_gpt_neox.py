@@ -11,6 +11,14 @@ the ``--mp`` ranks of a model-parallel group, DDP averages gradients over the
 data-parallel group, and ``GPTNeoXKFACPreconditioner`` gathers the sharded
 activations / gradients to one primary rank per MP group, preconditions the
 full matrices there and scatters the result back.  Synthetic token data.
+
+``--attention-window`` / ``--attention-sinks`` train with a sliding window;
+``--teacher FILE`` (a checkpoint that ``--save`` wrote) adds distillation from
+the teacher's ``--distill-topk`` best logits to the loss:
+
+    python examples/torch_gpt_neox.py --steps 50 --save teacher.pt
+    python examples/torch_gpt_neox.py --steps 50 --attention-window 256 \
+        --attention-sinks 4 --teacher teacher.pt --distill-weight 0.5
 """
 from __future__ import annotations
 
@@ -31,6 +39,9 @@ from distributed_kfac_pytorch_amd.neox.pipeline import PipelineModule  # noqa: E
 from distributed_kfac_pytorch_amd.neox.pipeline import allreduce_gradients  # noqa: E402
 from distributed_kfac_pytorch_amd.neox.preconditioner import GPTNeoXKFACPreconditioner  # noqa: E402
 from distributed_kfac_pytorch_amd.neox.topology import PipeModelDataParallelTopology  # noqa: E402
+from distributed_kfac_pytorch_amd.utils.training import TopKDistillLoss  # noqa: E402
+from distributed_kfac_pytorch_amd.utils.training import load_checkpoint  # noqa: E402
+from distributed_kfac_pytorch_amd.utils.training import save_checkpoint  # noqa: E402
 from examples import cli  # noqa: E402
 
 MODELS = {
@@ -59,6 +70,17 @@ def parse_args(argv: list[str] | None = None) -> argparse.Namespace:
     p.add_argument('--factor-checkpoint-dir', default=None,
                    help='save K-FAC factors as per-layer files here at the end')
     p.add_argument('--log-interval', type=int, default=5)
+    p.add_argument('--attention-window', type=int, default=0,
+                   help='tokens a token sees, itself included (0: all before it)')
+    p.add_argument('--attention-sinks', type=int, default=0,
+                   help='first tokens that stay visible behind the window')
+    p.add_argument('--teacher', default=None,
+                   help='model checkpoint (--save) to distill from; needs --mp 1 --pp 1')
+    p.add_argument('--distill-topk', type=int, default=64, help='teacher entries kept a token')
+    p.add_argument('--distill-temperature', type=float, default=2.0)
+    p.add_argument('--distill-weight', type=float, default=0.5,
+                   help='share of the distillation in the loss')
+    p.add_argument('--save', default=None, help='write a model checkpoint here at the end')
     cli.add_runtime_args(p)
     return p.parse_args(argv)
 
@@ -84,19 +106,28 @@ def main(argv: list[str] | None = None) -> dict[str, float]:
         raise ValueError(f'world size {args.world_size} is not divisible by --mp x --pp')
     if args.micro_batch % args.micro_batches != 0:
         raise ValueError('--micro-batch must be divisible by --micro-batches')
+    if (args.teacher or args.save) and args.mp * args.pp != 1:
+        raise ValueError('--teacher and --save need --mp 1 --pp 1')
     dp = args.world_size // (args.mp * args.pp)
     topo = PipeModelDataParallelTopology(num_pp=args.pp, num_mp=args.mp, num_dp=dp)
     mp_group, dp_group, pipe_group = build_groups(topo, args.rank)
     cfg = MODELS[args.model]
     torch.manual_seed(args.seed)
+    shape = dict(vocab=cfg['vocab'], hidden=cfg['hidden'], layers=cfg['layers'],
+                 heads=cfg['heads'], group=mp_group)
+    window = dict(attention_window=args.attention_window or None,
+                  attention_sinks=args.attention_sinks)
     if args.pp > 1:
         # embedding, blocks and head as separate pipeline layers
-        layers = gpt_neox_pipeline_layers(vocab=cfg['vocab'], hidden=cfg['hidden'],
-                                          layers=cfg['layers'], heads=cfg['heads'],
-                                          group=mp_group)
+        layers = gpt_neox_pipeline_layers(**shape, **window)
     else:
-        layers = [lambda: GPTNeoX(vocab=cfg['vocab'], hidden=cfg['hidden'], layers=cfg['layers'],
-                                  heads=cfg['heads'], group=mp_group)]
+        layers = [lambda: GPTNeoX(**shape, **window)]
+    teacher, distill = None, None
+    if args.teacher:
+        teacher = GPTNeoX(**shape).requires_grad_(False).eval()
+        teacher.load_state_dict(load_checkpoint(args.teacher, map_location='cpu')['model'])
+        teacher = teacher.to(args.device)
+        distill = TopKDistillLoss(args.distill_temperature, args.distill_weight)
     model = PipelineModule(layers, topo, rank=args.rank).to(args.device)
     if args.pp > 1:
         return _train_pipeline(args, model, topo, cfg, mp_group, dp_group, pipe_group)
@@ -142,6 +173,10 @@ def main(argv: list[str] | None = None) -> dict[str, float]:
         loss = torch.nn.functional.cross_entropy(
             logits.float().flatten(0, 1), tokens[:, 1:].flatten(),
         )
+        if teacher is not None:
+            with torch.no_grad(), ctx:
+                best, index = teacher(tokens[:, :-1]).topk(args.distill_topk, dim=-1)
+            loss = (1.0 - args.distill_weight) * loss + distill(logits, best, index)
         loss.backward()
         if pre is not None:
             pre.step()
@@ -159,6 +194,9 @@ def main(argv: list[str] | None = None) -> dict[str, float]:
     if pre is not None and args.factor_checkpoint_dir:
         pre.state_dict()  # writes the per-layer factor files
         cli.log(args, f'factors saved under {args.factor_checkpoint_dir}')
+    if args.save and args.rank == 0:
+        net = model.module if dp > 1 else model
+        save_checkpoint(net.layers[0], optimizer, None, None, args.save)
     return out
 
 
