@@ -9,7 +9,9 @@ import torch
 
 from distributed_kfac_pytorch_amd.models.gpt_neox import GPTNeoX
 from distributed_kfac_pytorch_amd.models.gpt_neox import gpt_neox_pipeline_layers
+from distributed_kfac_pytorch_amd.neox.pipeline import PipelineModule
 from distributed_kfac_pytorch_amd.neox.preconditioner import GPTNeoXKFACPreconditioner
+from distributed_kfac_pytorch_amd.neox.topology import PipeModelDataParallelTopology
 from distributed_kfac_pytorch_amd.utils.training import TopKDistillLoss
 from distributed_kfac_pytorch_amd.warnings import ExperimentalFeatureWarning
 from tests import lm_reference as ref
@@ -151,7 +153,9 @@ def test_model_on_the_gpu_matches_64_bits(cuda):
 def test_kfac_step_on_the_gpu(cuda, dtype):
     """K-FAC over the windowed model with distillation: every factor and
     preconditioned gradient is finite, and all eight linears are registered."""
-    model = GPTNeoX(**SHAPE, attention_window=16, attention_sinks=2).to(cuda)
+    topo = PipeModelDataParallelTopology(num_pp=1, num_mp=1, num_dp=1)
+    model = PipelineModule(
+        [lambda: GPTNeoX(**SHAPE, attention_window=16, attention_sinks=2)], topo, rank=0).to(cuda)
     pre = GPTNeoXKFACPreconditioner(model, factor_update_steps=1, inv_update_steps=1, lr=0.1)
     assert len(pre._layers) == 8
     tok = _tokens(4, 65).to(cuda)
