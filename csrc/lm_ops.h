@@ -79,7 +79,7 @@ struct AttnArgs {
   void* out;                    // [B, Hq, Tq, D] with strides os
   int64_t os[3];
   float* lse;                   // [B * Hkv, Tq * G] (rows), log2 units; +inf: sees nothing
-  float* delta;                 // the same
+  float* delta;                 // the same: -do . o
   void *dq, *dk, *dv;
   int64_t dqs[3], dks[3], dvs[3];
   const int* lengths;           // [B] or null

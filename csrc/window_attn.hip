@@ -633,7 +633,7 @@ __global__ void __launch_bounds__(NT) join_kernel(AttnArgs a) {
 }
 
 // --------------------------------------------------------------- backward
-// dq, and delta = do . o for the key-gradient kernel.  The forward's tiles
+// dq, and -delta = -do . o for the key-gradient kernel.  The forward's tiles
 // and layout once more: S^T = K Q^T, dP^T = V dO^T, dS^T = P (dP - delta),
 // dQ^T += K^T dS^T.
 template <typename T, int DP, int NW>
@@ -659,11 +659,18 @@ __global__ void __launch_bounds__(64 * NW, (kRowFit<T, DP>)) dq_kernel(AttnArgs 
 #pragma unroll
     for (int i = 0; i < 8; ++i) delta += (float)gf[k][i] * (float)of[i];
   }
-  delta = halves_sum(delta);
+  delta = -halves_sum(delta);
   const int64_t at = (int64_t)w.bh * (a.Tq * a.G) + w.r;
   if (w.live && h == 0) a.delta[at] = delta;
   const float lse = w.p >= 0 ? a.lse[at] : kInf;
 
+  // dP - delta comes out of the matrix units: they start from -delta (in fp32
+  // with heads over 32, whose registers are full, it is added afterwards)
+  constexpr bool kStart = sizeof(T) == 2 || DP <= 32;
+  v16f minus = zero16();
+#pragma unroll
+  for (int e = 0; e < 16; ++e)
+    if (kStart) minus[e] = delta;
   v16f dq[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) dq[d] = zero16();
@@ -673,7 +680,7 @@ __global__ void __launch_bounds__(64 * NW, (kRowFit<T, DP>)) dq_kernel(AttnArgs 
       const int js = j0 + sub * 32;
       const int cover = w.coverage(js, a.S);
       if (cover == 0) continue;
-      v16f s = zero16(), dp = zero16();
+      v16f s = zero16(), dp = minus;
 #pragma unroll
       for (int k = 0; k < KD; ++k) {
         s = Ops<T>::mma(row_frag<T, DP>(K, sub * 32, k), qf[k], s);
@@ -681,7 +688,7 @@ __global__ void __launch_bounds__(64 * NW, (kRowFit<T, DP>)) dq_kernel(AttnArgs 
       }
       if (cover == 1) hide(s, w.seen(js, a));
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] = ex2(__builtin_fmaf(s[e], c, -lse)) * (dp[e] - delta);
+      for (int e = 0; e < 16; ++e) s[e] = ex2(__builtin_fmaf(s[e], c, -lse)) * (kStart ? dp[e] : dp[e] + delta);
 #pragma unroll
       for (int ss = 0; ss < 2; ++ss) {
         const frag sf = acc_frag<T>(s, ss);
@@ -851,7 +858,13 @@ struct KeyGrad {
     if (cover == 0) return;
     const int h = (threadIdx.x & 63) >> 5;
     const float c = a.scale * kLog2e;
-    v16f s = zero16(), dp = zero16();
+    v16f s = zero16(), dp;
+#pragma unroll
+    for (int e4 = 0; e4 < 4; ++e4) {
+      const v4f de = *reinterpret_cast<const v4f*>(b.delta + i0 + acc_row(e4 * 4, h));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) dp[e4 * 4 + i] = de[i];
+    }
 #pragma unroll
     for (int k = 0; k < KD; ++k) {
       s = Ops<T>::mma(row_frag<T, DP>(b.q, i0, k), kf[k], s);
@@ -861,12 +874,11 @@ struct KeyGrad {
 #pragma unroll
     for (int e4 = 0; e4 < 4; ++e4) {
       const v4f le = *reinterpret_cast<const v4f*>(b.lse + i0 + acc_row(e4 * 4, h));
-      const v4f de = *reinterpret_cast<const v4f*>(b.delta + i0 + acc_row(e4 * 4, h));
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int e = e4 * 4 + i;
         s[e] = ex2(__builtin_fmaf(s[e], c, -le[i]));
-        dp[e] = s[e] * (dp[e] - de[i]);
+        dp[e] *= s[e];
       }
     }
 #pragma unroll
