@@ -75,7 +75,9 @@ __device__ __forceinline__ void store_wide(E* p, const float* f) {
   else *reinterpret_cast<uvec*>(p) = v;
 }
 
-// running (maximum, sum of 2^(y - maximum)); (-inf, 0) is empty
+// A sum of powers, as (base m, sum s of 2^(y - m)); s = 0 is empty.  It stays
+// in two parts to the end: m + log2 s rounds to a step of m's size, which
+// would put the same 2^-24 m on every probability of the row.
 struct Run {
   float m, s;
   __device__ __forceinline__ void join(float m2, float s2) {
@@ -84,15 +86,23 @@ struct Run {
     s = s * ex2(m - base) + s2 * ex2(m2 - base);
     m = mm;
   }
-  __device__ __forceinline__ float log2sum() const {
-    return s == 0.f ? KFAC_NEG_INF : m + log2f(s);
+  // 2^(x c), the product not rounded
+  __device__ __forceinline__ void add(float x, float c) {
+    const float y = x * c;
+    join(y, y == KFAC_NEG_INF ? 0.f : ex2(__builtin_fmaf(x, c, -y)));
+  }
+  // 2^(x c) as a part of the sum
+  __device__ __forceinline__ float part(float x, float c) const {
+    return ex2(__builtin_fmaf(x, c, -m)) / s;
+  }
+  __device__ __forceinline__ float log2part(float x, float c) const {
+    return __builtin_fmaf(x, c, -m) - log2f(s);
   }
 };
 
-__device__ __forceinline__ float add_log2(float a, float b) {
-  Run r{a, a == KFAC_NEG_INF ? 0.f : 1.f};
-  r.join(b, b == KFAC_NEG_INF ? 0.f : 1.f);
-  return r.log2sum();
+__device__ __forceinline__ Run joined(Run a, Run b) {
+  a.join(b.m, b.s);
+  return a;
 }
 
 __device__ __forceinline__ Run wave_join(Run r) {
@@ -114,67 +124,99 @@ __device__ __forceinline__ const E* row_of(const DistillArgs& a, int64_t n) {
   return reinterpret_cast<const E*>(a.z) + (n / a.inner) * a.zs0 + (n % a.inner) * a.zs1;
 }
 
-// The teacher's side of a row, by one wave.
-struct Teacher {
-  float norm, rest, r;  // log2 sum of its entries and rest; log2 rest; the rest's share
-  bool counts;          // the row has entries, and they or the rest have mass
-  bool outside;         // an index behind the vocabulary
-  __device__ __forceinline__ Teacher(const DistillArgs& a, int64_t n) {
-    const int lane = threadIdx.x & 63;
-    const float c = kLog2e / a.temperature;
-    rest = a.rest != nullptr ? a.rest[n] * kLog2e : KFAC_NEG_INF;
-    Run t{KFAC_NEG_INF, 0.f};
-    bool some = false, far = false;
-    for (int k = lane; k < a.K; k += 64) {
-      const int64_t j = index_at(a, n * a.K + k);
-      if (j < 0) continue;
-      some = true;
-      far |= j >= a.V;
-      const float y = a.teacher[n * a.K + k] * c;
-      t.join(y, y == KFAC_NEG_INF ? 0.f : 1.f);
-    }
-    t = wave_join(t);
-    outside = __any(far);
-    norm = add_log2(t.log2sum(), rest);
-    r = a.rest != nullptr && rest != KFAC_NEG_INF ? ex2(rest - norm) : 0.f;
-    counts = __any(some) && norm != KFAC_NEG_INF;
-  }
+// A row's statistics, as the backward pass finds them.
+struct RowInfo {
+  Run all, tail;  // the student's columns; those outside I (with a rest)
+  Run teacher;
+  float r;        // the rest's share of the teacher; -1: the row does not count
+  float unused;
 };
 
-// A row's loss, by one wave.  tail / lse: log2 sums of the student's columns
-// outside I (with a rest) and of all columns; both NaN where an index lies
-// behind the vocabulary.
-template <typename E>
-__device__ float row_loss(const DistillArgs& a, int64_t n, const Teacher& t, float lse,
-                          float tail) {
+__device__ __forceinline__ RowInfo load_info(const DistillArgs& a, int64_t n) {
+  const float4 u = a.info[2 * n], v = a.info[2 * n + 1];
+  return RowInfo{{u.x, u.y}, {u.z, u.w}, {v.x, v.y}, v.z, v.w};
+}
+
+__device__ __forceinline__ void store_info(const DistillArgs& a, int64_t n, const RowInfo& i) {
+  a.info[2 * n] = make_float4(i.all.m, i.all.s, i.tail.m, i.tail.s);
+  a.info[2 * n + 1] = make_float4(i.teacher.m, i.teacher.s, i.r, i.unused);
+}
+
+// The teacher's part of a row's info, by one wave.  An index behind the
+// vocabulary makes the teacher's sum NaN, and with it the loss and gradient.
+__device__ __forceinline__ void teacher_of(const DistillArgs& a, int64_t n, RowInfo& info) {
+  const int lane = threadIdx.x & 63;
   const float c = kLog2e / a.temperature;
-  const E* z = row_of<E>(a, n);
+  const float rest = a.rest != nullptr ? a.rest[n] : KFAC_NEG_INF;
+  Run t{KFAC_NEG_INF, 0.f};
+  bool some = false, far = false;
+  for (int k = lane; k < a.K; k += 64) {
+    const int64_t j = index_at(a, n * a.K + k);
+    if (j < 0) continue;
+    some = true;
+    far |= j >= a.V;
+    t.add(a.teacher[n * a.K + k], c);
+  }
+  t = wave_join(t);
+  t.add(rest, kLog2e);
+  if (__any(far)) t.s = __builtin_nanf("");
+  info.teacher = t;
+  info.r = !__any(some) || t.s == 0.f ? -1.f
+           : rest == KFAC_NEG_INF     ? 0.f
+                                      : t.part(rest, kLog2e);
+}
+
+// A row's loss, by one wave; raw(k, j) is the student's logit of entry k.
+// Each entry's two log-probabilities meet before they are weighted: apart,
+// the rounding of the weights would be multiplied by the row's logarithm.
+template <typename F>
+__device__ __forceinline__ float row_loss(const DistillArgs& a, int64_t n, const RowInfo& i,
+                                          F raw) {
+  const float c = kLog2e / a.temperature;
   float loss = 0.f;
   for (int k = threadIdx.x & 63; k < a.K; k += 64) {
     const int64_t j = index_at(a, n * a.K + k);
     if (j < 0 || j >= a.V) continue;
-    const float lp = a.teacher[n * a.K + k] * c - t.norm;
-    const float p = ex2(lp);
-    if (p > 0.f) loss += p * (lp - (up<E>(z[j]) * c - lse));
+    const float tl = a.teacher[n * a.K + k];
+    const float p = i.teacher.part(tl, c);
+    if (p > 0.f) loss += p * (i.teacher.log2part(tl, c) - i.all.log2part(raw(k, j), c));
   }
   loss = wave_reduce_sum(loss);
-  if (t.r > 0.f) loss += t.r * ((t.rest - t.norm) - (tail - lse));
+  if (i.r > 0.f)
+    loss += i.r * (i.teacher.log2part(a.rest[n], kLog2e) -
+                   ((i.tail.m - i.all.m) + (log2f(i.tail.s) - log2f(i.all.s))));
   // p = 0 terms drop out, but not what makes the row undefined
-  if (lse != lse || t.norm != t.norm) loss = lse + t.norm;
-  return t.counts ? loss * kLn2 * a.temperature * a.temperature : 0.f;
+  if (i.all.s != i.all.s || i.all.s == 0.f || i.teacher.s != i.teacher.s) loss = __builtin_nanf("");
+  return i.r < 0.f ? 0.f : loss * kLn2 * a.temperature * a.temperature;
 }
 
-// info: {lse, tail, r (-1: the row does not count), teacher norm}
 template <typename E>
-__device__ void finish_row(const DistillArgs& a, int64_t n, float lse, float tail) {
-  const Teacher t(a, n);
-  if (t.outside) lse = tail = __builtin_nanf("");
-  const float loss = row_loss<E>(a, n, t, lse, tail);
+__device__ void finish_row(const DistillArgs& a, int64_t n, const Run& all, const Run& tail) {
+  RowInfo info{all, tail, {0.f, 0.f}, 0.f, 0.f};
+  teacher_of(a, n, info);
+  const E* z = row_of<E>(a, n);
+  const float loss = row_loss(a, n, info, [&](int, int64_t j) { return up<E>(z[j]); });
   if ((threadIdx.x & 63) == 0) {
-    a.info[n] = make_float4(lse, tail, t.counts ? t.r : -1.f, t.norm);
+    store_info(a, n, info);
     a.row_loss[n] = loss;
   }
 }
+
+// The gradient of the columns outside I is f 2^(x c - base).
+struct Outside {
+  float base, f;
+  __device__ __forceinline__ Outside(const RowInfo& i, float g, bool rest) {
+    if (rest && i.tail.s > 0.f) {
+      const float share = i.tail.s * ex2(i.tail.m - i.all.m) / i.all.s;  // R
+      base = i.tail.m;
+      f = g * (share - i.r) / i.tail.s;
+    } else {
+      base = i.all.m;
+      f = g / i.all.s;
+    }
+    if (i.teacher.s != i.teacher.s) f = i.teacher.s;
+  }
+};
 
 // Statistics of a slice of a row: part = {tail m, s, member m, s}.
 template <typename E, bool ALIGNED, bool REST>
@@ -205,6 +247,7 @@ __global__ void __launch_bounds__(NT) stats_kernel(DistillArgs a) {
   some = __syncthreads_or(some);
 
   Run out{KFAC_NEG_INF, 0.f}, in{KFAC_NEG_INF, 0.f};
+  float raw = KFAC_NEG_INF;  // largest logit so far
   if (some) {
     const int64_t nv = (c1 - c0) / N;
     for (int64_t v0 = tid; v0 < nv; v0 += (int64_t)NT * U) {
@@ -219,7 +262,7 @@ __global__ void __launch_bounds__(NT) stats_kernel(DistillArgs a) {
           for (int i = 0; i < N; ++i) y[q][i] = KFAC_NEG_INF;
         }
       }
-      float mx = out.m;
+      float mx = raw;
 #pragma unroll
       for (int q = 0; q < U; ++q) {
         if (REST) {
@@ -230,33 +273,29 @@ __global__ void __launch_bounds__(NT) stats_kernel(DistillArgs a) {
 #pragma unroll
             for (int i = 0; i < N; ++i)
               if ((b >> i) & 1u) {
-                const float e = y[q][i] * c;
-                in.join(e, e == KFAC_NEG_INF ? 0.f : 1.f);
+                in.add(y[q][i], c);
                 y[q][i] = KFAC_NEG_INF;
               }
           }
         }
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          y[q][i] *= c;
-          mx = fmaxf(mx, y[q][i]);
-        }
+        for (int i = 0; i < N; ++i) mx = fmaxf(mx, y[q][i]);
       }
-      const float base = mx == KFAC_NEG_INF ? 0.f : mx;
+      raw = mx;
+      const float m = mx * c, base = m == KFAC_NEG_INF ? 0.f : m;
       float s = out.s * ex2(out.m - base);
 #pragma unroll
       for (int q = 0; q < U; ++q)
 #pragma unroll
-        for (int i = 0; i < N; ++i) s += ex2(y[q][i] - base);
+        for (int i = 0; i < N; ++i) s += ex2(__builtin_fmaf(y[q][i], c, -base));
       out.s = s;
-      out.m = mx;
+      out.m = m;
     }
     const int64_t rem = c0 + nv * N + tid;  // the last, partial access
     if (rem < c1) {
-      const float e = up<E>(z[rem]) * c;
       const int at = (int)(rem - c0);
       const bool member = REST && ((bits[at >> 5] >> (at & 31)) & 1u);
-      (member ? in : out).join(e, e == KFAC_NEG_INF ? 0.f : 1.f);
+      (member ? in : out).add(up<E>(z[rem]), c);
     }
   }
   out = wave_join(out);
@@ -275,8 +314,7 @@ __global__ void __launch_bounds__(NT) stats_kernel(DistillArgs a) {
     if (tid == 0) a.part[blockIdx.x] = make_float4(out.m, out.s, in.m, in.s);
     return;
   }
-  const float tail = out.log2sum();
-  finish_row<E>(a, n, REST ? add_log2(tail, in.log2sum()) : tail, tail);
+  finish_row<E>(a, n, REST ? joined(out, in) : out, out);
 }
 
 // rows of several slices: one wave joins them, in order
@@ -291,8 +329,7 @@ __global__ void __launch_bounds__(64) join_kernel(DistillArgs a) {
   }
   out = wave_join(out);
   if (REST) in = wave_join(in);
-  const float tail = out.log2sum();
-  finish_row<E>(a, n, REST ? add_log2(tail, in.log2sum()) : tail, tail);
+  finish_row<E>(a, n, REST ? joined(out, in) : out, out);
 }
 
 // sum or mean of the rows' losses (loss null: not yet known), and the factor
@@ -306,7 +343,7 @@ __global__ void __launch_bounds__(1024) reduce_kernel(const float* row_loss, con
   double s = 0.0, c = 0.0;
   for (int64_t n = threadIdx.x; n < N; n += 1024) {
     s += loss != nullptr ? row_loss[n] : 0.f;
-    c += info[n].z < 0.f ? 0.0 : 1.0;
+    c += info[2 * n + 1].z < 0.f ? 0.0 : 1.0;
   }
   s = wave_reduce_sum(s);
   c = wave_reduce_sum(c);
@@ -331,10 +368,9 @@ __global__ void __launch_bounds__(1024) reduce_kernel(const float* row_loss, con
 __global__ void __launch_bounds__(NT) teacher_kernel(DistillArgs a) {
   const int64_t n = (int64_t)blockIdx.x * (NT / 64) + (threadIdx.x >> 6);
   if (n >= a.N) return;
-  const Teacher t(a, n);
-  if ((threadIdx.x & 63) == 0)
-    a.info[n] = make_float4(t.outside ? __builtin_nanf("") : 0.f, 0.f, t.counts ? t.r : -1.f,
-                            t.norm);
+  RowInfo info{{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, 0.f, 0.f};
+  teacher_of(a, n, info);
+  if ((threadIdx.x & 63) == 0) store_info(a, n, info);
 }
 
 // Keeps 16 bytes packed: without it the compiler carries their fp32 values,
@@ -359,22 +395,21 @@ __global__ void __launch_bounds__(kRowThreads, VPT <= 9 ? 8 : 4) row_kernel(Dist
   __shared__ float4 red[kRowThreads / 64];
   __shared__ int at[kMaxK];     // the entries' columns, -1: none
   __shared__ float pk[kMaxK];   // their share of the teacher
-  __shared__ float yk[kMaxK];   // the student's logits there, in units of log2
+  __shared__ float xk[kMaxK];   // the student's logits there
   __shared__ float pj[kMaxK];   // the teacher's share of the column, all entries that name it
-  __shared__ float sums[2];     // sum p (ln p - y) and sum p, over the entries
   const int64_t n = blockIdx.x;
   const int tid = threadIdx.x, V = (int)a.V, nv = V / N;
   const E* z = row_of<E>(a, n);
   E* d = reinterpret_cast<E*>(a.dz) + n * a.V;
   const float c = kLog2e / a.temperature;
-  const float4 info = a.info[n];
+  RowInfo info = load_info(a, n);
   typedef E vec __attribute__((ext_vector_type(N)));
   typedef vec uvec __attribute__((aligned(sizeof(E))));
   auto put = [&](E* p, const vec& x) {
     if (ALIGNED) *reinterpret_cast<vec*>(p) = x;
     else *reinterpret_cast<uvec*>(p) = x;
   };
-  if (info.z < 0.f) {  // the row does not count (a NaN does)
+  if (info.r < 0.f) {  // the row does not count (a NaN does)
     vec zero;
 #pragma unroll
     for (int i = 0; i < N; ++i) zero[i] = (E)0.f;
@@ -404,8 +439,8 @@ __global__ void __launch_bounds__(kRowThreads, VPT <= 9 ? 8 : 4) row_kernel(Dist
     const int64_t j = index_at(a, n * a.K + k);
     const bool in = j >= 0 && j < V;
     at[k] = in ? (int)j : -1;
-    pk[k] = in ? ex2(a.teacher[n * a.K + k] * c - info.w) : 0.f;
-    yk[k] = in ? up<E>(z[j]) * c : 0.f;
+    pk[k] = in ? info.teacher.part(a.teacher[n * a.K + k], c) : 0.f;
+    xk[k] = in ? up<E>(z[j]) : 0.f;
     if (REST && in) atomicOr(&bits[j >> 5], 1u << (j & 31));
   }
   __syncthreads();
@@ -421,22 +456,8 @@ __global__ void __launch_bounds__(kRowThreads, VPT <= 9 ? 8 : 4) row_kernel(Dist
     for (int off = team >> 1; off > 0; off >>= 1) p += __shfl_xor(p, off, 64);
     if (k < a.K && part == 0) pj[k] = p;
   }
-  if (tid < 64) {
-    float sa = 0.f, sp = 0.f;
-    for (int k = tid; k < a.K; k += 64)
-      if (pk[k] > 0.f) {
-        sa += pk[k] * ((a.teacher[n * a.K + k] * c - info.w) - yk[k]);
-        sp += pk[k];
-      }
-    sa = wave_reduce_sum(sa);
-    sp = wave_reduce_sum(sp);
-    if (tid == 0) {
-      sums[0] = sa;
-      sums[1] = sp;
-    }
-  }
-
   Run out{KFAC_NEG_INF, 0.f}, in{KFAC_NEG_INF, 0.f};
+  float raw = KFAC_NEG_INF;  // largest logit so far
 #pragma unroll
   for (int q = 0; q < VPT; ++q) {
     if (REST) {
@@ -446,30 +467,29 @@ __global__ void __launch_bounds__(kRowThreads, VPT <= 9 ? 8 : 4) row_kernel(Dist
 #pragma unroll
         for (int i = 0; i < N; ++i)
           if ((b >> i) & 1u) {
-            const float e = up<E>(x[q][i]) * c;
-            in.join(e, e == KFAC_NEG_INF ? 0.f : 1.f);
+            in.add(up<E>(x[q][i]), c);
             x[q][i] = (E)KFAC_NEG_INF;
           }
       }
       stay_packed(x[q]);
     }
-    float y[N];
+    float y[N], mx = raw;
 #pragma unroll
-    for (int i = 0; i < N; ++i) y[i] = up<E>(x[q][i]) * c;
-    float mx = out.m;
-#pragma unroll
-    for (int i = 0; i < N; ++i) mx = fmaxf(mx, y[i]);
-    const float base = mx == KFAC_NEG_INF ? 0.f : mx;
+    for (int i = 0; i < N; ++i) {
+      y[i] = up<E>(x[q][i]);
+      mx = fmaxf(mx, y[i]);
+    }
+    raw = mx;
+    const float m = mx * c, base = m == KFAC_NEG_INF ? 0.f : m;
     float s = out.s * ex2(out.m - base);
 #pragma unroll
-    for (int i = 0; i < N; ++i) s += ex2(y[i] - base);
+    for (int i = 0; i < N; ++i) s += ex2(__builtin_fmaf(y[i], c, -base));
     out.s = s;
-    out.m = mx;
+    out.m = m;
   }
   if (rem < V) {
-    const float e = last * c;
     const bool member = REST && ((bits[rem >> 5] >> (rem & 31)) & 1u);
-    (member ? in : out).join(e, e == KFAC_NEG_INF ? 0.f : 1.f);
+    (member ? in : out).add(last, c);
   }
   out = wave_join(out);
   if (REST) in = wave_join(in);
@@ -482,15 +502,10 @@ __global__ void __launch_bounds__(kRowThreads, VPT <= 9 ? 8 : 4) row_kernel(Dist
     out.join(red[w].x, red[w].y);
     if (REST) in.join(red[w].z, red[w].w);
   }
-  float tail = out.log2sum();
-  float lse = REST ? add_log2(tail, in.log2sum()) : tail;
-  if (info.x != info.x) lse = tail = info.x;  // an index behind the vocabulary
-  const float r = info.z, g = a.temperature * a.mean[0];
-  float base = lse, f = g;
-  if (REST && tail != KFAC_NEG_INF) {
-    base = tail;
-    f = g * (ex2(tail - lse) - r);
-  }
+  info.tail = out;
+  info.all = REST ? joined(out, in) : out;
+  const float g = a.temperature * a.mean[0];
+  const Outside o(info, g, REST);
 #pragma unroll
   for (int q = 0; q < VPT; ++q) {
     const int v = tid + q * kRowThreads;
@@ -498,21 +513,22 @@ __global__ void __launch_bounds__(kRowThreads, VPT <= 9 ? 8 : 4) row_kernel(Dist
     if (v < nv) {
       vec y;
 #pragma unroll
-      for (int i = 0; i < N; ++i) y[i] = (E)(f * ex2(up<E>(x[q][i]) * c - base));
+      for (int i = 0; i < N; ++i) y[i] = (E)(o.f * ex2(__builtin_fmaf(up<E>(x[q][i]), c, -o.base)));
       put(d + (int64_t)v * N, y);
     }
   }
-  if (rem < V) d[rem] = (E)(f * ex2(last * c - base));
-  if (tid == 0) {
-    float loss = sums[0] + sums[1] * lse;
-    if (r > 0.f) loss += r * ((a.rest[n] * kLog2e - info.w) - (tail - lse));
-    if (lse != lse || info.w != info.w) loss = lse + info.w;
-    a.row_loss[n] = loss * kLn2 * a.temperature * a.temperature;
-    a.info[n] = make_float4(lse, tail, r, info.w);
+  if (rem < V) d[rem] = (E)(o.f * ex2(__builtin_fmaf(last, c, -o.base)));
+  if (tid < 64) {
+    const float loss = row_loss(a, n, info, [&](int k, int64_t) { return xk[k]; });
+    if (tid == 0) {
+      a.row_loss[n] = loss;
+      store_info(a, n, info);
+    }
   }
   __syncthreads();
+  const float nan = info.teacher.s != info.teacher.s ? info.teacher.s : 0.f;
   for (int k = tid; k < a.K; k += kRowThreads)
-    if (at[k] >= 0) d[at[k]] = (E)(g * (ex2(yk[k] - lse) - pj[k]));
+    if (at[k] >= 0) d[at[k]] = (E)(g * (info.all.part(xk[k], c) - pj[k]) + nan);
 }
 
 // dz *= *factor, in place; nothing to do where that is 1
@@ -533,9 +549,8 @@ __global__ void __launch_bounds__(NT) scale_kernel(E* dz, int64_t n, const float
   if (blockIdx.x == 0 && rem < n) dz[rem] = (E)(up<E>(dz[rem]) * f);
 }
 
-// dz of a slice of a row.  Every column is first written as one outside I
-// (e = 2^(y - tail), factor R - r; without a rest 2^(y - lse)), the block's
-// members are written over it behind a barrier.
+// dz of a slice of a row.  Every column is first written as one outside I,
+// the block's members are written over it behind a barrier.
 template <typename E, bool ALIGNED_Z, bool ALIGNED_D, bool REST>
 __global__ void __launch_bounds__(NT) grad_kernel(DistillArgs a) {
   constexpr int N = Wide<E>::N;
@@ -549,21 +564,16 @@ __global__ void __launch_bounds__(NT) grad_kernel(DistillArgs a) {
   const E* z = row_of<E>(a, n);
   E* d = reinterpret_cast<E*>(a.dz) + n * a.V;
   const float c = kLog2e / a.temperature;
-  const float4 info = a.info[n];
-  const float lse = info.x, tail = info.y, r = info.z, norm = info.w;
-  const bool counts = !(r < 0.f);
+  const RowInfo info = load_info(a, n);
+  const bool counts = !(info.r < 0.f);
   float g = a.upstream[a.upstream_rows ? n : 0] * a.temperature;
-  if (a.mean != nullptr) g *= a.mean[0];
-  float base = lse, f = g;
-  if (REST && tail != KFAC_NEG_INF) {
-    base = tail;
-    f = g * (ex2(tail - lse) - r);
-  }
+  g *= a.mean != nullptr ? a.mean[0] : a.weight;
+  const Outside o(info, g, REST);
   if (counts) {
     for (int k = tid; k < a.K; k += NT) {
       const int64_t j = index_at(a, n * a.K + k);
       at[k] = j >= c0 && j < c1 ? (int)(j - c0) : -1;
-      pk[k] = ex2(a.teacher[n * a.K + k] * c - norm);
+      pk[k] = info.teacher.part(a.teacher[n * a.K + k], c);
     }
   }
   const int64_t nv = (c1 - c0) / N;
@@ -579,13 +589,14 @@ __global__ void __launch_bounds__(NT) grad_kernel(DistillArgs a) {
       const int64_t v = v0 + (int64_t)q * NT;
       if (v < nv) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) y[q][i] = counts ? f * ex2(y[q][i] * c - base) : 0.f;
+        for (int i = 0; i < N; ++i) y[q][i] = counts ? o.f * ex2(__builtin_fmaf(y[q][i], c, -o.base)) : 0.f;
         store_wide<E, ALIGNED_D>(d + c0 + v * N, y[q]);
       }
     }
   }
   const int64_t rem = c0 + nv * N + tid;
-  if (rem < c1) d[rem] = (E)(counts ? f * ex2(up<E>(z[rem]) * c - base) : 0.f);
+  if (rem < c1)
+    d[rem] = (E)(counts ? o.f * ex2(__builtin_fmaf(up<E>(z[rem]), c, -o.base)) : 0.f);
   if (!counts) return;
   __syncthreads();
   for (int k = tid; k < a.K; k += NT) {
@@ -593,7 +604,7 @@ __global__ void __launch_bounds__(NT) grad_kernel(DistillArgs a) {
     if (j < 0) continue;
     float p = 0.f;  // an index given twice counts with both its parts
     for (int i = 0; i < a.K; ++i) p += at[i] == j ? pk[i] : 0.f;
-    d[c0 + j] = (E)(g * (ex2(up<E>(z[c0 + j]) * c - lse) - p));
+    d[c0 + j] = (E)(g * (info.all.part(up<E>(z[c0 + j]), c) - p));
   }
 }
 

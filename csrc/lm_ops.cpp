@@ -406,7 +406,7 @@ DistillOut distill_run(const at::Tensor& z, const at::Tensor& teacher, const at:
   kfac::DistillArgs a = distill_args(z, teacher, index, rest, temperature, weight);
   const auto f32 = z.options().dtype(at::kFloat);
   DistillOut o;
-  o.info = at::empty({a.N, 4}, f32);
+  o.info = at::empty({a.N, 8}, f32);
   at::Tensor rows = at::empty({a.N}, f32);
   a.info = reinterpret_cast<float4*>(o.info.data_ptr<float>());
   a.row_loss = rows.data_ptr<float>();
@@ -431,6 +431,7 @@ DistillOut distill_run(const at::Tensor& z, const at::Tensor& teacher, const at:
       a.part = reinterpret_cast<float4*>(part.data_ptr<float>());
     }
     kfac::distill_forward(tag(z), a, loss, mean, (int)reduction, stream());
+    if (reduction == 0 && weight != 1.0) rows.mul_(weight);
   }
   C10_HIP_KERNEL_LAUNCH_CHECK();
   return o;

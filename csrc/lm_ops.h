@@ -43,7 +43,7 @@ struct DistillArgs {
   int K, index64, aligned;
   float temperature, weight;
   float4* part;          // [N, splits]: running statistics of a slice of a row
-  float4* info;          // [N]: see distill.hip
+  float4* info;          // [N, 2]: RowInfo of distill.hip
   float* row_loss;       // [N]
   int splits;
   int64_t slice;         // columns of a split (a multiple of 8)

@@ -329,6 +329,19 @@ def test_distill_padding_repeats_views_and_int32(cuda, rest):
     assert float(none.detach()) == 0.0 and bool((torch.autograd.grad(none, z)[0] == 0).all())
 
 
+@pytest.mark.parametrize('reduction', ['none', 'sum', 'mean'])
+@pytest.mark.parametrize('dtype, n', [('fp16', 300), ('bf16', 20), ('fp32', 20)])
+def test_distill_weight(cuda, dtype, n, reduction):
+    z = rand(cuda, n, 700, seed=1, dtype=DTYPES[dtype]).requires_grad_()
+    t, i, r = _teacher(cuda, n, 700, 9, 1.0, True, 6)
+    loss = topk_distill_loss(z, t, i, teacher_rest=r, weight=-0.5, reduction=reduction)
+    up = torch.full_like(loss, 2.0)
+    # -0.5 and 2 are powers of two: no rounding of their own
+    want = ref.distill(z, t, i, rest=r, reduction=reduction, upstream=torch.ones(n) * -1.0)
+    ref.check('loss', loss, -0.5 * want[0], 0.5 * want[1])
+    ref.check('dz', *torch.autograd.grad(loss, z, up), *want[2:])
+
+
 def test_distill_bad_rows_stay_alone(cuda):
     n, v, k = 6, 300, 4
     z = rand(cuda, n, v, seed=3)
