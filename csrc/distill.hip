@@ -39,7 +39,8 @@ namespace {
 
 constexpr int NT = 256;
 constexpr int kMaxK = 1024;
-constexpr int kMaxVpt = 16;  // 16-byte accesses a thread of row_kernel holds
+constexpr int kMaxVpt = 16;  // 16-byte accesses that each of
+constexpr int kMaxRowThreads = 1024;  // threads of row_kernel holds, at most
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 #define KFAC_NEG_INF (-__builtin_inff())
@@ -384,12 +385,11 @@ __device__ __forceinline__ void stay_packed(V& x) {
 
 // A row in one block: its logits stay in registers between the statistics
 // and the gradient.
-constexpr int kRowThreads = 1024;
-
-// Two blocks a CU (64 registers a thread) up to 9 accesses a thread, so that
-// one loads while the other forms its sums; one block above.
-template <typename E, int VPT, bool ALIGNED, bool REST>
-__global__ void __launch_bounds__(kRowThreads, VPT <= 9 ? 8 : 4) row_kernel(DistillArgs a) {
+// Waves a SIMD are chosen so that two blocks or more share a CU where their
+// logits leave the registers for it: one loads while another forms its sums.
+template <typename E, int VPT, int kRowThreads, bool ALIGNED, bool REST>
+__global__ void __launch_bounds__(kRowThreads, VPT <= 7 ? 8 : 4)
+row_kernel(DistillArgs a) {
   constexpr int N = Wide<E>::N;
   extern __shared__ uint32_t bits[];  // with a rest: one bit a column
   __shared__ float4 red[kRowThreads / 64];
@@ -639,29 +639,33 @@ void backward_type(const DistillArgs& a, hipStream_t st) {
   else backward_aligned<E, false, false>(a, st);
 }
 
-template <typename E, int VPT>
+template <typename E, int VPT, int THREADS>
 void row_vpt(const DistillArgs& a, hipStream_t st) {
   const unsigned grid = (unsigned)a.N;
   const bool al = a.aligned && a.dz_aligned;
   const size_t lds = a.rest != nullptr ? (size_t)((a.V + 31) / 32) * 4 : 0;
   if (a.rest != nullptr) {
-    if (al) row_kernel<E, VPT, true, true><<<grid, kRowThreads, lds, st>>>(a);
-    else row_kernel<E, VPT, false, true><<<grid, kRowThreads, lds, st>>>(a);
+    if (al) row_kernel<E, VPT, THREADS, true, true><<<grid, THREADS, lds, st>>>(a);
+    else row_kernel<E, VPT, THREADS, false, true><<<grid, THREADS, lds, st>>>(a);
   } else {
-    if (al) row_kernel<E, VPT, true, false><<<grid, kRowThreads, lds, st>>>(a);
-    else row_kernel<E, VPT, false, false><<<grid, kRowThreads, lds, st>>>(a);
+    if (al) row_kernel<E, VPT, THREADS, true, false><<<grid, THREADS, lds, st>>>(a);
+    else row_kernel<E, VPT, THREADS, false, false><<<grid, THREADS, lds, st>>>(a);
   }
 }
 
 template <typename E>
 void row_type(const DistillArgs& a, hipStream_t st) {
-  const int64_t vpt = ceil_div(a.V / Wide<E>::N, kRowThreads);
-  if (vpt <= 1) row_vpt<E, 1>(a, st);
-  else if (vpt <= 2) row_vpt<E, 2>(a, st);
-  else if (vpt <= 4) row_vpt<E, 4>(a, st);
-  else if (vpt <= 7) row_vpt<E, 7>(a, st);
-  else if (vpt <= 9) row_vpt<E, 9>(a, st);
-  else row_vpt<E, kMaxVpt>(a, st);
+  // 1024 threads up to 7 accesses each (50304 bf16 logits, 16384 rows: 0.67
+  // ms, 0.80 as 512 x 13, whose registers do not suffice); where 1024 x 9
+  // would not fit a CU twice, 512 x 18 does (33278 fp32, 1280 rows: 83 us for
+  // the pass against 99)
+  const int64_t vpt = ceil_div(a.V / Wide<E>::N, kMaxRowThreads);
+  if (vpt <= 1) row_vpt<E, 1, kMaxRowThreads>(a, st);
+  else if (vpt <= 2) row_vpt<E, 2, kMaxRowThreads>(a, st);
+  else if (vpt <= 4) row_vpt<E, 4, kMaxRowThreads>(a, st);
+  else if (vpt <= 7) row_vpt<E, 7, kMaxRowThreads>(a, st);
+  else if (vpt <= 9) row_vpt<E, 18, kMaxRowThreads / 2>(a, st);
+  else row_vpt<E, kMaxVpt, kMaxRowThreads>(a, st);
 }
 
 }  // namespace
@@ -693,7 +697,7 @@ void distill_forward(int dtype, const DistillArgs& a, float* loss, float* factor
 bool distill_fuses(int dtype, int64_t N, int64_t V) {
   // 256 rows: a block on every CU
   const int64_t n = dtype == kBF16 ? 8 : 4;
-  return dtype != kF16 && N >= 256 && V <= kRowThreads * kMaxVpt * n;
+  return dtype != kF16 && N >= 256 && V <= kMaxRowThreads * kMaxVpt * n;
 }
 
 void distill_forward_grad(int dtype, const DistillArgs& a, float* loss, int reduction,
