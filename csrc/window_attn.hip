@@ -709,9 +709,9 @@ __device__ __forceinline__ int clip(int64_t t, const AttnArgs& a) {
 
 // Rows that look at the keys [k0, k0 + BM): the near ones, whose window
 // reaches there, and, where the block holds sinks, the far ones behind them.
-template <int NW>
+template <int KG>
 struct RowRange {
-  static constexpr int BM = 32 * NW;
+  static constexpr int BM = 32 * KG;
   int n0, n1, f1;  // near [n0, n1), far [n1, f1)
   __device__ __forceinline__ RowRange(int k0, const AttnArgs& a, const Seq& s) {
     const int64_t last = (int64_t)s.len - 1;        // last position
@@ -898,9 +898,14 @@ struct KeyGrad {
 // which all waves own together, 32 rows each of a tile of 128; their sums
 // are added in wave order.  Sinks are few and the rows behind the window
 // many, so a far item has its rows spread over the waves and not its keys.
-template <typename T, int DP, int NW>
-__global__ void __launch_bounds__(64 * NW, (kKeyFit<T, DP>)) dkv_kernel(AttnArgs a, int key_blocks) {
-  constexpr int ND = DP / 32, LD = kLd<T, DP>, NT = 64 * NW, BM = 32 * NW;
+//
+// KG groups of 32 keys and, for each, RS waves that take every RS-th 32 rows
+// of a tile and add up at the end: where there are fewer waves than the chip
+// can hold, a key's rows are the time that is left to divide.
+template <typename T, int DP, int KG, int RS>
+__global__ void __launch_bounds__(64 * KG * RS, (kKeyFit<T, DP>))
+dkv_kernel(AttnArgs a, int key_blocks) {
+  constexpr int ND = DP / 32, LD = kLd<T, DP>, NW = KG * RS, NT = 64 * NW, BM = 32 * KG;
   __shared__ __attribute__((aligned(16))) T Q0[BN * LD];
   __shared__ __attribute__((aligned(16))) T Q1[BN * LD];
   __shared__ __attribute__((aligned(16))) T G0[BN * LD];
@@ -920,7 +925,7 @@ __global__ void __launch_bounds__(64 * NW, (kKeyFit<T, DP>)) dkv_kernel(AttnArgs
     const int item = (int)blockIdx.y - key_blocks;
     const int group = item / a.far_chunks, chunk = item - group * a.far_chunks;
     const int j0 = group * kSinkKeys, key = j0 + (l & 31);
-    const RowRange<NW> rr(j0 / BM * BM, a, seq);
+    const RowRange<KG> rr(j0 / BM * BM, a, seq);
     const int tokens = (rr.f1 - rr.n1) / a.G;
     const int per = (tokens + a.far_chunks - 1) / a.far_chunks * a.G;
     const int ra = rr.n1 + per * chunk < rr.f1 ? rr.n1 + per * chunk : rr.f1;
@@ -969,14 +974,17 @@ __global__ void __launch_bounds__(64 * NW, (kKeyFit<T, DP>)) dkv_kernel(AttnArgs
     return;
   }
 
-  const int k0 = (int)blockIdx.y * BM;
-  const RowRange<NW> rr(k0, a, seq);
-  const int key = k0 + wave * 32 + (l & 31);
-  const KeyRows kr(k0 + wave * 32, key, a, seq);
+  const int k0 = (int)blockIdx.y * BM, group = wave % KG, turn = wave / KG;
+  const RowRange<KG> rr(k0, a, seq);
+  const int key = k0 + group * 32 + (l & 31);
+  const KeyRows kr(k0 + group * 32, key, a, seq);
   kg.init(a, b, hk, key, key < seq.len);
   auto step = [&](const RowBuf<T>& buf, int t0) {
 #pragma unroll
-    for (int sub = 0; sub < BN / 32; ++sub) kg.rows(a, buf, sub * 32, t0 + sub * 32, kr);
+    for (int sub = 0; sub < BN / 32; sub += RS) {
+      const int i0 = (sub + (RS > 1 ? turn : 0)) * 32;
+      kg.rows(a, buf, i0, t0 + i0, kr);
+    }
   };
   if (rr.n0 < rr.n1) rs.fetch(a, rr.n0, rr.n1, b0);
   for (int t0 = rr.n0; t0 < rr.n1; t0 += 2 * BN) {
@@ -987,6 +995,29 @@ __global__ void __launch_bounds__(64 * NW, (kKeyFit<T, DP>)) dkv_kernel(AttnArgs
     arrived();
     if (t0 + 2 * BN < rr.n1) rs.fetch(a, t0 + 2 * BN, rr.n1, b0);
     step(b1, t0 + BN);
+  }
+  if (RS > 1) {
+    float* sk = reinterpret_cast<float*>(group == 0 ? Q0 : Q1) + l * 4;
+    float* sv = reinterpret_cast<float*>(group == 0 ? G0 : G1) + l * 4;
+    __syncthreads();
+    if (turn == 1)
+#pragma unroll
+      for (int i = 0; i < 4 * ND; ++i) {
+        *reinterpret_cast<v4f*>(sk + i * 256) = quad_of(kg.dk[i / 4], i % 4);
+        *reinterpret_cast<v4f*>(sv + i * 256) = quad_of(kg.dv[i / 4], i % 4);
+      }
+    __syncthreads();
+    if (turn == 1) return;
+#pragma unroll
+    for (int i = 0; i < 4 * ND; ++i) {
+      const v4f fk = *reinterpret_cast<const v4f*>(sk + i * 256);
+      const v4f fv = *reinterpret_cast<const v4f*>(sv + i * 256);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        kg.dk[i / 4][i % 4 * 4 + e] += fk[e];
+        kg.dv[i / 4][i % 4 * 4 + e] += fv[e];
+      }
+    }
   }
   if (a.far_chunks > 0 && key < a.S) {
     float* part = sink_part(a, bh, key / kSinkKeys, 0) + key % kSinkKeys * a.D;
@@ -1038,13 +1069,18 @@ void forward_dp(const AttnArgs& a, hipStream_t st) {
 
 template <typename T, int DP>
 void backward_dp(const AttnArgs& a, hipStream_t st) {
-  constexpr int QN = kRowWaves, KN = kKeyWaves<DP>;
+  constexpr int QN = kRowWaves, KG = kKeyWaves<DP>;
   const unsigned bh = (unsigned)(a.B * a.Hkv);
   dq_kernel<T, DP, QN><<<dim3(bh, (unsigned)ceil_div((int64_t)a.Tq * a.G, 32 * QN)), 64 * QN, 0,
                          st>>>(a);
-  const int kb = (int)ceil_div(a.Tk, 32 * KN);
-  dkv_kernel<T, DP, KN><<<dim3(bh, (unsigned)(kb + a.sink_groups * a.far_chunks)), 64 * KN, 0,
-                          st>>>(a, kb);
+  const int kb = (int)ceil_div(a.Tk, 32 * KG);
+  const dim3 grid(bh, (unsigned)(kb + a.sink_groups * a.far_chunks));
+  // up to one wave a SIMD: two share a group of keys (fp32 padded batch, 500
+  // waves: 60 -> 52 us)
+  if (KG == 2 && (int64_t)bh * kb * KG <= 1024)
+    dkv_kernel<T, DP, KG, KG == 2 ? 2 : 1><<<grid, 64 * KG * 2, 0, st>>>(a, kb);
+  else
+    dkv_kernel<T, DP, KG, 1><<<grid, 64 * KG, 0, st>>>(a, kb);
   if (a.far_chunks > 0) {
     const int64_t n = (int64_t)bh * a.S * 2 * (a.D / 4);
     join_kv_kernel<T><<<(unsigned)ceil_div(n, NT), NT, 0, st>>>(a);
