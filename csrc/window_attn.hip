@@ -193,7 +193,7 @@ __device__ __forceinline__ typename Ops<T>::frag col_frag(const T* L, int r0, in
 
 // registers 8s .. 8s + 7 of an accumulator as a right operand, rounded once
 // to the operands' type (16-bit probabilities and their gradients are the
-// price of the matrix units; they are at most 2^-9 off relative each, and
+// price of the matrix units; each is off by 2^-8 of itself at most, and
 // the sums over them stay in 32 bits)
 template <typename T>
 __device__ __forceinline__ typename Ops<T>::frag acc_frag(const v16f& a, int s) {
@@ -893,10 +893,10 @@ struct KeyGrad {
   }
 };
 
-// blockIdx.y < key_blocks: the near rows of 128 keys, 32 a wave, the rows
+// blockIdx.y < key_blocks: the near rows of 32 KG keys, 32 a wave, the rows
 // streamed in tiles of 64.  Above: a chunk of the far rows of 32 sink keys,
-// which all waves own together, 32 rows each of a tile of 128; their sums
-// are added in wave order.  Sinks are few and the rows behind the window
+// which all waves own together, 32 rows each of a tile of one or two times
+// 64; their sums are added in wave order.  Sinks are few and the rows behind the window
 // many, so a far item has its rows spread over the waves and not its keys.
 //
 // KG groups of 32 keys and, for each, RS waves that take every RS-th 32 rows
@@ -932,7 +932,7 @@ dkv_kernel(AttnArgs a, int key_blocks) {
     const int rb = ra + per < rr.f1 ? ra + per : rr.f1;
     const KeyRows kr(j0, key, a, seq);
     kg.init(a, b, hk, key, key < seq.len);
-    for (int t0 = ra; t0 < rb; t0 += BM) {
+    for (int t0 = ra; t0 < rb; t0 += 32 * NW) {
       __syncthreads();
       rs.fetch(a, t0, rb, b0);
       if (NW > 2) rs.fetch(a, t0 + BN, rb, b1);
