@@ -695,9 +695,9 @@ void distill_forward(int dtype, const DistillArgs& a, float* loss, float* factor
 }
 
 bool distill_fuses(int dtype, int64_t N, int64_t V) {
-  // 256 rows: a block on every CU
+  // 256 rows: a block on every CU; a launch has at most 2^32 threads
   const int64_t n = dtype == kBF16 ? 8 : 4;
-  return dtype != kF16 && N >= 256 && V <= kMaxRowThreads * kMaxVpt * n;
+  return dtype != kF16 && N >= 256 && N < (1LL << 22) && V <= kMaxRowThreads * kMaxVpt * n;
 }
 
 void distill_forward_grad(int dtype, const DistillArgs& a, float* loss, int reduction,

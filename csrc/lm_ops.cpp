@@ -113,7 +113,8 @@ kfac::AttnArgs attn_args(const at::Tensor& q, const at::Tensor& k, const at::Ten
   TORCH_CHECK(q.size(3) % 8 == 0 && q.size(3) >= 8 && q.size(3) <= 128,
               "window_attention: head size must be a multiple of 8, at most 128");
   const int64_t lim = (int64_t)1 << 30;
-  TORCH_CHECK(q.size(2) < lim && k.size(2) < lim && q.size(0) * q.size(1) < lim,
+  // a launch has at most 2^32 threads along x
+  TORCH_CHECK(q.size(2) < lim && k.size(2) < lim && q.size(0) * q.size(1) < ((int64_t)1 << 24),
               "window_attention: too large");
   a.B = (int)q.size(0);
   a.Hq = (int)q.size(1);
@@ -313,6 +314,8 @@ std::tuple<at::Tensor, at::Tensor> rotary_run(const at::Tensor& q, const at::Ten
   const int64_t unit = 16 / (int64_t)q.element_size();
   const bool vec = rows16(q) && rows16(k) && D % unit == 0 &&
                    (!c.halves || (pairs % unit == 0 && (D - 2 * pairs) % unit == 0));
+  // a thread a unit of a token's head, at most 2^32 of a launch
+  TORCH_CHECK(B * T * (vec ? D / unit : D) < (1LL << 32) - 256, "rotary_axes: too large");
   kfac::rotary_axes(tag(q), a, c.halves, vec, stream());
   C10_HIP_KERNEL_LAUNCH_CHECK();
   return {qo, ko};
@@ -390,7 +393,8 @@ kfac::DistillArgs distill_args(const at::Tensor& z, const at::Tensor& teacher,
   a.weight = (float)weight;
   a.aligned = rows16(z);
   kfac::distill_split(a.N, a.V, rest.has_value(), &a.slice, &a.splits);
-  TORCH_CHECK(a.N * a.splits < (1LL << 31), "topk_distill_loss: too many rows");
+  // blocks of 256 threads, at most 2^32 of a launch
+  TORCH_CHECK(a.N * a.splits < (1LL << 24), "topk_distill_loss: too many rows");
   return a;
 }
 

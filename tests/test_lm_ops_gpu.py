@@ -456,6 +456,83 @@ def test_chain_in_two_graphs(cuda):
             assert all(torch.equal(a, b) for a, b in zip(kept, eager)), (rep, n)
 
 
+def test_offsets_behind_32_bits(cuda):
+    """Operands of more than 2^31 elements: what lies at their end is what a
+    small call on a copy of it gives, bit for bit."""
+    d, tk = 128, 2 ** 24 + 77
+    k = torch.zeros(1, 1, tk, d, dtype=torch.bfloat16, device=cuda)
+    v = torch.zeros_like(k)
+    q = rand(cuda, 1, 2, 3, d, seed=1, dtype=torch.bfloat16)
+    for x, s in ((k, 2), (v, 3)):
+        x[:, :, -200:] = rand(cuda, 1, 1, 200, d, seed=s, dtype=torch.bfloat16)
+        x[:, :, :5] = rand(cuda, 1, 1, 5, d, seed=s + 5, dtype=torch.bfloat16)
+    got = window_attention(q, k, v, window=150, sinks=5)
+    kk, vv = (torch.cat([x[:, :, :5], x[:, :, -200:]], dim=2) for x in (k, v))
+    want, tol = ref.attention(q, kk, vv, window=150, sinks=5)
+    ref.check('out', got, want[0], tol[0])
+    del k, v
+
+    hk, tk = 9, 2 ** 21 + 5
+    k = torch.zeros(1, hk, tk, d, dtype=torch.bfloat16, device=cuda)
+    v = torch.zeros_like(k)
+    q = rand(cuda, 1, hk, 3, d, seed=11, dtype=torch.bfloat16)
+    do = rand(cuda, 1, hk, 3, d, seed=12, dtype=torch.bfloat16)
+    for x, s in ((k, 13), (v, 14)):
+        x[:, -1:, -200:] = rand(cuda, 1, 1, 200, d, seed=s, dtype=torch.bfloat16)
+        x.requires_grad_()
+    out = window_attention(q, k, v, window=150)
+    got = torch.autograd.grad(out, (k, v), do)
+    ends = [x.detach()[:, -1:, -200:] for x in (k, v)]
+    want, tol = ref.attention(q[:, -1:], *ends, window=150, do=do[:, -1:])
+    for i, name in enumerate(('dk', 'dv')):
+        ref.check(name, got[i][:, -1:, -200:], want[2 + i], tol[2 + i])
+        assert not bool(got[i][:, -1, :-200].any())
+    del k, v, got, out
+
+    b, h, t = 70, 16, 16384                       # 2.35e9 elements
+    x = torch.zeros(b, h, t, d, dtype=torch.bfloat16, device=cuda)
+    x[-1, -1, -9:] = rand(cuda, 9, d, seed=4, dtype=torch.bfloat16)
+    pos = torch.arange(t, device=cuda)[:, None]
+    one = x[-1:, -1:, -9:].clone()
+    _, big = rotary_axes(x[:, :1], x, pos, sections=(64,))
+    _, small = rotary_axes(one, one, pos[-9:], sections=(64,))
+    assert torch.equal(big[-1:, -1:, -9:], small)
+    del x, big
+
+    n, vocab = 43000, 50304                       # 2.16e9 logits
+    z = torch.zeros(n, vocab, dtype=torch.bfloat16, device=cuda)
+    z[-3:] = rand(cuda, 3, vocab, seed=5, dtype=torch.bfloat16)
+    t3, i3, _ = _teacher(cuda, 3, vocab, 6, 1.0, False, 8)
+    idx = torch.full((n, 6), -1, device=cuda)
+    idx[-3:] = i3
+    tl = torch.zeros(n, 6, device=cuda)
+    tl[-3:] = t3
+    z.requires_grad_()
+    loss = topk_distill_loss(z, tl, idx)
+    want = ref.distill(z[-3:], t3, i3)
+    ref.check('loss', loss, *want[:2])
+    (g,) = torch.autograd.grad(loss, z)
+    ref.check('dz', g[-3:], *want[2:])
+    assert not bool(g[:-3].any())
+
+
+def test_too_large_is_refused_on_the_host(cuda):
+    one = torch.zeros(1, 1, 1, 8, device=cuda)
+    many = one.expand(2 ** 25, 1, 1, 8)
+    with pytest.raises(RuntimeError, match='too large'):
+        window_attention(many, many, many, window=1)
+    with pytest.raises(RuntimeError, match='row blocks'):
+        window_attention(one.expand(1, 1, 2 ** 24, 8), one, one, window=1)
+    with pytest.raises(RuntimeError, match='too large'):
+        rotary_axes(one.expand(2, 1, 2 ** 30, 8), one.expand(2, 1, 2 ** 30, 8),
+                    torch.zeros(1, 1, dtype=torch.int32, device=cuda).expand(2 ** 30, 1),
+                    sections=(4,))
+    row = torch.zeros(1, 1, device=cuda)
+    with pytest.raises(RuntimeError, match='too many rows'):
+        topk_distill_loss(row.expand(2 ** 24, 1), row.expand(2 ** 24, 1),
+                          torch.zeros(1, 1, dtype=torch.int32, device=cuda).expand(2 ** 24, 1))
+
+
 def test_gradients_of_gradients_are_refused(cuda):
     q = rand(cuda, 1, 1, 4, 8).requires_grad_()
     z = rand(cuda, 2, 9).requires_grad_()
