@@ -29,6 +29,7 @@
 
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 
 namespace kfac {
 
@@ -96,6 +97,16 @@ template <> struct Ops<float> {
   }
 };
 
+// f(0), f(1) .. f(N - 1), each with its number as a constant
+template <typename F, int... I>
+__device__ __forceinline__ void each_of(F f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>()), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void each(F f) {
+  each_of(f, std::make_integer_sequence<int, N>());
+}
+
 template <typename T> constexpr int kUnit = 16 / (int)sizeof(T);  // elements of 16 bytes
 
 // An LDS tile is BN rows of CR 16-byte chunks (a power of two), chunk c of
@@ -123,7 +134,7 @@ template <typename T, int DP> constexpr int kKeyFit = (sizeof(T) == 2 ? DP <= 64
 // with 8; 8192 tokens with heads of 128: 94, 148, 115).  Keys: 2 up to heads
 // of 64, where the shorter blocks even out the load (67 us, 74 with 4; fp32
 // padded batch 60, 78), 4 above, where the traffic of the rows weighs more
-// (228 us, 243 with 2).
+// (228 us, 243 with 2, before the fixed order of KeyGrad::rows64).
 constexpr int kRowWaves = 4;
 template <int DP> constexpr int kKeyWaves = DP <= 64 ? 2 : 4;
 
@@ -145,18 +156,40 @@ __device__ __forceinline__ v16f zero16() {
   return z;
 }
 
+// Where a lane reads a tile, in bytes from its start.  Rows and chunks lie in
+// different bits and place_of is linear over the bits of a row, so every
+// other operand's place is one exclusive or and a constant away.
+template <typename T, int DP>
+struct Lane {
+  static constexpr int CR = kChunks<T, DP>, ROW = kLd<T, DP> * (int)sizeof(T);
+  uint32_t row, col;
+  __device__ __forceinline__ Lane() {
+    const int l = threadIdx.x & 63, h = l >> 5;
+    if constexpr (sizeof(T) == 2) {
+      const int i = l & 15, g = l >> 4, r = 4 * (g >> 1) + (i >> 2);
+      row = (l & 31) * ROW + (h ^ place_of<CR>(l & 31)) * 16;
+      col = r * ROW + ((2 * (g & 1) + ((i & 3) >> 1)) ^ place_of<CR>(r)) * 16 + 8 * (i & 1);
+    } else {
+      row = (l & 31) * ROW + ((2 * h) ^ place_of<CR>(l & 31)) * 16;
+      col = 4 * h * ROW + (((l & 31) / 4) ^ place_of<CR>(4 * h)) * 16 + (l & 3) * 4;
+    }
+  }
+  // Once a tile: the compiler would keep every operand's address of every
+  // tile in a register of its own (100 and more) instead of these two.
+  __device__ __forceinline__ void fresh() { asm volatile("" : "+v"(row), "+v"(col)); }
+};
+
 // Left operand from rows: lane l holds row r0 + (l & 31), elements
 // 16 k + 8 (l >> 5) .. + 7 (r0 a multiple of 16)
 template <typename T, int DP>
-__device__ __forceinline__ typename Ops<T>::frag row_frag(const T* L, int r0, int k) {
-  const int l = threadIdx.x & 63, f = place_of<kChunks<T, DP>>(l & 31);
-  const T* p = L + (r0 + (l & 31)) * kLd<T, DP>;
+__device__ __forceinline__ typename Ops<T>::frag row_frag(const T* L, const Lane<T, DP>& at, int r0,
+                                                          int k) {
+  const char* p = reinterpret_cast<const char*>(L) + r0 * Lane<T, DP>::ROW;
   if constexpr (sizeof(T) == 2) {
-    return *reinterpret_cast<const typename Ops<T>::frag*>(p + ((2 * k + (l >> 5)) ^ f) * 8);
+    return *reinterpret_cast<const typename Ops<T>::frag*>(p + (at.row ^ (k * 32)));
   } else {
-    const int c = 4 * k + 2 * (l >> 5);
-    const v4f a = *reinterpret_cast<const v4f*>(p + (c ^ f) * 4);
-    const v4f b = *reinterpret_cast<const v4f*>(p + ((c + 1) ^ f) * 4);
+    const v4f a = *reinterpret_cast<const v4f*>(p + (at.row ^ (k * 64)));
+    const v4f b = *reinterpret_cast<const v4f*>(p + (at.row ^ (k * 64 + 16)));
     return v8f{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
   }
 }
@@ -165,27 +198,26 @@ __device__ __forceinline__ typename Ops<T>::frag row_frag(const T* L, int r0, in
 // r0 + 4h + {0..3} and r0 + 8 + 4h + {0..3}: the order in which registers
 // 8s .. 8s + 7 of an accumulator hold its rows (r0 = 16 s)
 template <typename T, int DP>
-__device__ __forceinline__ typename Ops<T>::frag col_frag(const T* L, int r0, int c0) {
-  constexpr int CR = kChunks<T, DP>, LD = kLd<T, DP>;
-  const int l = threadIdx.x & 63;
+__device__ __forceinline__ typename Ops<T>::frag col_frag(const T* L, const Lane<T, DP>& at, int r0,
+                                                          int c0) {
+  constexpr int CR = Lane<T, DP>::CR, ROW = Lane<T, DP>::ROW;
+  const char* p = reinterpret_cast<const char*>(L) + r0 * ROW;
   if constexpr (sizeof(T) == 2) {
     // ds_read_b64_tr_b16: 16 lanes read 4 rows x 16 columns (lane 4q + p row
     // q, columns 4p ..) and get a column's 4 rows each
-    const int i = l & 15, g = l >> 4, r = 4 * (g >> 1) + (i >> 2);
-    const int c = c0 / 8 + 2 * (g & 1) + ((i & 3) >> 1);
-    const T* lp = L + (r0 + r) * LD + (c ^ place_of<CR>(r)) * 8 + 4 * (i & 1);
-    const T* hp = L + (r0 + r + 8) * LD + (c ^ place_of<CR>(r + 8)) * 8 + 4 * (i & 1);
+    const char* lp = p + (at.col ^ (c0 * 2));
+    const char* hp = p + 8 * ROW + (at.col ^ (c0 * 2 ^ place_of<CR>(8) * 16));
     const v4i16 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)lp);
     const v4i16 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)hp);
     const v8i16 f = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     return __builtin_bit_cast(typename Ops<T>::frag, f);
   } else {
-    const int c = (c0 + (l & 31)) / 4, r = 4 * (l >> 5);
     v8f f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int rr = r + (i & 3) + 8 * (i >> 2);
-      f[i] = L[(r0 + rr) * LD + (c ^ place_of<CR>(rr)) * 4 + (l & 3)];
+      const int x = (i & 3) + 8 * (i >> 2);
+      f[i] = *reinterpret_cast<const float*>(p + x * ROW +
+                                             (at.col ^ (c0 * 4 ^ place_of<CR>(x) * 16)));
     }
     return f;
   }
@@ -504,8 +536,10 @@ __global__ void __launch_bounds__(64 * NW, (kRowFit<T, DP>)) fwd_kernel(AttnArgs
 #pragma unroll
   for (int d = 0; d < ND; ++d) o[d] = zero16();
   float m = -kInf, sum = 0.f;
+  Lane<T, DP> at;
 
   stream_keys<T, DP, NW>(a, w, kt, it0, it1, [&](const T* K, const T* V, int j0) {
+    at.fresh();
 #pragma unroll
     for (int sub = 0; sub < BN / 32; ++sub) {
       const int js = j0 + sub * 32;
@@ -513,7 +547,7 @@ __global__ void __launch_bounds__(64 * NW, (kRowFit<T, DP>)) fwd_kernel(AttnArgs
       if (cover == 0) continue;
       v16f s = zero16();
 #pragma unroll
-      for (int k = 0; k < KD; ++k) s = Ops<T>::mma(row_frag<T, DP>(K, sub * 32, k), qf[k], s);
+      for (int k = 0; k < KD; ++k) s = Ops<T>::mma(row_frag<T, DP>(K, at, sub * 32, k), qf[k], s);
       if (cover == 1) hide(s, w.seen(js, a));
       float mx = s[0];
 #pragma unroll
@@ -547,7 +581,7 @@ __global__ void __launch_bounds__(64 * NW, (kRowFit<T, DP>)) fwd_kernel(AttnArgs
         const frag pf = acc_frag<T>(s, ss);
 #pragma unroll
         for (int d = 0; d < ND; ++d)
-          o[d] = Ops<T>::mma(col_frag<T, DP>(V, sub * 32 + ss * 16, d * 32), pf, o[d]);
+          o[d] = Ops<T>::mma(col_frag<T, DP>(V, at, sub * 32 + ss * 16, d * 32), pf, o[d]);
       }
     }
   });
@@ -558,9 +592,9 @@ __global__ void __launch_bounds__(64 * NW, (kRowFit<T, DP>)) fwd_kernel(AttnArgs
   const float lse = none ? kInf : m + log2f(sum);
   if (!w.live) return;
   if (SPLIT) {
-    const int64_t at = ((int64_t)blockIdx.z * gridDim.x + w.bh) * (a.Tq * a.G) + w.r;
-    if (h == 0) a.lpart[at] = none ? -kInf : lse;
-    put<T, float, ND>(a.opart + at * a.D, o, inv, none, a.D, h);
+    const int64_t row = ((int64_t)blockIdx.z * gridDim.x + w.bh) * (a.Tq * a.G) + w.r;
+    if (h == 0) a.lpart[row] = none ? -kInf : lse;
+    put<T, float, ND>(a.opart + row * a.D, o, inv, none, a.D, h);
     return;
   }
   if (h == 0 && a.lse != nullptr) a.lse[(int64_t)w.bh * (a.Tq * a.G) + w.r] = lse;
@@ -660,9 +694,9 @@ __global__ void __launch_bounds__(64 * NW, (kRowFit<T, DP>)) dq_kernel(AttnArgs 
     for (int i = 0; i < 8; ++i) delta += (float)gf[k][i] * (float)of[i];
   }
   delta = -halves_sum(delta);
-  const int64_t at = (int64_t)w.bh * (a.Tq * a.G) + w.r;
-  if (w.live && h == 0) a.delta[at] = delta;
-  const float lse = w.p >= 0 ? a.lse[at] : kInf;
+  const int64_t row = (int64_t)w.bh * (a.Tq * a.G) + w.r;
+  if (w.live && h == 0) a.delta[row] = delta;
+  const float lse = w.p >= 0 ? a.lse[row] : kInf;
 
   // dP - delta comes out of the matrix units: they start from -delta (in fp32
   // with heads over 32, whose registers are full, it is added afterwards)
@@ -674,7 +708,9 @@ __global__ void __launch_bounds__(64 * NW, (kRowFit<T, DP>)) dq_kernel(AttnArgs 
   v16f dq[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) dq[d] = zero16();
+  Lane<T, DP> at;
   stream_keys<T, DP, NW>(a, w, kt, 0, w.tiles, [&](const T* K, const T* V, int j0) {
+    at.fresh();
 #pragma unroll
     for (int sub = 0; sub < BN / 32; ++sub) {
       const int js = j0 + sub * 32;
@@ -683,8 +719,8 @@ __global__ void __launch_bounds__(64 * NW, (kRowFit<T, DP>)) dq_kernel(AttnArgs 
       v16f s = zero16(), dp = minus;
 #pragma unroll
       for (int k = 0; k < KD; ++k) {
-        s = Ops<T>::mma(row_frag<T, DP>(K, sub * 32, k), qf[k], s);
-        dp = Ops<T>::mma(row_frag<T, DP>(V, sub * 32, k), gf[k], dp);
+        s = Ops<T>::mma(row_frag<T, DP>(K, at, sub * 32, k), qf[k], s);
+        dp = Ops<T>::mma(row_frag<T, DP>(V, at, sub * 32, k), gf[k], dp);
       }
       if (cover == 1) hide(s, w.seen(js, a));
 #pragma unroll
@@ -694,7 +730,7 @@ __global__ void __launch_bounds__(64 * NW, (kRowFit<T, DP>)) dq_kernel(AttnArgs 
         const frag sf = acc_frag<T>(s, ss);
 #pragma unroll
         for (int d = 0; d < ND; ++d)
-          dq[d] = Ops<T>::mma(col_frag<T, DP>(K, sub * 32 + ss * 16, d * 32), sf, dq[d]);
+          dq[d] = Ops<T>::mma(col_frag<T, DP>(K, at, sub * 32 + ss * 16, d * 32), sf, dq[d]);
       }
     }
   });
@@ -835,8 +871,10 @@ template <typename T, int DP>
 struct KeyGrad {
   static constexpr int KD = DP / 16, ND = DP / 32;
   typedef typename Ops<T>::frag frag;
+  static constexpr int kAhead = 4;
   frag kf[KD], vf[KD];
   v16f dk[ND], dv[ND];
+  Lane<T, DP> at;
 
   __device__ __forceinline__ void init(const AttnArgs& a, int b, int hk, int key, bool ok) {
     const int h = (threadIdx.x & 63) >> 5;
@@ -857,7 +895,6 @@ struct KeyGrad {
     const int cover = kr.coverage(r0);
     if (cover == 0) return;
     const int h = (threadIdx.x & 63) >> 5;
-    const float c = a.scale * kLog2e;
     v16f s = zero16(), dp;
 #pragma unroll
     for (int e4 = 0; e4 < 4; ++e4) {
@@ -867,10 +904,99 @@ struct KeyGrad {
     }
 #pragma unroll
     for (int k = 0; k < KD; ++k) {
-      s = Ops<T>::mma(row_frag<T, DP>(b.q, i0, k), kf[k], s);
-      dp = Ops<T>::mma(row_frag<T, DP>(b.g, i0, k), vf[k], dp);
+      s = Ops<T>::mma(row_frag<T, DP>(b.q, at, i0, k), kf[k], s);
+      dp = Ops<T>::mma(row_frag<T, DP>(b.g, at, i0, k), vf[k], dp);
     }
     if (cover == 1) hide(s, kr.seen(r0, h));
+    weigh(a, b, i0, s, dp);
+    add(b, i0, s, dp);
+  }
+
+  // The 64 rows of a tile in one fixed sequence of products: those of one
+  // half run beside the powers of the other, and a product's left operand is
+  // read kAhead products before it.  The compiler's own order reads an operand
+  // right before its product and keeps the powers apart from the products.
+  // 8192 tokens, heads of 128: 217 -> 187 us (32% of the matrix units' time,
+  // one wave a SIMD: an instruction of a lone wave takes 6 cycles to issue,
+  // 33 ns for a product of 17 with all that goes with it); heads of 64: 69 ->
+  // 67 us.  Reading 8 ahead, or a second copy of the sequence without masks,
+  // is not faster (195, 227 us).
+  __device__ __forceinline__ void rows64(const AttnArgs& a, const RowBuf<T>& b, int r0,
+                                         const KeyRows& kr) {
+    constexpr int HALF = 2 * KD, SUMS = 4 * ND, ALL = 2 * (HALF + SUMS);
+    constexpr int E = (16 + HALF - 1) / HALF;  // powers beside a product
+    const int h = (threadIdx.x & 63) >> 5;
+    const float c = a.scale * kLog2e;
+    auto left = [&](auto ic) {
+      constexpr int i = decltype(ic)::value, j = i - 2 * HALF;
+      if constexpr (i < 2 * HALF)
+        return row_frag<T, DP>(i % 2 == 0 ? b.q : b.g, at, i / HALF * 32, i % HALF / 2);
+      else
+        return col_frag<T, DP>(i % 2 == 0 ? b.g : b.q, at, j / (2 * ND) * 16, j / 2 % ND * 32);
+    };
+    frag ring[kAhead];
+    v16f s[2] = {zero16(), zero16()}, dp[2];
+    v4f le[2][4];
+    frag pf[2][2], sf[2][2];
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+      for (int e4 = 0; e4 < 4; ++e4) {
+        const v4f de = *reinterpret_cast<const v4f*>(b.delta + sub * 32 + acc_row(e4 * 4, h));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dp[sub][e4 * 4 + i] = de[i];
+      }
+    const bool mixed[2] = {kr.coverage(r0) != 2, kr.coverage(r0 + 32) != 2};
+    each<kAhead>([&](auto ic) { ring[decltype(ic)::value] = left(ic); });
+    each<ALL>([&](auto ic) {
+      constexpr int i = decltype(ic)::value;
+      const frag f = ring[i % kAhead];
+      if constexpr (i == HALF || i == 2 * HALF) {
+        constexpr int sub = i / HALF - 1;
+        if (mixed[sub]) hide(s[sub], kr.seen(r0 + sub * 32, h));
+      }
+      if constexpr (i < 2 * HALF) {
+        constexpr int sub = i / HALF, k = i % HALF / 2;
+        if constexpr (i % 2 == 0) s[sub] = Ops<T>::mma(f, kf[k], s[sub]);
+        else dp[sub] = Ops<T>::mma(f, vf[k], dp[sub]);
+      } else {
+        constexpr int j = i - 2 * HALF, sub = j / SUMS, ss = j % SUMS / (2 * ND), d = j / 2 % ND;
+        if constexpr (i % 2 == 0) dv[d] = Ops<T>::mma(f, pf[sub][ss], dv[d]);
+        else dk[d] = Ops<T>::mma(f, sf[sub][ss], dk[d]);
+      }
+      if constexpr (i + kAhead < ALL)
+        ring[i % kAhead] = left(std::integral_constant<int, i + kAhead>());
+      // the first half's powers beside the second half's scores, the second
+      // half's beside the first half's sums
+      each<2>([&](auto subc) {
+        constexpr int sub = decltype(subc)::value, o = i - HALF * (1 + sub) - 1;
+        if constexpr (o == -2)
+          each<4>([&](auto e4) {
+            le[sub][e4] = *reinterpret_cast<const v4f*>(b.lse + sub * 32 + acc_row(e4 * 4, h));
+          });
+        if constexpr (o >= 0 && o * E < 16)
+          each<E>([&](auto ec) {
+            constexpr int e = o * E + decltype(ec)::value;
+            if constexpr (e < 16) {
+              const float x = __builtin_fmaf(s[sub][e], c, -le[sub][e / 4][e % 4]);
+              s[sub][e] = ex2(x);
+              dp[sub][e] *= s[sub][e];
+              if constexpr (e % 8 == 7) {
+                pf[sub][e / 8] = acc_frag<T>(s[sub], e / 8);
+                sf[sub][e / 8] = acc_frag<T>(dp[sub], e / 8);
+              }
+            }
+          });
+      });
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  }
+
+  // scores and dO V^T - delta become P and dS
+  __device__ __forceinline__ void weigh(const AttnArgs& a, const RowBuf<T>& b, int i0, v16f& s,
+                                        v16f& dp) {
+    const int h = (threadIdx.x & 63) >> 5;
+    const float c = a.scale * kLog2e;
 #pragma unroll
     for (int e4 = 0; e4 < 4; ++e4) {
       const v4f le = *reinterpret_cast<const v4f*>(b.lse + i0 + acc_row(e4 * 4, h));
@@ -881,13 +1007,16 @@ struct KeyGrad {
         dp[e] *= s[e];
       }
     }
+  }
+
+  __device__ __forceinline__ void add(const RowBuf<T>& b, int i0, const v16f& s, const v16f& dp) {
 #pragma unroll
     for (int ss = 0; ss < 2; ++ss) {
       const frag pf = acc_frag<T>(s, ss), sf = acc_frag<T>(dp, ss);
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
-        dv[d] = Ops<T>::mma(col_frag<T, DP>(b.g, i0 + ss * 16, d * 32), pf, dv[d]);
-        dk[d] = Ops<T>::mma(col_frag<T, DP>(b.q, i0 + ss * 16, d * 32), sf, dk[d]);
+        dv[d] = Ops<T>::mma(col_frag<T, DP>(b.g, at, i0 + ss * 16, d * 32), pf, dv[d]);
+        dk[d] = Ops<T>::mma(col_frag<T, DP>(b.q, at, i0 + ss * 16, d * 32), sf, dk[d]);
       }
     }
   }
@@ -937,6 +1066,7 @@ dkv_kernel(AttnArgs a, int key_blocks) {
       rs.fetch(a, t0, rb, b0);
       if (NW > 2) rs.fetch(a, t0 + BN, rb, b1);
       arrived();
+      kg.at.fresh();
       if (t0 + wave * 32 < rb)
         kg.rows(a, NW <= 2 || wave < 2 ? b0 : b1, (wave & 1) * 32, t0 + wave * 32, kr);
     }
@@ -980,6 +1110,11 @@ dkv_kernel(AttnArgs a, int key_blocks) {
   const KeyRows kr(k0 + group * 32, key, a, seq);
   kg.init(a, b, hk, key, key < seq.len);
   auto step = [&](const RowBuf<T>& buf, int t0) {
+    kg.at.fresh();
+    if constexpr (RS == 1 && sizeof(T) == 2) {
+      if (kr.coverage(t0) != 0 || kr.coverage(t0 + 32) != 0) kg.rows64(a, buf, t0, kr);
+      return;
+    }
 #pragma unroll
     for (int sub = 0; sub < BN / 32; sub += RS) {
       const int i0 = (sub + (RS > 1 ? turn : 0)) * 32;
@@ -1075,8 +1210,8 @@ void backward_dp(const AttnArgs& a, hipStream_t st) {
                          st>>>(a);
   const int kb = (int)ceil_div(a.Tk, 32 * KG);
   const dim3 grid(bh, (unsigned)(kb + a.sink_groups * a.far_chunks));
-  // up to one wave a SIMD: two share a group of keys (fp32 padded batch, 500
-  // waves: 60 -> 52 us)
+  // up to one wave a SIMD: two share a group of keys (fp32 padded batch, 520
+  // waves: 60 -> 44 us)
   if (KG == 2 && (int64_t)bh * kb * KG <= 1024)
     dkv_kernel<T, DP, KG, KG == 2 ? 2 : 1><<<grid, 64 * KG * 2, 0, st>>>(a, kb);
   else

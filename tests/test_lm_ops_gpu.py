@@ -45,6 +45,22 @@ ATTN = [
 
 
 @pytest.mark.parametrize('dtype', sorted(DTYPES))
+@pytest.mark.parametrize('d', [24, 64, 88, 128])
+def test_attention_with_many_heads(cuda, d, dtype):
+    """Enough blocks that no two waves share keys; sinks over two groups of
+    keys, far rows in chunks."""
+    dt = DTYPES[dtype]
+    q, k, v, do = (rand(cuda, 2, 27, 600, d, seed=s, dtype=dt) for s in range(4))
+    for x in (q, k, v):
+        x.requires_grad_()
+    out = window_attention(q, k, v, window=70, sinks=35)
+    got = (out, *torch.autograd.grad(out, (q, k, v), do))
+    want, tol = ref.attention(q, k, v, window=70, sinks=35, do=do)
+    for name, *x in zip(('out', 'dq', 'dk', 'dv'), got, want, tol):
+        ref.check(name, *x)
+
+
+@pytest.mark.parametrize('dtype', sorted(DTYPES))
 @pytest.mark.parametrize('case', ATTN, ids=lambda c: '-'.join(str(x) for x in c[:8]))
 def test_attention_matches_formula(cuda, case, dtype):
     b, hq, hk, tq, tk, d, window, sinks, lengths, start = case

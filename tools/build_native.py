@@ -32,6 +32,13 @@ ARCH = os.environ.get('KFAC_OFFLOAD_ARCH', 'gfx950')
 NO_PACKED_FP32 = ('distill.hip', 'rotary.hip', 'window_attn.hip')
 NO_PACKED_FLAGS = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 
+# Matrix results that the vector unit reads next stay in vector registers.  By
+# default a kernel of more than 256 registers keeps all of them in the
+# accumulation half and copies each out before its use (key gradients, heads
+# of 128: 124 copies a tile; fp32 there spills 27 registers, and none with it).
+MATRIX_IN_VGPRS = ('window_attn.hip',)
+MATRIX_IN_VGPRS_FLAGS = ['-mllvm', '-amdgpu-mfma-vgpr-form=1']
+
 
 def _hipcc() -> str:
     rocm = os.environ.get('ROCM_PATH', '/opt/rocm')
@@ -115,6 +122,8 @@ def build(force: bool = False, jobs: int = 8, verbose: bool = False) -> str:
         obj = os.path.join(BUILD, os.path.basename(src) + '.o')
         objs.append(obj)
         extra = NO_PACKED_FLAGS if os.path.basename(src) in NO_PACKED_FP32 else []
+        if os.path.basename(src) in MATRIX_IN_VGPRS:
+            extra = extra + MATRIX_IN_VGPRS_FLAGS
         cmd = [hipcc, *common, *extra, '-c', src, '-o', obj]
         if force or _newer([src] + header_deps, obj) or _other_command(cmd, obj):
             jobs_list.append((cmd, obj))
