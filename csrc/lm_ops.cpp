@@ -152,19 +152,27 @@ kfac::AttnArgs attn_args(const at::Tensor& q, const at::Tensor& k, const at::Ten
 }
 
 // out [B, Hq, Tq, D] over memory laid out [B, Tq, Hq, D] (what the output
-// projection reads), and the rows' lse where a backward pass may follow
-std::tuple<at::Tensor, at::Tensor> attn_forward(const at::Tensor& q, const at::Tensor& k,
-                                                const at::Tensor& v, const OptTensor& lengths,
-                                                const OptTensor& starts, const AttnConf& c,
-                                                bool want_lse) {
+// projection reads), and where a backward pass may follow the rows' lse and,
+// for 16-bit types and short windows, what out's rounding took away
+std::tuple<at::Tensor, at::Tensor, at::Tensor> attn_forward(const at::Tensor& q,
+                                                            const at::Tensor& k,
+                                                            const at::Tensor& v,
+                                                            const OptTensor& lengths,
+                                                            const OptTensor& starts,
+                                                            const AttnConf& c, bool training) {
   c10::hip::HIPGuardMasqueradingAsCUDA g(q.device());
   kfac::AttnArgs a = attn_args(q, k, v, lengths, starts, c);
   at::Tensor out = at::empty({a.B, a.Tq, a.Hq, a.D}, q.options()).transpose(1, 2);
-  at::Tensor lse;
-  if (want_lse) lse = at::empty({a.B * a.Hkv, (int64_t)a.Tq * a.G}, q.options().dtype(at::kFloat));
+  at::Tensor lse, rest;
+  if (training) {
+    lse = at::empty({a.B * a.Hkv, (int64_t)a.Tq * a.G}, q.options().dtype(at::kFloat));
+    if (q.scalar_type() != at::kFloat && kfac::attn_keeps_rest(a))
+      rest = at::empty({a.B, a.Tq, a.Hq, a.D}, q.options());
+  }
   a.out = out.data_ptr();
   strides3(out, a.os);
-  a.lse = want_lse ? lse.data_ptr<float>() : nullptr;
+  a.rest = rest.defined() ? rest.data_ptr() : nullptr;
+  a.lse = training ? lse.data_ptr<float>() : nullptr;
   int64_t floats = 0;
   kfac::attn_plan(a, &a.splits, &floats);
   at::Tensor ws;
@@ -176,7 +184,7 @@ std::tuple<at::Tensor, at::Tensor> attn_forward(const at::Tensor& q, const at::T
   }
   kfac::attn_forward(tag(q), a, stream());
   C10_HIP_KERNEL_LAUNCH_CHECK();
-  return {out, lse};
+  return {out, lse, rest};
 }
 
 int64_t groups(const at::Tensor& q, const at::Tensor& k) {
@@ -193,8 +201,8 @@ struct WindowAttnFn : public torch::autograd::Function<WindowAttnFn> {
     const AttnConf c{window, sinks, start, start_given, scale};
     const int64_t G = groups(q_, k_);
     const at::Tensor q = operand(q_, G), k = operand(k_, 1), v = operand(v_, 1);
-    auto [out, lse] = attn_forward(q, k, v, lengths, starts, c, true);
-    ctx->save_for_backward({q, k, v, out, lse, lengths.has_value() ? *lengths : at::Tensor(),
+    auto [out, lse, rest] = attn_forward(q, k, v, lengths, starts, c, true);
+    ctx->save_for_backward({q, k, v, out, lse, rest, lengths.has_value() ? *lengths : at::Tensor(),
                             starts.has_value() ? *starts : at::Tensor()});
     ctx->saved_data["conf"] = pack(c);
     return out;
@@ -202,10 +210,10 @@ struct WindowAttnFn : public torch::autograd::Function<WindowAttnFn> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once_only("window_attention");
     auto sv = ctx->get_saved_variables();
-    const at::Tensor &q = sv[0], &k = sv[1], &v = sv[2], &out = sv[3], &lse = sv[4];
+    const at::Tensor &q = sv[0], &k = sv[1], &v = sv[2], &out = sv[3], &lse = sv[4], &rest = sv[5];
     const AttnConf c = unpack(ctx->saved_data["conf"].toDoubleVector());
-    const OptTensor lengths = sv[5].defined() ? OptTensor(sv[5]) : c10::nullopt;
-    const OptTensor starts = sv[6].defined() ? OptTensor(sv[6]) : c10::nullopt;
+    const OptTensor lengths = sv[6].defined() ? OptTensor(sv[6]) : c10::nullopt;
+    const OptTensor starts = sv[7].defined() ? OptTensor(sv[7]) : c10::nullopt;
     c10::hip::HIPGuardMasqueradingAsCUDA g(q.device());
     kfac::AttnArgs a = attn_args(q, k, v, lengths, starts, c);
     const at::Tensor go = operand(grads[0], a.G);
@@ -216,6 +224,7 @@ struct WindowAttnFn : public torch::autograd::Function<WindowAttnFn> {
     } else {
       a.out = out.data_ptr();
       strides3(out, a.os);
+      a.rest = rest.defined() ? rest.data_ptr() : nullptr;
       a.dout = go.data_ptr();
       strides3(go, a.dos);
       a.dq = dq.data_ptr();

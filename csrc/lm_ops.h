@@ -78,6 +78,7 @@ struct AttnArgs {
   int64_t dos[3];
   void* out;                    // [B, Hq, Tq, D] with strides os
   int64_t os[3];
+  void* rest;                   // what out's rounding took away, laid out like out, or null
   float* lse;                   // [B * Hkv, Tq * G] (rows), log2 units; +inf: sees nothing
   float* delta;                 // the same: -do . o
   void *dq, *dk, *dv;
@@ -98,6 +99,7 @@ struct AttnArgs {
 
 // how a forward call is split over the keys, and the floats of its partial
 // results; the same for the backward call's sinks
+bool attn_keeps_rest(const AttnArgs& a);
 void attn_plan(const AttnArgs& a, int* splits, int64_t* floats);
 void attn_bwd_plan(const AttnArgs& a, int* sink_groups, int* far_chunks, int64_t* floats);
 void attn_forward(int dtype, const AttnArgs& a, hipStream_t st);

@@ -390,6 +390,28 @@ __device__ __forceinline__ void put(O* out, const v16f (&x)[ND], float f, bool z
     }
 }
 
+// what rounding x times f to T takes away, rounded to T itself
+template <typename T, int ND>
+__device__ __forceinline__ void put_rest(T* out, const v16f (&x)[ND], float f, bool zero, int D,
+                                         int h) {
+  typedef T quad __attribute__((ext_vector_type(4)));
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int e4 = 0; e4 < 4; ++e4) {
+      const int dd = d * 32 + acc_row(e4 * 4, h);
+      if (dd < D) {
+        v4f v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[i] = zero ? 0.f : x[d][e4 * 4 + i] * f;
+          v[i] -= (float)(T)v[i];
+        }
+        *reinterpret_cast<quad*>(out + dd) = __builtin_convertvector(v, quad);
+      }
+    }
+}
+
 // What a block of the row kernels (forward, dq) works on.
 template <int NW>
 struct RowBlock {
@@ -512,6 +534,14 @@ __device__ __forceinline__ void stream_keys(const AttnArgs& a, const RowBlock<NW
 }
 
 // ---------------------------------------------------------------- forward
+// 8192 tokens, 16 heads of 128 over 4, window 1024: 95 us, 690 TFLOP/s, the
+// matrix units busy for 32% and the vector unit for 36% of it with two waves a
+// SIMD, as many as the tiles leave room for.  GPT-NeoX batch (8 x 2048 tokens,
+// 12 heads of 64, window 256): 38 us; a block sees 7 tiles there, one of them
+// the sinks', and a product of 64 elements is shorter than its powers.
+// SPLIT, for few rows: the keys over blockIdx.z.  16 sequences of one token,
+// 32 heads of 128 over 8, 4096 keys each: 54 us and 5 to join, 4.6 TB/s of
+// keys and values.
 template <typename T, int DP, int NW, bool SPLIT>
 __global__ void __launch_bounds__(64 * NW, (kRowFit<T, DP>)) fwd_kernel(AttnArgs a) {
   constexpr int KD = DP / 16, ND = DP / 32;
@@ -598,8 +628,10 @@ __global__ void __launch_bounds__(64 * NW, (kRowFit<T, DP>)) fwd_kernel(AttnArgs
     return;
   }
   if (h == 0 && a.lse != nullptr) a.lse[(int64_t)w.bh * (a.Tq * a.G) + w.r] = lse;
-  put<T, T, ND>(reinterpret_cast<T*>(a.out) + w.b * a.os[0] + w.head * a.os[1] + w.t * a.os[2], o,
-                inv, none, a.D, h);
+  const int64_t at_out = w.b * a.os[0] + w.head * a.os[1] + w.t * a.os[2];
+  put<T, T, ND>(reinterpret_cast<T*>(a.out) + at_out, o, inv, none, a.D, h);
+  if (sizeof(T) == 2 && a.rest != nullptr)
+    put_rest<T, ND>(reinterpret_cast<T*>(a.rest) + at_out, o, inv, none, a.D, h);
 }
 
 // Joins the key slices of a row: one block a row, 8 lanes groups of 32 (4
@@ -658,18 +690,35 @@ __global__ void __launch_bounds__(NT) join_kernel(AttnArgs a) {
   const int bh = (int)(row / rows), b = bh / a.Hkv;
   const Row rw((int)(row - (int64_t)bh * rows), a);
   const int head = (bh - b * a.Hkv) * a.G + rw.g;
-  if (d < a.D)
-    *reinterpret_cast<typename Ops<T>::quad*>(reinterpret_cast<T*>(a.out) + b * a.os[0] +
-                                              head * a.os[1] + rw.t * a.os[2] + d) =
+  if (d < a.D) {
+    const int64_t at = b * a.os[0] + head * a.os[1] + rw.t * a.os[2] + d;
+    *reinterpret_cast<typename Ops<T>::quad*>(reinterpret_cast<T*>(a.out) + at) =
         __builtin_convertvector(o, typename Ops<T>::quad);
+    if (sizeof(T) == 2 && a.rest != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] -= (float)(T)o[i];
+      *reinterpret_cast<typename Ops<T>::quad*>(reinterpret_cast<T*>(a.rest) + at) =
+          __builtin_convertvector(o, typename Ops<T>::quad);
+    }
+  }
   if (tid == 0 && a.lse != nullptr)
     a.lse[row] = sum == 0.f ? kInf : base + log2f(sum);
+}
+
+// The factor of the gradients to q and k.  Where a row sees itself alone its
+// probability is 1 whatever they are, and the gradient exactly 0: not the
+// difference of two sums that were taken in different orders.
+__device__ __forceinline__ float score_factor(const AttnArgs& a) {
+  return a.W == 1 && (a.S == 0 || a.Tk == 1) ? 0.f : a.scale;
 }
 
 // --------------------------------------------------------------- backward
 // dq, and -delta = -do . o for the key-gradient kernel.  The forward's tiles
 // and layout once more: S^T = K Q^T, dP^T = V dO^T, dS^T = P (dP - delta),
-// dQ^T += K^T dS^T.
+// dQ^T += K^T dS^T.  8192 tokens, heads of 128: 140 us, 700 TFLOP/s; GPT-NeoX
+// batch 49 us.  The fixed order of KeyGrad::rows64 costs the second wave of a
+// SIMD its registers here (57 us for the latter), four waves a SIMD with 128
+// registers are no faster (49).
 template <typename T, int DP, int NW>
 __global__ void __launch_bounds__(64 * NW, (kRowFit<T, DP>)) dq_kernel(AttnArgs a) {
   constexpr int KD = DP / 16, ND = DP / 32;
@@ -682,7 +731,9 @@ __global__ void __launch_bounds__(64 * NW, (kRowFit<T, DP>)) dq_kernel(AttnArgs 
   const T* q = reinterpret_cast<const T*>(a.q) + w.b * a.qs[0] + w.head * a.qs[1] + w.t * a.qs[2];
   const T* g =
       reinterpret_cast<const T*>(a.dout) + w.b * a.dos[0] + w.head * a.dos[1] + w.t * a.dos[2];
-  const T* o = reinterpret_cast<const T*>(a.out) + w.b * a.os[0] + w.head * a.os[1] + w.t * a.os[2];
+  const int64_t at_out = w.b * a.os[0] + w.head * a.os[1] + w.t * a.os[2];
+  const T* o = reinterpret_cast<const T*>(a.out) + at_out;
+  const T* rest = reinterpret_cast<const T*>(a.rest) + at_out;
   frag qf[KD], gf[KD];
   float delta = 0.f;
 #pragma unroll
@@ -692,6 +743,11 @@ __global__ void __launch_bounds__(64 * NW, (kRowFit<T, DP>)) dq_kernel(AttnArgs 
     const frag of = global_frag<T>(o, k * 16 + 8 * h, a.D, w.p >= 0);
 #pragma unroll
     for (int i = 0; i < 8; ++i) delta += (float)gf[k][i] * (float)of[i];
+    if (sizeof(T) == 2 && a.rest != nullptr) {
+      const frag rf = global_frag<T>(rest, k * 16 + 8 * h, a.D, w.p >= 0);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) delta += (float)gf[k][i] * (float)rf[i];
+    }
   }
   delta = -halves_sum(delta);
   const int64_t row = (int64_t)w.bh * (a.Tq * a.G) + w.r;
@@ -736,7 +792,7 @@ __global__ void __launch_bounds__(64 * NW, (kRowFit<T, DP>)) dq_kernel(AttnArgs 
   });
   if (!w.live) return;
   put<T, T, ND>(reinterpret_cast<T*>(a.dq) + w.b * a.dqs[0] + w.head * a.dqs[1] + w.t * a.dqs[2],
-                dq, a.scale, w.p < 0, a.D, h);
+                dq, score_factor(a), w.p < 0, a.D, h);
 }
 
 __device__ __forceinline__ int clip(int64_t t, const AttnArgs& a) {
@@ -1156,11 +1212,11 @@ dkv_kernel(AttnArgs a, int key_blocks) {
   }
   if (a.far_chunks > 0 && key < a.S) {
     float* part = sink_part(a, bh, key / kSinkKeys, 0) + key % kSinkKeys * a.D;
-    put<T, float, ND>(part, kg.dk, a.scale, false, a.D, h);
+    put<T, float, ND>(part, kg.dk, score_factor(a), false, a.D, h);
     put<T, float, ND>(part + kSinkKeys * a.D, kg.dv, 1.f, false, a.D, h);
   } else if (key < a.Tk) {
     put<T, T, ND>(reinterpret_cast<T*>(a.dk) + b * a.dks[0] + hk * a.dks[1] + key * a.dks[2],
-                  kg.dk, a.scale, false, a.D, h);
+                  kg.dk, score_factor(a), false, a.D, h);
     put<T, T, ND>(reinterpret_cast<T*>(a.dv) + b * a.dvs[0] + hk * a.dvs[1] + key * a.dvs[2],
                   kg.dv, 1.f, false, a.D, h);
   }
@@ -1239,6 +1295,15 @@ void backward_type(const AttnArgs& a, hipStream_t st) {
 }
 
 }  // namespace
+
+// dP - delta is small where few keys share the weight, and the rounding of o
+// then weighs in delta: with a window of 2 the gradients of q and k are off by
+// 0.0037 of their norm (bf16), and by 0.0024 when delta also counts what that
+// rounding took away, of which their own rounding is 0.0017; of 6 0.0027, of 30
+// 0.0025, 0.0024 with it.  The first rows of a short sequence see as few keys.
+// Writing and reading it costs a tenth of the pass
+// (GPT-NeoX batch, window 256: 171 us against 155).
+bool attn_keeps_rest(const AttnArgs& a) { return std::min<int64_t>((int64_t)a.W + a.S, a.Tk) <= 128; }
 
 void attn_plan(const AttnArgs& a, int* splits, int64_t* floats) {
   const int64_t rows = (int64_t)a.Tq * a.G;

@@ -45,6 +45,51 @@ ATTN = [
 
 
 @pytest.mark.parametrize('dtype', sorted(DTYPES))
+@pytest.mark.parametrize('n', [2, 60])
+def test_attention_gradients_between_two_values_one_step_apart(cuda, dtype, n):
+    """The output lies halfway between two numbers of its type: gradients that
+    go by the rounded output are all wrong, those of the formula are exact.
+    Short windows, whose few keys do not average that out."""
+    dt, d = DTYPES[dtype], 64
+    eps = torch.finfo(dt).eps
+    q = torch.zeros(1, 1, 2, d, dtype=dt, device=cuda, requires_grad=True)
+    k = torch.zeros(1, 1, n, d, dtype=dt, device=cuda)
+    k[:, :, :2] = rand(cuda, 1, 1, 2, d, seed=1, dtype=dt)
+    k[:, :, -2:] = k[:, :, :2]
+    v = torch.ones(1, 1, n, d, dtype=dt, device=cuda)
+    v[:, :, 0::2] += eps
+    out = window_attention(q, k, v, window=n)
+    (dq,) = torch.autograd.grad(out[:, :, 1].sum() / eps, q)
+    # P = 1 / n, dP - delta = +-d / 2, so dq = d ** -0.5 / n * d / 2 * sum of
+    # +-k; one rounding (dS is a power of two, or rounds once more by n).  dP
+    # and delta are each a sum of d terms of 1 / eps in 32 bits, off by
+    # d * 2^-24 of d / eps at most: in fp32 that is more than their difference.
+    sign = torch.where(torch.arange(n, device=cuda) % 2 == 0, 1.0, -1.0).double()
+    terms = sign[:, None] * k[0, 0].double()
+    want = d ** -0.5 / n * d / 2 * terms.sum(0)
+    sums = 2 * d * 2.0 ** -24 * d / eps
+    tol = ((2 * eps + 2.0 ** -12) * d / 2 + sums) * d ** -0.5 / n * terms.abs().sum(0)
+    ref.check('dq', dq[0, 0, 1], want.cpu(), tol.cpu())
+
+
+@pytest.mark.parametrize('dtype', sorted(DTYPES))
+@pytest.mark.parametrize('d', [16, 64, 128])
+def test_a_token_that_sees_itself_alone(cuda, d, dtype):
+    dt = DTYPES[dtype]
+    q, k, v, do = (rand(cuda, 2, 4, 90, d, seed=s, dtype=dt) for s in range(4))
+    for x in (q, k, v):
+        x.requires_grad_()
+    out = window_attention(q, k, v, window=1)
+    dq, dk, dv = torch.autograd.grad(out, (q, k, v), do)
+    # powers of 2 are off by the scores' 32-bit rounding, 40 * 2^-24: below half
+    # a step of the 16-bit types, which give the values back as they are
+    off = 2.0 ** -18 if dtype == 'fp32' else 0.0
+    for got, want in ((out, v), (dv, do)):
+        assert bool(((got - want).abs() <= off * want.abs()).all())
+    assert not bool(dq.any()) and not bool(dk.any())
+
+
+@pytest.mark.parametrize('dtype', sorted(DTYPES))
 @pytest.mark.parametrize('d', [24, 64, 88, 128])
 def test_attention_with_many_heads(cuda, d, dtype):
     """Enough blocks that no two waves share keys; sinks over two groups of
