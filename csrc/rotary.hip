@@ -9,9 +9,9 @@
 // little else, so it is bound by memory as long as the trigonometry is done
 // once per (token, pair) and not once per head: a thread owns one 16-byte
 // unit of a token's head and walks the heads, q's first and k's after them.
-// GPT-NeoX batch (8 x 2048 tokens, q and k of 12 heads of 64, bf16): 20 us,
-// 5 TB/s; 2 x 4719 video tokens, 16 + 4 heads of 128 in fp32, three axes: 48 us,
-// 4 TB/s.
+// GPT-NeoX batch (8 x 2048 tokens, q and k of 12 heads of 64, bf16): 27 us,
+// 3.7 TB/s; 2 x 4719 video tokens, 16 + 4 heads of 128 in fp32, three axes: 48
+// us, 4 TB/s.
 // Angles are formed in turns in 64 bits (position 10^6 times frequency 1 is
 // 0.06 rad off in 32 bits), reduced to [-1/2, 1/2] turn there, and only the
 // rest goes to sincospif.
