@@ -236,20 +236,29 @@ __device__ __forceinline__ typename Ops<T>::frag acc_frag(const v16f& a, int s) 
 }
 
 // 8 elements of a global row from element d on; zeros behind D (D % 8 == 0)
+// and where the row is not `ok`.  Those lanes read `there`, the tensor's
+// beginning: with a branch round the load, a row's loads would wait for each
+// other.
 template <typename T>
-__device__ __forceinline__ typename Ops<T>::frag global_frag(const T* row, int d, int D, bool ok) {
+__device__ __forceinline__ typename Ops<T>::frag global_frag(const void* there, const T* row, int d,
+                                                             int D, bool ok) {
+  ok = ok && d < D;
+  const T* p = ok ? row + d : reinterpret_cast<const T*>(there);
   typename Ops<T>::frag f;
-  if (ok && d < D) {
-    if constexpr (sizeof(T) == 2) {
-      f = *reinterpret_cast<const typename Ops<T>::frag*>(row + d);
-    } else {
-      const v4f a = *reinterpret_cast<const v4f*>(row + d);
-      const v4f b = *reinterpret_cast<const v4f*>(row + d + 4);
-      f = v8f{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-    }
-  } else {
+  if constexpr (sizeof(T) == 2) {
+    typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+    v4u u = *reinterpret_cast<const v4u*>(p);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = (T)0.f;
+    for (int i = 0; i < 4; ++i) u[i] = ok ? u[i] : 0u;
+    f = __builtin_bit_cast(typename Ops<T>::frag, u);
+  } else {
+    const v4f a = *reinterpret_cast<const v4f*>(p);
+    const v4f b = *reinterpret_cast<const v4f*>(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[i] = ok ? a[i] : 0.f;
+      f[4 + i] = ok ? b[i] : 0.f;
+    }
   }
   return f;
 }
@@ -560,7 +569,7 @@ __global__ void __launch_bounds__(64 * NW, (kRowFit<T, DP>)) fwd_kernel(AttnArgs
   const T* q = reinterpret_cast<const T*>(a.q) + w.b * a.qs[0] + w.head * a.qs[1] + w.t * a.qs[2];
   frag qf[KD];
 #pragma unroll
-  for (int k = 0; k < KD; ++k) qf[k] = global_frag<T>(q, k * 16 + 8 * h, a.D, w.p >= 0);
+  for (int k = 0; k < KD; ++k) qf[k] = global_frag<T>(a.q, q, k * 16 + 8 * h, a.D, w.p >= 0);
 
   v16f o[ND];
 #pragma unroll
@@ -715,7 +724,7 @@ __device__ __forceinline__ float score_factor(const AttnArgs& a) {
 // --------------------------------------------------------------- backward
 // dq, and -delta = -do . o for the key-gradient kernel.  The forward's tiles
 // and layout once more: S^T = K Q^T, dP^T = V dO^T, dS^T = P (dP - delta),
-// dQ^T += K^T dS^T.  8192 tokens, heads of 128: 140 us, 700 TFLOP/s; GPT-NeoX
+// dQ^T += K^T dS^T.  8192 tokens, heads of 128: 130 us, 750 TFLOP/s; GPT-NeoX
 // batch 49 us.  The fixed order of KeyGrad::rows64 costs the second wave of a
 // SIMD its registers here (57 us for the latter), four waves a SIMD with 128
 // registers are no faster (49).
@@ -738,13 +747,16 @@ __global__ void __launch_bounds__(64 * NW, (kRowFit<T, DP>)) dq_kernel(AttnArgs 
   float delta = 0.f;
 #pragma unroll
   for (int k = 0; k < KD; ++k) {
-    qf[k] = global_frag<T>(q, k * 16 + 8 * h, a.D, w.p >= 0);
-    gf[k] = global_frag<T>(g, k * 16 + 8 * h, a.D, w.p >= 0);
-    const frag of = global_frag<T>(o, k * 16 + 8 * h, a.D, w.p >= 0);
+    qf[k] = global_frag<T>(a.q, q, k * 16 + 8 * h, a.D, w.p >= 0);
+    gf[k] = global_frag<T>(a.dout, g, k * 16 + 8 * h, a.D, w.p >= 0);
+    const frag of = global_frag<T>(a.out, o, k * 16 + 8 * h, a.D, w.p >= 0);
 #pragma unroll
     for (int i = 0; i < 8; ++i) delta += (float)gf[k][i] * (float)of[i];
-    if (sizeof(T) == 2 && a.rest != nullptr) {
-      const frag rf = global_frag<T>(rest, k * 16 + 8 * h, a.D, w.p >= 0);
+  }
+  if (sizeof(T) == 2 && a.rest != nullptr) {
+#pragma unroll
+    for (int k = 0; k < KD; ++k) {
+      const frag rf = global_frag<T>(a.rest, rest, k * 16 + 8 * h, a.D, w.p >= 0);
 #pragma unroll
       for (int i = 0; i < 8; ++i) delta += (float)gf[k][i] * (float)rf[i];
     }
@@ -936,10 +948,19 @@ struct KeyGrad {
     const int h = (threadIdx.x & 63) >> 5;
     const T* kp = reinterpret_cast<const T*>(a.k) + b * a.ks[0] + hk * a.ks[1] + key * a.ks[2];
     const T* vp = reinterpret_cast<const T*>(a.v) + b * a.vs[0] + hk * a.vs[1] + key * a.vs[2];
+    // with a branch each: the sums' registers fall out worse without (heads of
+    // 128: 200 us against 185)
+    auto load = [&](const T* p, int d) {
+      if (ok && d < a.D) return global_frag<T>(p, p, d, a.D, true);
+      frag f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = (T)0.f;
+      return f;
+    };
 #pragma unroll
     for (int k = 0; k < KD; ++k) {
-      kf[k] = global_frag<T>(kp, k * 16 + 8 * h, a.D, ok);
-      vf[k] = global_frag<T>(vp, k * 16 + 8 * h, a.D, ok);
+      kf[k] = load(kp, k * 16 + 8 * h);
+      vf[k] = load(vp, k * 16 + 8 * h);
     }
 #pragma unroll
     for (int d = 0; d < ND; ++d) dk[d] = dv[d] = zero16();
