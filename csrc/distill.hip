@@ -447,15 +447,19 @@ row_kernel(DistillArgs a) {
   __syncthreads();
   {
     // an index given twice counts with both its parts: `team` lanes of a wave
-    // add up the entries that name the column of entry k
+    // add up the entries that name the column of entry k (with more entries
+    // than threads, those of entry k + kRowThreads afterwards)
     int team = 64;
     while (team > 1 && team * a.K > kRowThreads) team >>= 1;
-    const int k = tid / team, part = tid & (team - 1);
-    float p = 0.f;
-    if (k < a.K && at[k] >= 0)
-      for (int i = part; i < a.K; i += team) p += at[i] == at[k] ? pk[i] : 0.f;
-    for (int off = team >> 1; off > 0; off >>= 1) p += __shfl_xor(p, off, 64);
-    if (k < a.K && part == 0) pj[k] = p;
+    const int part = tid & (team - 1);
+    for (int k0 = 0; k0 < a.K; k0 += kRowThreads / team) {
+      const int k = k0 + tid / team;
+      float p = 0.f;
+      if (k < a.K && at[k] >= 0)
+        for (int i = part; i < a.K; i += team) p += at[i] == at[k] ? pk[i] : 0.f;
+      for (int off = team >> 1; off > 0; off >>= 1) p += __shfl_xor(p, off, 64);
+      if (k < a.K && part == 0) pj[k] = p;
+    }
   }
   Run out{KFAC_NEG_INF, 0.f}, in{KFAC_NEG_INF, 0.f};
   float raw = KFAC_NEG_INF;  // largest logit so far

@@ -341,6 +341,25 @@ def test_distill_rows_in_registers(cuda, dtype, rest, v, k):
     ref.check('dz of sum', *torch.autograd.grad(summed, z), *want[2:])
 
 
+@pytest.mark.parametrize('rest', [False, True])
+@pytest.mark.parametrize('k', [100, 512, 513, 1024])
+@pytest.mark.parametrize('dtype, v', [('fp32', 32000), ('bf16', 65536)])
+def test_distill_many_entries_in_registers(cuda, dtype, v, k, rest):
+    """Up to twice as many entries as the block has threads, with columns that
+    several entries name, on one side of the 512th and across it."""
+    n, dt = 256, DTYPES[dtype]
+    z = (rand(cuda, n, v, seed=n) * 2).to(dt).requires_grad_()
+    t, i, r = _teacher(cuda, n, v, k, 2.0, rest, v)
+    i[2, 0] = i[2, k - 1]
+    i[5, k - 3] = i[5, k - 1] = i[5, 1]
+    i[9] = -1
+    i[11, k // 2:] = -1
+    loss = topk_distill_loss(z, t, i, teacher_rest=r, temperature=2.0, reduction='sum')
+    want = ref.distill(z, t, i, rest=r, temperature=2.0, reduction='sum')
+    ref.check('loss', loss, *want[:2])
+    ref.check('dz', *torch.autograd.grad(loss, z), *want[2:])
+
+
 def test_distill_rows_in_registers_alone(cuda):
     """Bad rows, views and no rows that count, where the forward writes the
     gradient."""
