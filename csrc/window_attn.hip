@@ -925,6 +925,8 @@ struct KeyRows {
     if (r0 + 32 <= any0 || r0 >= any1) return 0;
     return r0 >= full0 && r0 + 32 <= full1 ? 2 : 1;
   }
+  // some row sees this lane's key
+  __device__ __forceinline__ bool key_seen() const { return mine0 < mine1; }
   // bit o is row r0 + 4h + o
   __device__ __forceinline__ uint32_t seen(int r0, int h) const {
     const int first = r0 + 4 * h;
@@ -944,7 +946,11 @@ struct KeyGrad {
   v16f dk[ND], dv[ND];
   Lane<T, DP> at;
 
-  __device__ __forceinline__ void init(const AttnArgs& a, int b, int hk, int key, bool ok) {
+  // A key that no row sees is taken for zeros, as the row kernels do: it may
+  // hold anything, and 0 times that need not be 0.
+  __device__ __forceinline__ void init(const AttnArgs& a, int b, int hk, int key,
+                                       const KeyRows& kr) {
+    const bool ok = kr.key_seen();
     const int h = (threadIdx.x & 63) >> 5;
     const T* kp = reinterpret_cast<const T*>(a.k) + b * a.ks[0] + hk * a.ks[1] + key * a.ks[2];
     const T* vp = reinterpret_cast<const T*>(a.v) + b * a.vs[0] + hk * a.vs[1] + key * a.vs[2];
@@ -1137,7 +1143,7 @@ dkv_kernel(AttnArgs a, int key_blocks) {
     const int ra = rr.n1 + per * chunk < rr.f1 ? rr.n1 + per * chunk : rr.f1;
     const int rb = ra + per < rr.f1 ? ra + per : rr.f1;
     const KeyRows kr(j0, key, a, seq);
-    kg.init(a, b, hk, key, key < seq.len);
+    kg.init(a, b, hk, key, kr);
     for (int t0 = ra; t0 < rb; t0 += 32 * NW) {
       __syncthreads();
       rs.fetch(a, t0, rb, b0);
@@ -1185,7 +1191,7 @@ dkv_kernel(AttnArgs a, int key_blocks) {
   const RowRange<KG> rr(k0, a, seq);
   const int key = k0 + group * 32 + (l & 31);
   const KeyRows kr(k0 + group * 32, key, a, seq);
-  kg.init(a, b, hk, key, key < seq.len);
+  kg.init(a, b, hk, key, kr);
   auto step = [&](const RowBuf<T>& buf, int t0) {
     kg.at.fresh();
     if constexpr (RS == 1 && sizeof(T) == 2) {

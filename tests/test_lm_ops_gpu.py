@@ -130,6 +130,27 @@ def test_attention_matches_formula(cuda, case, dtype):
         assert torch.equal(window_attention(*x, **conf), out)
 
 
+@pytest.mark.parametrize('dtype', sorted(DTYPES))
+@pytest.mark.parametrize('d', [16, 64, 128])
+def test_keys_that_no_row_sees_may_hold_anything(cuda, d, dtype):
+    """A chunk of rows behind a cache, whose older entries are stale."""
+    dt = DTYPES[dtype]
+    q, do = (rand(cuda, 1, 4, 4, d, seed=s, dtype=dt) for s in range(2))
+    k, v = (rand(cuda, 1, 2, 64, d, seed=s, dtype=dt) for s in (2, 3))
+    conf = dict(window=8, sinks=3)
+    x = [t.requires_grad_() for t in (q, k, v)]
+    want = [window_attention(*x, **conf)]
+    want += torch.autograd.grad(want[0], x, do)
+    with torch.no_grad():
+        for bad, at in ((float('nan'), 40), (float('inf'), 52), (float('nan'), 3)):
+            k[:, :, at] = bad
+            v[:, :, at] = bad
+    got = [window_attention(*x, **conf)]
+    got += torch.autograd.grad(got[0], x, do)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
 TOKEN = [
     # b, hq, hk, tq, tk, d, window, sinks, lengths
     (1, 2, 2, 1, 1, 64, 1, 0, None),
