@@ -36,16 +36,17 @@ def _reference(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, s
     n = torch.full_like(p[:, :1], tk) if lengths is None else lengths.long().clamp(0, tk)[:, None, None]
     see = (j <= p) & ((p - j < window) | (j < sinks)) & (p < n) & (j < n)
     see = see[:, None]
-    # keys that no row sees may hold anything
-    used = see.any(dim=2)[..., None]
+    # keys that no row sees may hold anything, and so may rows of padding and
+    # what comes back for them
+    used, rows = see.any(dim=2)[..., None], see.any(dim=3)[..., None]
     kk = torch.where(used, k, 0.0).to(work).repeat_interleave(group, dim=1)
     vv = torch.where(used, v, 0.0).to(work).repeat_interleave(group, dim=1)
-    s = (q.to(work) @ kk.transpose(-1, -2)) * scale
+    s = (torch.where(rows, q, 0.0).to(work) @ kk.transpose(-1, -2)) * scale
     s = s.masked_fill(~see, float('-inf'))
     m = s.detach().amax(dim=-1, keepdim=True) if tk else s.new_zeros(*s.shape[:-1], 1)
     e = torch.exp(s - m.masked_fill(m == float('-inf'), 0.0))
     total = e.sum(dim=-1, keepdim=True)
-    o = (e / total.masked_fill(total == 0.0, 1.0)) @ vv
+    o = torch.where(rows, (e / total.masked_fill(total == 0.0, 1.0)) @ vv, 0.0)
     return o.to(q.dtype).transpose(1, 2).contiguous().transpose(1, 2)
 
 

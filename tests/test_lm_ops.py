@@ -143,6 +143,33 @@ def test_attention_formula(hq, hk, tq, tk, window, sinks, lengths, start):
         ref.check(name, g, w, t)
 
 
+def test_rows_of_padding_may_hold_anything():
+    q, k, v, do = (rand(2, h, 6, 8, seed=s) for s, h in enumerate((4, 2, 2, 4)))
+    conf = dict(window=2, sinks=1, lengths=torch.tensor([6, 3], dtype=torch.int32), q_start=0)
+    want, tol = ref.attention(q, k, v, do=do, **conf)
+    for x in (q, k, v, do):
+        x[1, :, 3:] = float('nan')
+    x = [t.requires_grad_() for t in (q, k, v)]
+    out = window_attention(*x, **conf)
+    got = [out, *torch.autograd.grad(out, x, do)]
+    for name, g, w, t in zip(('out', 'dq', 'dk', 'dv'), got, want, tol):
+        ref.check(name, g, w, t)
+
+
+def test_keys_that_no_row_sees_may_hold_anything():
+    q, do = (rand(1, 4, 4, 8, seed=s) for s in range(2))
+    k, v = (rand(1, 2, 64, 8, seed=s) for s in (2, 3))
+    conf = dict(window=8, sinks=3)
+    want, tol = ref.attention(q, k, v, do=do, **conf)
+    for x in (k, v):
+        x[:, :, 3], x[:, :, 40] = float('nan'), float('inf')
+    x = [t.requires_grad_() for t in (q, k, v)]
+    out = window_attention(*x, **conf)
+    got = [out, *torch.autograd.grad(out, x, do)]
+    for name, g, w, t in zip(('out', 'dq', 'dk', 'dv'), got, want, tol):
+        ref.check(name, g, w, t)
+
+
 def test_attention_differences():
     q, k, v = (t.double().requires_grad_() for t in _qkv(2, 4, 2, 5))
     ln = torch.tensor([5, 3], dtype=torch.int32)

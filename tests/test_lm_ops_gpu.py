@@ -151,6 +151,25 @@ def test_keys_that_no_row_sees_may_hold_anything(cuda, d, dtype):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize('dtype', sorted(DTYPES))
+@pytest.mark.parametrize('d', [16, 64, 128])
+def test_rows_of_padding_may_hold_anything(cuda, d, dtype):
+    dt = DTYPES[dtype]
+    q, k, v, do = (rand(cuda, 2, h, 130, d, seed=s, dtype=dt) for s, h in enumerate((4, 2, 2, 4)))
+    conf = dict(window=40, sinks=1, lengths=torch.tensor([130, 71], dtype=torch.int32, device=cuda),
+                q_start=0)
+    x = [t.requires_grad_() for t in (q, k, v)]
+    want = [window_attention(*x, **conf)]
+    want += torch.autograd.grad(want[0], x, do)
+    with torch.no_grad():
+        for t in (q, k, v, do):
+            t[1, :, 71:] = float('nan')
+    got = [window_attention(*x, **conf)]
+    got += torch.autograd.grad(got[0], x, do)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
 TOKEN = [
     # b, hq, hk, tq, tk, d, window, sinks, lengths
     (1, 2, 2, 1, 1, 64, 1, 0, None),
