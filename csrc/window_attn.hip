@@ -97,6 +97,14 @@ template <> struct Ops<float> {
   }
 };
 
+// fp16 holds numbers from 2^-14 on (2^-24 with one bit) and up to 2^16.
+// Probabilities are at most 1 and a long row has many small ones, so they are
+// rounded 2^kLift larger than they are, and the sums that they enter are
+// divided by it, a power of two, in 32 bits.  Forward: 2^7, the base of a
+// row's powers lies up to 2^8 below its maximum, so they end at 2^15.
+template <typename T> constexpr int kLift = 0;
+template <> constexpr int kLift<_Float16> = 7;
+
 // f(0), f(1) .. f(N - 1), each with its number as a constant
 template <typename F, int... I>
 __device__ __forceinline__ void each_of(F f, std::integer_sequence<int, I...>) {
@@ -594,9 +602,9 @@ __global__ void __launch_bounds__(64 * NW, (kRowFit<T, DP>)) fwd_kernel(AttnArgs
       // c > 0: the maximum of the products is the product of the maximum
       mx = halves_max(mx) * c;
       // The base of a row's powers may lie up to 2^8 below its maximum: sums
-      // and accumulators have the exponents for that (fp16 probabilities end
-      // at 2^16), the quotient at the end does not change, and most tiles of
-      // a row leave its accumulators alone.
+      // and accumulators have the exponents for that (fp16: kLift), the
+      // quotient at the end does not change, and most tiles of a row leave its
+      // accumulators alone.
       if (__any(mx > m + 8.f)) {
         const float mn = fmaxf(m, mx);
         const float alpha = ex2(m - (mn == -kInf ? 0.f : mn));
@@ -607,7 +615,7 @@ __global__ void __launch_bounds__(64 * NW, (kRowFit<T, DP>)) fwd_kernel(AttnArgs
 #pragma unroll
           for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
       }
-      const float base = m == -kInf ? 0.f : m;
+      const float base = (m == -kInf ? 0.f : m) - kLift<T>;
       float add = 0.f;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
@@ -628,7 +636,7 @@ __global__ void __launch_bounds__(64 * NW, (kRowFit<T, DP>)) fwd_kernel(AttnArgs
   sum = halves_sum(sum);
   const bool none = w.p < 0 || sum == 0.f;
   const float inv = none ? 0.f : 1.f / sum;
-  const float lse = none ? kInf : m + log2f(sum);
+  const float lse = none ? kInf : (m - kLift<T>) + log2f(sum);
   if (!w.live) return;
   if (SPLIT) {
     const int64_t row = ((int64_t)blockIdx.z * gridDim.x + w.bh) * (a.Tq * a.G) + w.r;

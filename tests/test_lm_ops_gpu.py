@@ -170,6 +170,24 @@ def test_rows_of_padding_may_hold_anything(cuda, d, dtype):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize('tq, hq', [(1, 1), (1, 300), (70, 1)])
+def test_fp16_rows_of_small_probabilities(cuda, tq, hq):
+    """4096 keys of 2^-20.6 each beside one of 1, which has no value: the
+    output is their sum.  Off by the rounding of the probabilities and of the
+    output, half a step of 2^-11 each, and of the scores in 32 bits."""
+    n, d = 4097, 64
+    q = torch.ones(1, 1, tq, d, dtype=torch.half, device=cuda)
+    k = torch.zeros(1, 1, n, d, dtype=torch.half, device=cuda)
+    k[:, :, 0] = 1.785
+    v = torch.ones_like(k)
+    v[:, :, 0] = 0.0
+    want = ref.attention(q, k, v, window=n)[0][0]
+    # many heads: one block goes over all keys of a row
+    out = window_attention(*(x.expand(1, hq, -1, d) for x in (q, k, v)), window=n)
+    err = ((out.cpu().double() - want).abs() / want).max()
+    assert float(err) <= 2.0 ** -10 + 2.0 ** -16, float(err)
+
+
 TOKEN = [
     # b, hq, hk, tq, tk, d, window, sinks, lengths
     (1, 2, 2, 1, 1, 64, 1, 0, None),
