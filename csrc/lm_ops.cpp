@@ -237,11 +237,16 @@ struct WindowAttnFn : public torch::autograd::Function<WindowAttnFn> {
       kfac::attn_bwd_plan(a, &a.sink_groups, &a.far_chunks, &floats);
       TORCH_CHECK((int64_t)(a.Tk + 63) / 64 + (int64_t)a.sink_groups * a.far_chunks <= 65535,
                   "window_attention: more than 65535 key blocks");
-      // the sinks' shares (16-byte aligned), then delta
-      const at::Tensor ws = at::empty({floats + lse.numel()}, lse.options());
+      a.bound_chunks = kfac::attn_bound_chunks(tag(q), a);
+      const int64_t rows = lse.numel(), bounds = (int64_t)a.B * a.Hkv * a.bound_chunks * 2;
+      // the sinks' shares (16-byte aligned), the bounds (8), delta, lse_keys
+      const at::Tensor ws =
+          at::empty({floats + bounds + (bounds > 0 ? 2 : 1) * rows}, lse.options());
       a.lse = lse.data_ptr<float>();
       a.kvpart = ws.data_ptr<float>();
-      a.delta = a.kvpart + floats;
+      a.bounds = a.kvpart + floats;
+      a.delta = a.bounds + bounds;
+      a.lse_keys = bounds > 0 ? a.delta + rows : nullptr;
       if (a.Tk == 0) dq.zero_();
       kfac::attn_backward(tag(q), a, stream());
       C10_HIP_KERNEL_LAUNCH_CHECK();

@@ -95,6 +95,11 @@ struct AttnArgs {
   uint32_t Gmagic;              // floor(2^32 / G)
   int sink_groups, far_chunks;  // backward: groups of sink keys, chunks of their far rows
   float* kvpart;                // their shares
+  // fp16 backward: of each chunk of a (sequence, key head) the largest |do|^2
+  // of its rows and |v|^2 of its keys; the rows' lse for the key gradients
+  int bound_chunks;
+  float* bounds;                // [B * Hkv, bound_chunks, 2]
+  float* lse_keys;              // like lse
 };
 
 // how a forward call is split over the keys, and the floats of its partial
@@ -102,6 +107,8 @@ struct AttnArgs {
 bool attn_keeps_rest(const AttnArgs& a);
 void attn_plan(const AttnArgs& a, int* splits, int64_t* floats);
 void attn_bwd_plan(const AttnArgs& a, int* sink_groups, int* far_chunks, int64_t* floats);
+// chunks of AttnArgs::bounds, 0: the type needs none
+int attn_bound_chunks(int dtype, const AttnArgs& a);
 void attn_forward(int dtype, const AttnArgs& a, hipStream_t st);
 void attn_backward(int dtype, const AttnArgs& a, hipStream_t st);
 

@@ -101,9 +101,15 @@ template <> struct Ops<float> {
 // Probabilities are at most 1 and a long row has many small ones, so they are
 // rounded 2^kLift larger than they are, and the sums that they enter are
 // divided by it, a power of two, in 32 bits.  Forward: 2^7, the base of a
-// row's powers lies up to 2^8 below its maximum, so they end at 2^15.
+// row's powers lies up to 2^8 below its maximum, so they end at 2^15.  Key
+// gradients, whose powers have the row's sum in their base: 2^15.  Their
+// products with dP - delta follow the upstream gradient's size and get a power
+// of two of their own (lift_of).
 template <typename T> constexpr int kLift = 0;
 template <> constexpr int kLift<_Float16> = 7;
+template <typename T> constexpr int kKeyLift = 0;
+template <> constexpr int kKeyLift<_Float16> = 15;
+template <typename T> constexpr bool kLifts = kLift<T> != 0;
 
 // f(0), f(1) .. f(N - 1), each with its number as a constant
 template <typename F, int... I>
@@ -233,8 +239,12 @@ __device__ __forceinline__ typename Ops<T>::frag col_frag(const T* L, const Lane
 
 // registers 8s .. 8s + 7 of an accumulator as a right operand, rounded once
 // to the operands' type (16-bit probabilities and their gradients are the
-// price of the matrix units; each is off by 2^-8 of itself at most, and
-// the sums over them stay in 32 bits)
+// price of the matrix units; each is off by half a step, 2^-8 of itself in
+// bf16 and 2^-11 in fp16, and the sums over them stay in 32 bits).  fp16's
+// stay clear of its subnormals and of its end: kLift.  What falls below 2^-14
+// there all the same is off by 2^-25, that is 2^-32 of a row's largest
+// probability (forward), 2^-40 (key gradients), and 2^-40 of what dP - delta
+// can be.
 template <typename T>
 __device__ __forceinline__ typename Ops<T>::frag acc_frag(const v16f& a, int s) {
   v8f f;
@@ -722,6 +732,123 @@ __global__ void __launch_bounds__(NT) join_kernel(AttnArgs a) {
     a.lse[row] = sum == 0.f ? kInf : base + log2f(sum);
 }
 
+__device__ __forceinline__ int clip(int64_t t, const AttnArgs& a) {
+  return (int)(t < 0 ? 0 : (t < a.Tq ? t : a.Tq));
+}
+
+// The rows that see a wave's 32 keys, as rows: first and behind the last
+// that see some of them, that see all of them, and that see this lane's.
+struct KeyRows {
+  int any0, any1, full0, full1, mine0, mine1;
+  __device__ __forceinline__ KeyRows(int j0, int key, const AttnArgs& a, const Seq& s) {
+    // row of the first token at position p or later
+    auto row = [&](int64_t p) { return clip(p - s.start, a) * a.G; };
+    const int64_t last = s.len, w = a.W;
+    any0 = row(j0);
+    any1 = row(j0 < a.S || j0 + 31 + w > last ? last : j0 + 31 + w);
+    full0 = row((int64_t)j0 + 31);
+    full1 = row(j0 + 31 < a.S || j0 + w > last ? last : j0 + w);
+    mine0 = row(key);
+    mine1 = row(key < a.S || key + w > last ? last : key + w);
+  }
+  __device__ __forceinline__ int coverage(int r0) const {
+    if (r0 + 32 <= any0 || r0 >= any1) return 0;
+    return r0 >= full0 && r0 + 32 <= full1 ? 2 : 1;
+  }
+  // some row sees this lane's key
+  __device__ __forceinline__ bool key_seen() const { return mine0 < mine1; }
+  // bit o is row r0 + 4h + o
+  __device__ __forceinline__ uint32_t seen(int r0, int h) const {
+    const int first = r0 + 4 * h;
+    return below(mine1 - first) & ~below(mine0 - first);
+  }
+};
+
+// fp16's products P (dP - delta) would pass 65504 under a large loss scale, and
+// lie among the subnormals, or below them, for small upstream gradients and
+// long windows: they are rounded 2^n larger than they are, n from the bound
+// |dP - delta| <= 2 |do| |v|, so that none reaches 2^15.  n of a row for dq,
+// whose sums are a row's own; of a (sequence, key head) for dk.
+__device__ __forceinline__ int lift_of(float do2, float v2) {
+  const float b = 4.f * do2 * v2;
+  // nothing to bound, or no bound: infinities are the caller's
+  if (!(b > 0.f && b < kInf)) return 0;
+  return 15 - ((__builtin_amdgcn_frexp_expf(b) + 1) >> 1);  // sqrt(b) < 2^that
+}
+
+__device__ __forceinline__ float power2(int n) { return __builtin_amdgcn_ldexpf(1.f, n); }
+
+// The largest |do|^2 and |v|^2 of a chunk of the rows and keys that take part:
+// blockIdx.y of a.bound_chunks.  One read of do and v, 16 lanes a row of them.
+// fp16, GPT-NeoX batch (8 x 2048 tokens, 12 heads of 64): 13 us of the pass's
+// 157, with the factors on dS 4 us each in dq and dk/dv; 140 us without all of
+// it, and then products under 2^-25 are lost and those over 65504 infinite.
+template <typename T>
+__global__ void __launch_bounds__(NT) bounds_kernel(AttnArgs a) {
+  constexpr int U = 8;  // rows in flight
+  __shared__ float red[2][NT / 64];
+  const int bh = blockIdx.x, b = bh / a.Hkv, hk = bh - b * a.Hkv;
+  const int d = ((int)threadIdx.x & 15) * 8, first = (int)threadIdx.x >> 4;
+  const Seq seq = sequence(a, b);
+  const int chunk = blockIdx.y;
+  float best[2];
+  auto largest = [&](int n, auto load) {
+    const int per = (n + a.bound_chunks - 1) / a.bound_chunks;
+    const int from = per * chunk < n ? per * chunk : n, to = from + per < n ? from + per : n;
+    float mx = 0.f;
+    for (int i = from + first; i < to; i += U * (NT / 16)) {
+      typename Ops<T>::frag f[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int at = i + u * (NT / 16);
+        f[u] = load(at < to ? at : i);
+      }
+      float s[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        s[u] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[u] += (float)f[u][e] * (float)f[u][e];
+      }
+#pragma unroll
+      for (int off = 8; off > 0; off >>= 1)
+#pragma unroll
+        for (int u = 0; u < U; ++u) s[u] += __shfl_xor(s[u], off, 64);
+      // leaves out a NaN, which is in the gradient anyway
+#pragma unroll
+      for (int u = 0; u < U; ++u) mx = fmaxf(mx, s[u]);
+    }
+    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+    return fmaxf(mx, __shfl_xor(mx, 32, 64));
+  };
+  best[0] = largest(a.Tq * a.G, [&](int i) {
+    const Row r(i, a);
+    const T* p = reinterpret_cast<const T*>(a.dout) + b * a.dos[0] + (hk * a.G + r.g) * a.dos[1] +
+                 r.t * a.dos[2];
+    return global_frag<T>(a.dout, p, d, a.D, position(r.t, seq) >= 0);
+  });
+  best[1] = largest(a.Tk, [&](int j) {
+    const T* p = reinterpret_cast<const T*>(a.v) + b * a.vs[0] + hk * a.vs[1] + j * a.vs[2];
+    return global_frag<T>(a.v, p, d, a.D, KeyRows(j, j, a, seq).key_seen());
+  });
+  if ((threadIdx.x & 63) == 0)
+    for (int i = 0; i < 2; ++i) red[i][threadIdx.x >> 6] = best[i];
+  __syncthreads();
+  if (threadIdx.x >= 2) return;
+  const float* x = red[threadIdx.x];
+  a.bounds[((int64_t)bh * a.bound_chunks + chunk) * 2 + threadIdx.x] =
+      fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+}
+
+// which: 0 the largest |do|^2 of a (sequence, key head), 1 |v|^2
+__device__ __forceinline__ float bound_of(const AttnArgs& a, int bh, int which) {
+  const int l = threadIdx.x & 63;
+  float x = l < a.bound_chunks ? a.bounds[((int64_t)bh * a.bound_chunks + l) * 2 + which] : 0.f;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) x = fmaxf(x, __shfl_xor(x, off, 64));
+  return x;
+}
+
 // The factor of the gradients to q and k.  Where a row sees itself alone its
 // probability is 1 whatever they are, and the gradient exactly 0: not the
 // difference of two sums that were taken in different orders.
@@ -773,6 +900,20 @@ __global__ void __launch_bounds__(64 * NW, (kRowFit<T, DP>)) dq_kernel(AttnArgs 
   const int64_t row = (int64_t)w.bh * (a.Tq * a.G) + w.r;
   if (w.live && h == 0) a.delta[row] = delta;
   const float lse = w.p >= 0 ? a.lse[row] : kInf;
+  // multiplied on, not put into the base of the powers: a power of two more on
+  // the upstream gradient is then one on dq, bit for bit
+  float more = 1.f, back = 1.f;
+  if constexpr (kLifts<T>) {
+    if (w.live && h == 0) a.lse_keys[row] = lse - kKeyLift<T>;
+    float do2 = 0.f;
+#pragma unroll
+    for (int k = 0; k < KD; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) do2 += (float)gf[k][i] * (float)gf[k][i];
+    const int lift = lift_of(halves_sum(do2), bound_of(a, w.bh, 1));
+    more = power2(lift);
+    back = power2(-lift);
+  }
 
   // dP - delta comes out of the matrix units: they start from -delta (in fp32
   // with heads over 32, whose registers are full, it is added afterwards)
@@ -800,7 +941,10 @@ __global__ void __launch_bounds__(64 * NW, (kRowFit<T, DP>)) dq_kernel(AttnArgs 
       }
       if (cover == 1) hide(s, w.seen(js, a));
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] = ex2(__builtin_fmaf(s[e], c, -lse)) * (kStart ? dp[e] : dp[e] + delta);
+      for (int e = 0; e < 16; ++e) {
+        const float x = ex2(__builtin_fmaf(s[e], c, -lse));
+        s[e] = (kLifts<T> ? x * more : x) * (kStart ? dp[e] : dp[e] + delta);
+      }
 #pragma unroll
       for (int ss = 0; ss < 2; ++ss) {
         const frag sf = acc_frag<T>(s, ss);
@@ -812,11 +956,7 @@ __global__ void __launch_bounds__(64 * NW, (kRowFit<T, DP>)) dq_kernel(AttnArgs 
   });
   if (!w.live) return;
   put<T, T, ND>(reinterpret_cast<T*>(a.dq) + w.b * a.dqs[0] + w.head * a.dqs[1] + w.t * a.dqs[2],
-                dq, score_factor(a), w.p < 0, a.D, h);
-}
-
-__device__ __forceinline__ int clip(int64_t t, const AttnArgs& a) {
-  return (int)(t < 0 ? 0 : (t < a.Tq ? t : a.Tq));
+                dq, score_factor(a) * back, w.p < 0, a.D, h);
 }
 
 // Rows that look at the keys [k0, k0 + BM): the near ones, whose window
@@ -868,7 +1008,7 @@ struct RowStream {
     q = reinterpret_cast<const T*>(a.q) + b * a.qs[0] + hk * a.G * a.qs[1];
     g = reinterpret_cast<const T*>(a.dout) + b * a.dos[0] + hk * a.G * a.dos[1];
     const int64_t at = ((int64_t)b * a.Hkv + hk) * (a.Tq * a.G);
-    lse = a.lse + at;
+    lse = (kLifts<T> ? a.lse_keys : a.lse) + at;
     delta = a.delta + at;
     repeats = BN % a.G == 0;
     if (repeats) offsets(a, 0, BN, qo, go);
@@ -914,34 +1054,6 @@ struct RowStream {
   }
 };
 
-// The rows that see a wave's 32 keys, as rows: first and behind the last
-// that see some of them, that see all of them, and that see this lane's.
-struct KeyRows {
-  int any0, any1, full0, full1, mine0, mine1;
-  __device__ __forceinline__ KeyRows(int j0, int key, const AttnArgs& a, const Seq& s) {
-    // row of the first token at position p or later
-    auto row = [&](int64_t p) { return clip(p - s.start, a) * a.G; };
-    const int64_t last = s.len, w = a.W;
-    any0 = row(j0);
-    any1 = row(j0 < a.S || j0 + 31 + w > last ? last : j0 + 31 + w);
-    full0 = row((int64_t)j0 + 31);
-    full1 = row(j0 + 31 < a.S || j0 + w > last ? last : j0 + w);
-    mine0 = row(key);
-    mine1 = row(key < a.S || key + w > last ? last : key + w);
-  }
-  __device__ __forceinline__ int coverage(int r0) const {
-    if (r0 + 32 <= any0 || r0 >= any1) return 0;
-    return r0 >= full0 && r0 + 32 <= full1 ? 2 : 1;
-  }
-  // some row sees this lane's key
-  __device__ __forceinline__ bool key_seen() const { return mine0 < mine1; }
-  // bit o is row r0 + 4h + o
-  __device__ __forceinline__ uint32_t seen(int r0, int h) const {
-    const int first = r0 + 4 * h;
-    return below(mine1 - first) & ~below(mine0 - first);
-  }
-};
-
 // dk and dv: a wave owns 32 keys.  S = Q K^T and dP = dO V^T have a row's
 // scores in register order, so dV^T += dO^T P and dK^T += Q^T dS take P and
 // dS from where they are.
@@ -953,12 +1065,23 @@ struct KeyGrad {
   frag kf[KD], vf[KD];
   v16f dk[ND], dv[ND];
   Lane<T, DP> at;
+  // Probabilities carry 2^kKeyLift (in lse), their products with dP - delta
+  // times `more` the power of two that suits them; k_back and v_back take both
+  // out of the sums again.
+  float more = 1.f, k_back = 1.f, v_back = 1.f;
 
   // A key that no row sees is taken for zeros, as the row kernels do: it may
   // hold anything, and 0 times that need not be 0.
   __device__ __forceinline__ void init(const AttnArgs& a, int b, int hk, int key,
                                        const KeyRows& kr) {
     const bool ok = kr.key_seen();
+    if constexpr (kLifts<T>) {
+      const int bh = b * a.Hkv + hk;
+      const int lift = __builtin_amdgcn_readfirstlane(lift_of(bound_of(a, bh, 0), bound_of(a, bh, 1)));
+      more = power2(lift - kKeyLift<T>);
+      k_back = power2(-lift);
+      v_back = power2(-kKeyLift<T>);
+    }
     const int h = (threadIdx.x & 63) >> 5;
     const T* kp = reinterpret_cast<const T*>(a.k) + b * a.ks[0] + hk * a.ks[1] + key * a.ks[2];
     const T* vp = reinterpret_cast<const T*>(a.v) + b * a.vs[0] + hk * a.vs[1] + key * a.vs[2];
@@ -1071,7 +1194,7 @@ struct KeyGrad {
             if constexpr (e < 16) {
               const float x = __builtin_fmaf(s[sub][e], c, -le[sub][e / 4][e % 4]);
               s[sub][e] = ex2(x);
-              dp[sub][e] *= s[sub][e];
+              dp[sub][e] *= kLifts<T> ? s[sub][e] * more : s[sub][e];
               if constexpr (e % 8 == 7) {
                 pf[sub][e / 8] = acc_frag<T>(s[sub], e / 8);
                 sf[sub][e / 8] = acc_frag<T>(dp[sub], e / 8);
@@ -1095,7 +1218,7 @@ struct KeyGrad {
       for (int i = 0; i < 4; ++i) {
         const int e = e4 * 4 + i;
         s[e] = ex2(__builtin_fmaf(s[e], c, -le[i]));
-        dp[e] *= s[e];
+        dp[e] *= kLifts<T> ? s[e] * more : s[e];
       }
     }
   }
@@ -1187,10 +1310,11 @@ dkv_kernel(AttnArgs a, int key_blocks) {
       const int kk = i / (DP / 4), d = i % (DP / 4) * 4;
       if (d >= a.D || j0 + kk >= a.S) continue;
       const v4f fk = *reinterpret_cast<const v4f*>(sk + kk * DP + d);
-      *reinterpret_cast<v4f*>(part + kk * a.D + d) =
-          v4f{fk[0] * a.scale, fk[1] * a.scale, fk[2] * a.scale, fk[3] * a.scale};
+      const v4f fv = *reinterpret_cast<const v4f*>(sv + kk * DP + d);
+      const float f = a.scale * kg.k_back, g = kg.v_back;
+      *reinterpret_cast<v4f*>(part + kk * a.D + d) = v4f{fk[0] * f, fk[1] * f, fk[2] * f, fk[3] * f};
       *reinterpret_cast<v4f*>(part + (kSinkKeys + kk) * a.D + d) =
-          *reinterpret_cast<const v4f*>(sv + kk * DP + d);
+          v4f{fv[0] * g, fv[1] * g, fv[2] * g, fv[3] * g};
     }
     return;
   }
@@ -1245,15 +1369,16 @@ dkv_kernel(AttnArgs a, int key_blocks) {
       }
     }
   }
+  const float f = score_factor(a) * kg.k_back;
   if (a.far_chunks > 0 && key < a.S) {
     float* part = sink_part(a, bh, key / kSinkKeys, 0) + key % kSinkKeys * a.D;
-    put<T, float, ND>(part, kg.dk, score_factor(a), false, a.D, h);
-    put<T, float, ND>(part + kSinkKeys * a.D, kg.dv, 1.f, false, a.D, h);
+    put<T, float, ND>(part, kg.dk, f, false, a.D, h);
+    put<T, float, ND>(part + kSinkKeys * a.D, kg.dv, kg.v_back, false, a.D, h);
   } else if (key < a.Tk) {
     put<T, T, ND>(reinterpret_cast<T*>(a.dk) + b * a.dks[0] + hk * a.dks[1] + key * a.dks[2],
-                  kg.dk, score_factor(a), false, a.D, h);
+                  kg.dk, f, false, a.D, h);
     put<T, T, ND>(reinterpret_cast<T*>(a.dv) + b * a.dvs[0] + hk * a.dvs[1] + key * a.dvs[2],
-                  kg.dv, 1.f, false, a.D, h);
+                  kg.dv, kg.v_back, false, a.D, h);
   }
 }
 
@@ -1381,11 +1506,23 @@ void attn_bwd_plan(const AttnArgs& a, int* sink_groups, int* far_chunks, int64_t
   *floats = bh * groups * (1 + ch) * 2 * kSinkKeys * a.D;
 }
 
+int attn_bound_chunks(int dtype, const AttnArgs& a) {
+  if (dtype != kF16) return 0;
+  // a wave reads them all at once
+  const int64_t most = std::max<int64_t>((int64_t)a.Tq * a.G, a.Tk);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(most, 256), 64));
+}
+
 void attn_backward(int dtype, const AttnArgs& a, hipStream_t st) {
   if ((int64_t)a.B * a.Hkv * a.Tk == 0 || a.Tq == 0) return;
-  if (dtype == kBF16) backward_type<__bf16>(a, st);
-  else if (dtype == kF16) backward_type<_Float16>(a, st);
-  else backward_type<float>(a, st);
+  if (dtype == kBF16) {
+    backward_type<__bf16>(a, st);
+  } else if (dtype == kF16) {
+    bounds_kernel<_Float16><<<dim3((unsigned)(a.B * a.Hkv), (unsigned)a.bound_chunks), NT, 0, st>>>(a);
+    backward_type<_Float16>(a, st);
+  } else {
+    backward_type<float>(a, st);
+  }
 }
 
 }  // namespace kfac

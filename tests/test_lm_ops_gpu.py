@@ -188,6 +188,98 @@ def test_fp16_rows_of_small_probabilities(cuda, tq, hq):
     assert float(err) <= 2.0 ** -10 + 2.0 ** -16, float(err)
 
 
+def _signs(dev, n, d):
+    """[1, 1, n, d] of rows +1, -1, +1, .."""
+    x = torch.where(torch.arange(n, device=dev) % 2 == 0, 1.0, -1.0).half()
+    return x[:, None].expand(n, d)[None, None].contiguous()
+
+
+def test_fp16_small_gradients_of_queries(cuda):
+    """4096 products P (dP - delta) of +-2^-26, below fp16, whose sum is not:
+    all numbers are powers of two and the answer exact."""
+    n, d = 4096, 64
+    q = torch.zeros(1, 1, 1, d, dtype=torch.half, device=cuda, requires_grad=True)
+    kv = _signs(cuda, n, d)
+    do = torch.full((1, 1, 1, d), 2.0 ** -20, dtype=torch.half, device=cuda)
+    (dq,) = torch.autograd.grad(window_attention(q, kv, kv, window=n), q, do)
+    assert bool((dq == 2.0 ** -17).all()), dq[0, 0, 0, :4]
+
+
+@pytest.mark.parametrize('d', [64, 128])
+def test_fp16_small_gradients_of_keys(cuda, d):
+    """512 rows of 4096 equally weighted keys each: products of +-2^-32 d."""
+    n, rows = 4096, 512
+    q = torch.ones(1, 1, rows, d, dtype=torch.half, device=cuda)
+    k = torch.ones(1, 1, n + rows, d, dtype=torch.half, device=cuda, requires_grad=True)
+    v = _signs(cuda, n + rows, d)
+    do = torch.full_like(q, 2.0 ** -20)
+    (dk,) = torch.autograd.grad(window_attention(q, k, v, window=n, scale=0.125), k, do)
+    # keys that all rows see; factor 1/8 on the sum
+    assert torch.equal(dk[:, :, rows:n], v[:, :, rows:n] * (d * 2.0 ** -26)), dk[0, 0, rows]
+
+
+def test_fp16_small_gradients_of_values(cuda):
+    """Keys of probability 2^-27 or less under large upstream gradients: off
+    by the rounding of the probabilities and of the result, 2^-11 each, and of
+    the scores (27 times a few 2^-24).  The last keys' results lie under 2^-14
+    (one row: 2^-17), where fp16 has a step of 2^-24 and half of it, 2^-25, is
+    no 2^-11 of the value."""
+    n, d = 1024, 64
+    q = torch.ones(1, 1, n, d, dtype=torch.half, device=cuda)
+    k = torch.zeros_like(q)
+    k[:, :, 0] = 2.34
+    v = torch.zeros_like(q).requires_grad_()
+    do = torch.full_like(q, 2.0 ** 10)
+    (dv,) = torch.autograd.grad(window_attention(q, k, v, window=n), v, do)
+    want = ref.attention(q, k, v, window=n, do=do)[0][3][0, 0, 1:]
+    ref.check('dv', dv[0, 0, 1:], want, (2.0 ** -10 + 2.0 ** -16) * want + 2.0 ** -25)
+
+
+def test_fp16_large_gradients(cuda):
+    """P (dP - delta) of 2^18, behind fp16's end, under gradients that are
+    not: powers of two once more."""
+    n, d = 70, 64
+    q = torch.zeros(1, 1, n, d, dtype=torch.half, device=cuda, requires_grad=True)
+    v = _signs(cuda, n, d)
+    k = (v / 64).requires_grad_()
+    do = torch.full_like(q, 2.0 ** 13)
+    dq, dk = torch.autograd.grad(window_attention(q, k, v, window=2), (q, k), do)
+    assert bool((dq[0, 0, 1:] == 2.0 ** 10).all()), dq[0, 0, :, 0]
+    assert not bool(dk.any())
+
+
+@pytest.mark.parametrize('d', [16, 64, 128])
+@pytest.mark.parametrize('factor', [2.0 ** -7, 2.0 ** 9])
+def test_fp16_gradients_follow_the_upstream_scale(cuda, factor, d):
+    """A power of two on the upstream gradient is one on every gradient, bit
+    for bit, as long as the results are normal numbers of fp16.  2^-14 itself
+    is left out: 2^-14 (1 - 2^-11) rounds up to it from below, where the step
+    is 2^-24, and is a number of its own at any other scale."""
+    q, k, v, do = (rand(cuda, 1, h, 700, d, seed=s).half() for s, h in enumerate((4, 2, 2, 4)))
+    do = torch.where(do.abs() < 2.0 ** -7, 0.0, do)
+    x = [t.requires_grad_() for t in (q, k, v)]
+    got = []
+    for f in (1.0, factor):
+        got.append(torch.autograd.grad(window_attention(*x, window=600, sinks=4), x, do * f))
+    for a, b in zip(*got):
+        a, b = a.float(), b.float()
+        keep = (a.abs() > 2.0 ** -14) & (b.abs() > 2.0 ** -14)
+        assert float(keep.float().mean()) > 0.5
+        assert torch.equal(a[keep] * factor, b[keep])
+
+
+def test_fp16_gradients_beside_an_infinite_one(cuda):
+    """An infinite upstream gradient reaches its own sequence and head."""
+    q, k, v, do = (rand(cuda, 2, 2, 90, 32, seed=s).half().requires_grad_() for s in range(4))
+    x, do = (q, k, v), do.detach()
+    want = torch.autograd.grad(window_attention(*x, window=20), x, do)
+    do[0, 1, 50, 3] = float('inf')
+    got = torch.autograd.grad(window_attention(*x, window=20), x, do)
+    for a, b in zip(got, want):
+        assert torch.equal(a[1], b[1]) and torch.equal(a[0, 0], b[0, 0])
+        assert not bool(a[0, 1].isfinite().all())
+
+
 TOKEN = [
     # b, hq, hk, tq, tk, d, window, sinks, lengths
     (1, 2, 2, 1, 1, 64, 1, 0, None),
