@@ -28,8 +28,10 @@ def save_checkpoint(
     preconditioner: Any,
     lr_scheduler: Any,
     filepath: str,
+    config: dict[str, Any] | None = None,
 ) -> None:
-    """Save the reference-format training checkpoint (rank 0 should call)."""
+    """Save the reference-format training checkpoint (rank 0 should call).
+    ``config``: plain values that the model is built from, kept beside it."""
     state = {
         'model': model.state_dict(),
         'optimizer': optimizer.state_dict(),
@@ -38,6 +40,8 @@ def save_checkpoint(
         ),
         'lr_scheduler': lr_scheduler.state_dict() if lr_scheduler is not None else None,
     }
+    if config is not None:
+        state['config'] = config
     d = os.path.dirname(filepath)
     if d:
         os.makedirs(d, exist_ok=True)

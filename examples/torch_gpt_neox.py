@@ -13,8 +13,9 @@ activations / gradients to one primary rank per MP group, preconditions the
 full matrices there and scatters the result back.  Synthetic token data.
 
 ``--attention-window`` / ``--attention-sinks`` train with a sliding window;
-``--teacher FILE`` (a checkpoint that ``--save`` wrote) adds distillation from
-the teacher's ``--distill-topk`` best logits to the loss:
+``--teacher FILE`` (a checkpoint that ``--save`` wrote, with the model's sizes
+and window) adds distillation from the teacher's ``--distill-topk`` best logits
+to the loss:
 
     python examples/torch_gpt_neox.py --steps 50 --save teacher.pt
     python examples/torch_gpt_neox.py --steps 50 --attention-window 256 \
@@ -98,6 +99,20 @@ def build_groups(topo: PipeModelDataParallelTopology, rank: int) -> tuple:
     return found['model'], found['data'], found['pipe']
 
 
+def load_teacher(path: str, vocab: int, fallback: dict[str, int],
+                 group: dist.ProcessGroup | None) -> GPTNeoX:
+    """The model of a ``--save`` checkpoint, built from the sizes and the window
+    kept in it (``fallback``: the sizes for a checkpoint without them, whose
+    model saw all tokens before each)."""
+    state = load_checkpoint(path, map_location='cpu')
+    config = state.get('config', fallback)
+    if config['vocab'] != vocab:
+        raise ValueError(f"the teacher's vocabulary is {config['vocab']}, the model's {vocab}")
+    teacher = GPTNeoX(**config, group=group).requires_grad_(False).eval()
+    teacher.load_state_dict(state['model'])
+    return teacher
+
+
 def main(argv: list[str] | None = None) -> dict[str, float]:
     args = parse_args(argv)
     cli.init_distributed(args)
@@ -113,20 +128,17 @@ def main(argv: list[str] | None = None) -> dict[str, float]:
     mp_group, dp_group, pipe_group = build_groups(topo, args.rank)
     cfg = MODELS[args.model]
     torch.manual_seed(args.seed)
-    shape = dict(vocab=cfg['vocab'], hidden=cfg['hidden'], layers=cfg['layers'],
-                 heads=cfg['heads'], group=mp_group)
+    sizes = {name: cfg[name] for name in ('vocab', 'hidden', 'layers', 'heads')}
     window = dict(attention_window=args.attention_window or None,
                   attention_sinks=args.attention_sinks)
     if args.pp > 1:
         # embedding, blocks and head as separate pipeline layers
-        layers = gpt_neox_pipeline_layers(**shape, **window)
+        layers = gpt_neox_pipeline_layers(**sizes, **window, group=mp_group)
     else:
-        layers = [lambda: GPTNeoX(**shape, **window)]
+        layers = [lambda: GPTNeoX(**sizes, **window, group=mp_group)]
     teacher, distill = None, None
     if args.teacher:
-        teacher = GPTNeoX(**shape).requires_grad_(False).eval()
-        teacher.load_state_dict(load_checkpoint(args.teacher, map_location='cpu')['model'])
-        teacher = teacher.to(args.device)
+        teacher = load_teacher(args.teacher, cfg['vocab'], sizes, mp_group).to(args.device)
         distill = TopKDistillLoss(args.distill_temperature, args.distill_weight)
     model = PipelineModule(layers, topo, rank=args.rank).to(args.device)
     if args.pp > 1:
@@ -196,7 +208,7 @@ def main(argv: list[str] | None = None) -> dict[str, float]:
         cli.log(args, f'factors saved under {args.factor_checkpoint_dir}')
     if args.save and args.rank == 0:
         net = model.module if dp > 1 else model
-        save_checkpoint(net.layers[0], optimizer, None, None, args.save)
+        save_checkpoint(net.layers[0], optimizer, None, None, args.save, config={**sizes, **window})
     return out
 
 

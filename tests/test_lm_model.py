@@ -122,6 +122,33 @@ def test_cli_window_and_teacher(tmp_path):
     assert all(line['loss'] == line['loss'] for line in lines)
 
 
+def test_cli_teacher_keeps_its_window(tmp_path):
+    """A teacher that was trained with a window is evaluated with it."""
+    from distributed_kfac_pytorch_amd.utils.training import load_checkpoint
+    from examples.torch_gpt_neox import MODELS
+    from examples.torch_gpt_neox import load_teacher
+
+    path = str(tmp_path / 'teacher.pt')
+    _run(['examples/torch_gpt_neox.py', '--steps', '1', '--seq-len', '16', '--micro-batch', '2',
+          '--attention-window', '5', '--attention-sinks', '1', '--save', path,
+          '--no-cuda', '--backend', 'gloo'])
+    sizes = {n: MODELS['tiny'][n] for n in ('vocab', 'hidden', 'layers', 'heads')}
+    teacher = load_teacher(path, sizes['vocab'], sizes, None)
+    state = load_checkpoint(path)
+    windowed, full = GPTNeoX(**sizes, attention_window=5, attention_sinks=1), GPTNeoX(**sizes)
+    for m in (windowed, full):
+        m.load_state_dict(state['model'])
+    tok = torch.randint(0, sizes['vocab'], (2, 16), generator=torch.Generator().manual_seed(1))
+    assert torch.equal(teacher(tok), windowed(tok))
+    assert not torch.equal(teacher(tok), full(tok))
+    # a checkpoint that says nothing: the model's sizes, all tokens seen
+    del state['config']
+    torch.save(state, path)
+    assert torch.equal(load_teacher(path, sizes['vocab'], sizes, None)(tok), full(tok))
+    with pytest.raises(ValueError, match='vocabulary'):
+        load_teacher(path, sizes['vocab'] + 1, sizes, None)
+
+
 def _grads(model, tok, teacher):
     logits = model(tok[:, :-1])
     best, index = teacher
