@@ -71,6 +71,14 @@ void once_only(const char* op) {
   TORCH_CHECK(!at::GradMode::is_enabled(), op, ": gradients of gradients are not supported");
 }
 
+// A tangent would be dropped without a word: the kernels have no forward-mode
+// derivative.
+void reverse_only(const char* op, std::initializer_list<const at::Tensor*> ts) {
+  for (const auto* t : ts)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), op,
+                ": forward-mode derivatives are not supported");
+}
+
 bool records(std::initializer_list<const at::Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return false;
   for (const auto* t : ts)
@@ -259,6 +267,7 @@ struct WindowAttnFn : public torch::autograd::Function<WindowAttnFn> {
 at::Tensor window_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                             const OptTensor& lengths, const OptTensor& starts, int64_t window,
                             int64_t sinks, int64_t start, bool start_given, double scale) {
+  reverse_only("window_attention", {&q, &k, &v});
   if (records({&q, &k, &v}))
     return WindowAttnFn::apply(q, k, v, lengths, starts, window, sinks, start, start_given, scale);
   const AttnConf c{window, sinks, start, start_given, scale};
@@ -362,6 +371,7 @@ struct RotaryFn : public torch::autograd::Function<RotaryFn> {
 std::tuple<at::Tensor, at::Tensor> rotary_axes(const at::Tensor& q, const at::Tensor& k,
                                                const at::Tensor& pos, const at::Tensor& table,
                                                bool halves) {
+  reverse_only("rotary_axes", {&q, &k});
   if (records({&q, &k})) {
     auto r = RotaryFn::apply(q, k, pos, table, halves);
     return {r[0], r[1]};
@@ -508,6 +518,7 @@ struct DistillFn : public torch::autograd::Function<DistillFn> {
 at::Tensor topk_distill_loss(const at::Tensor& z, const at::Tensor& teacher,
                              const at::Tensor& index, const OptTensor& rest, double temperature,
                              double weight, int64_t reduction) {
+  reverse_only("topk_distill_loss", {&z});
   if (records({&z}))
     return DistillFn::apply(z, teacher, index, rest, temperature, weight, reduction);
   return distill_run(z, teacher, index, rest, temperature, weight, reduction, false).loss;

@@ -115,6 +115,28 @@ def test_distill_refuses_operands(z, t, i, error):
         topk_distill_loss(z, t, i)
 
 
+def test_the_kernels_refuse_tangents():
+    """Before anything else, so this shows on the CPU too; the CPU's formulas
+    carry them."""
+    from distributed_kfac_pytorch_amd.ops import _native
+
+    q, z = rand(1, 1, 4, 8), rand(1, 2, 9)
+    pos, t, i = torch.arange(4)[:, None], rand(2, 2), torch.zeros(2, 2, dtype=torch.int64)
+    table = torch.zeros(4, 2, dtype=torch.float64)
+    with torch.autograd.forward_ad.dual_level():
+        dq, dz = (torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)) for x in (q, z))
+        lib = _native.native()
+        if lib is not None:
+            for call in (lambda: lib.window_attention(q, q, dq, None, None, 2, 0, 0, False, 1.0),
+                         lambda: lib.rotary_axes(dq, q, pos, table, False),
+                         lambda: lib.topk_distill_loss(dz, t, i, None, 1.0, 1.0, 2)):
+                with pytest.raises(RuntimeError, match='forward-mode'):
+                    call()
+        for out in (window_attention(q, q, dq, window=2), rotary_axes(dq, q, pos, sections=(4,))[0],
+                    topk_distill_loss(dz[0], t, i)):
+            assert torch.autograd.forward_ad.unpack_dual(out).tangent is not None
+
+
 # -------------------------------------------------------- against 64 bits
 @pytest.mark.parametrize('hq, hk, tq, tk, window, sinks, lengths, start', [
     (2, 2, 7, 7, 3, 0, None, None),

@@ -775,6 +775,20 @@ def test_gradients_of_gradients_are_refused(cuda):
             torch.autograd.grad(out, leaf, create_graph=True)
 
 
+def test_forward_mode_is_refused(cuda):
+    q, z = rand(cuda, 1, 1, 4, 8), rand(cuda, 2, 9)
+    pos = torch.arange(4, device=cuda)[:, None]
+    t, i, _ = _teacher(cuda, 2, 9, 2, 1.0, False, 1)
+    with torch.autograd.forward_ad.dual_level():
+        dq, dz = (torch.autograd.forward_ad.make_dual(x, x) for x in (q, z))
+        for call in (lambda: window_attention(dq, q, q, window=2),
+                     lambda: window_attention(q, q.clone().requires_grad_(), dq, window=2),
+                     lambda: rotary_axes(q, dq, pos, sections=(4,)),
+                     lambda: topk_distill_loss(dz, t, i)):
+            with pytest.raises(RuntimeError, match='forward-mode'):
+                call()
+
+
 def test_one_operand_learns(cuda):
     q, k, v = (rand(cuda, 1, 2, 40, 16, seed=s) for s in range(3))
     do = rand(cuda, 1, 2, 40, 16, seed=5)
