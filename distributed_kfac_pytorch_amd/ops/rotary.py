@@ -31,22 +31,39 @@ _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
 @functools.lru_cache(maxsize=64)
-def _table(sections: tuple[int, ...], base: float, ladder: str) -> torch.Tensor:
-    """fp64 [pairs, 2] on the CPU: frequency in turns per position, axis."""
+def _rows(sections: tuple[int, ...], base: float, ladder: str) -> tuple[tuple[float, float], ...]:
+    """(frequency in turns per position, axis) of each pair."""
     pairs = sum(sections)
     rows: list[tuple[float, float]] = []
     for a, n in enumerate(sections):
         for i in range(n):
             e = i / n if ladder == 'per_axis' else len(rows) / pairs
             rows.append((base ** -e / (2.0 * math.pi), float(a)))
-    return torch.tensor(rows, dtype=torch.float64, device='cpu')
+    return tuple(rows)
 
 
-def _reference(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor,
+_kept: dict[tuple[tuple[int, ...], float, str], torch.Tensor] = {}
+
+
+def _table(sections: tuple[int, ...], base: float, ladder: str) -> torch.Tensor:
+    """The rows as fp64 [pairs, 2] on the CPU.  Kept for the next call, unless
+    the tensor belongs to the mode that this call runs under (a fake one, one
+    of inference mode)."""
+    key = (sections, base, ladder)
+    table = _kept.get(key)
+    if table is None:
+        table = torch.tensor(_rows(*key), dtype=torch.float64, device='cpu')
+        if type(table) is torch.Tensor and not table.is_inference() and len(_kept) < 64:
+            _kept[key] = table
+    return table
+
+
+def _reference(x: torch.Tensor, positions: torch.Tensor, rows: tuple[tuple[float, float], ...],
                halves: bool) -> torch.Tensor:
-    n = table.shape[0]
+    n = len(rows)
+    table = torch.tensor(rows, dtype=torch.float64, device=x.device)
     pos = positions if positions.dim() == 3 else positions[None]
-    freq, axis = (table[:, 0] * (2.0 * math.pi)).to(x.device), table[:, 1].long().to(x.device)
+    freq, axis = table[:, 0] * (2.0 * math.pi), table[:, 1].long()
     ang = pos.double()[..., axis] * freq
     # a 64-bit input keeps its bits; the others are turned in 32
     work = torch.float64 if x.dtype == torch.float64 else torch.float32
@@ -114,9 +131,10 @@ def rotary_axes(
         raise ValueError(f'base must be positive, got {base}')
     if ladder not in ('shared', 'per_axis') or layout not in ('interleaved', 'halves'):
         raise ValueError(f'unknown ladder {ladder!r} or layout {layout!r}')
-    table = _table(sections, float(base), ladder)
+    base = float(base)
     if _nat.use_native(q, k):
         return _nat.native().rotary_axes(  # type: ignore[union-attr]
-            q, k, positions, table, layout == 'halves')
-    return (_reference(q, positions, table, layout == 'halves'),
-            _reference(k, positions, table, layout == 'halves'))
+            q, k, positions, _table(sections, base, ladder), layout == 'halves')
+    rows = _rows(sections, base, ladder)
+    return (_reference(q, positions, rows, layout == 'halves'),
+            _reference(k, positions, rows, layout == 'halves'))

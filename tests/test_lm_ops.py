@@ -211,6 +211,32 @@ def test_rotary_formula_and_differences(layout, ladder):
                                     (q.double().requires_grad_(), k.double().requires_grad_()))
 
 
+def test_rotary_keeps_no_tensor_of_another_mode():
+    """A call under a fake-tensor mode or inference mode leaves nothing behind
+    that a later call would trip over, and the other way round."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    from distributed_kfac_pytorch_amd.ops import rotary
+
+    def call(**kw):
+        q, pos = torch.ones(1, 2, 4, 24, **kw), torch.arange(4)[:, None]
+        return rotary_axes(q, q, pos, sections=(11,), base=77.0)[0]
+
+    key = ((11,), 77.0, 'shared')
+    with FakeTensorMode():
+        assert call().shape == (1, 2, 4, 24)
+        assert rotary._table(*key).shape == (11, 2)
+    with torch.inference_mode():
+        call()
+        rotary._table(*key)
+    call(requires_grad=True).sum().backward()
+    table = rotary._table(*key)
+    assert type(table) is torch.Tensor and not table.is_inference()
+    assert rotary._table(*key) is table
+    with FakeTensorMode():
+        call()
+
+
 def test_rotary_one_axis_is_the_models_rotation():
     from distributed_kfac_pytorch_amd.models.gpt_neox import _rotary
 
