@@ -46,14 +46,15 @@ _kept: dict[tuple[tuple[int, ...], float, str], torch.Tensor] = {}
 
 
 def _table(sections: tuple[int, ...], base: float, ladder: str) -> torch.Tensor:
-    """The rows as fp64 [pairs, 2] on the CPU.  Kept for the next call, unless
-    the tensor belongs to the mode that this call runs under (a fake one, one
-    of inference mode)."""
+    """The rows as fp64 [pairs, 2] on the CPU.  Kept for the next call: an
+    ordinary tensor under inference mode too, and not kept at all where the
+    call's own mode makes another one of it (a fake one)."""
     key = (sections, base, ladder)
     table = _kept.get(key)
     if table is None:
-        table = torch.tensor(_rows(*key), dtype=torch.float64, device='cpu')
-        if type(table) is torch.Tensor and not table.is_inference() and len(_kept) < 64:
+        with torch.inference_mode(False):
+            table = torch.tensor(_rows(*key), dtype=torch.float64, device='cpu')
+        if type(table) is torch.Tensor and len(_kept) < 64:
             _kept[key] = table
     return table
 
