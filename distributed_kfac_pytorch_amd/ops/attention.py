@@ -15,6 +15,7 @@ The backward pass sums in a fixed order: no atomics, bit-reproducible.
 """
 from __future__ import annotations
 
+import contextlib
 import math
 
 import torch
@@ -41,12 +42,15 @@ def _reference(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, s
     used, rows = see.any(dim=2)[..., None], see.any(dim=3)[..., None]
     kk = torch.where(used, k, 0.0).to(work).repeat_interleave(group, dim=1)
     vv = torch.where(used, v, 0.0).to(work).repeat_interleave(group, dim=1)
-    s = (torch.where(rows, q, 0.0).to(work) @ kk.transpose(-1, -2)) * scale
-    s = s.masked_fill(~see, float('-inf'))
-    m = s.detach().amax(dim=-1, keepdim=True) if tk else s.new_zeros(*s.shape[:-1], 1)
-    e = torch.exp(s - m.masked_fill(m == float('-inf'), 0.0))
-    total = e.sum(dim=-1, keepdim=True)
-    o = torch.where(rows, (e / total.masked_fill(total == 0.0, 1.0)) @ vv, 0.0)
+    # the products keep `work` under autocast, as the kernels' sums do
+    with (torch.autocast(q.device.type, enabled=False)
+          if torch.amp.is_autocast_available(q.device.type) else contextlib.nullcontext()):
+        s = (torch.where(rows, q, 0.0).to(work) @ kk.transpose(-1, -2)) * scale
+        s = s.masked_fill(~see, float('-inf'))
+        m = s.detach().amax(dim=-1, keepdim=True) if tk else s.new_zeros(*s.shape[:-1], 1)
+        e = torch.exp(s - m.masked_fill(m == float('-inf'), 0.0))
+        total = e.sum(dim=-1, keepdim=True)
+        o = torch.where(rows, (e / total.masked_fill(total == 0.0, 1.0)) @ vv, 0.0)
     return o.to(q.dtype).transpose(1, 2).contiguous().transpose(1, 2)
 
 

@@ -192,6 +192,27 @@ def test_keys_that_no_row_sees_may_hold_anything():
         ref.check(name, g, w, t)
 
 
+def test_autocast_changes_nothing():
+    q, k, v = _qkv(2, 4, 2, 9)
+    pos, (z, t, i, r) = torch.arange(9)[:, None], _distill_case(rest=True)
+
+    def call(*x):
+        turned = rotary_axes(*x[:2], pos, sections=(4,))
+        return (window_attention(*turned, x[2], window=4, sinks=1), *turned,
+                topk_distill_loss(x[3], t, i, teacher_rest=r))
+
+    x = [a.requires_grad_() for a in (q, k, v, z)]
+    want = call(*x)
+    with torch.autocast('cpu', dtype=torch.bfloat16):
+        got = call(*x)
+    for a, b in zip(got, want):
+        assert a.dtype == b.dtype and torch.equal(a, b)
+    for a, b in zip(*(torch.autograd.grad(sum(y.sum() for y in out), x) for out in (got, want))):
+        assert torch.equal(a, b)
+    q = torch.empty(1, 2, 4, 8, device='meta')        # a device without autocast
+    assert window_attention(q, q, q, window=2).shape == q.shape
+
+
 def test_attention_differences():
     q, k, v = (t.double().requires_grad_() for t in _qkv(2, 4, 2, 5))
     ln = torch.tensor([5, 3], dtype=torch.int32)
