@@ -16,7 +16,6 @@ The backward pass sums in a fixed order: no atomics, bit-reproducible.
 from __future__ import annotations
 
 import contextlib
-import math
 
 import torch
 
@@ -26,6 +25,7 @@ __all__ = ['window_attention']
 
 MAX_HEAD = 128
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+_SMALLEST = 2.0 ** -126  # fp32 holds numbers from here to 1 / here in full
 
 
 def _reference(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sinks: int,
@@ -81,7 +81,8 @@ def window_attention(
             the rows are a sequence's last ones, ``lengths - Tq`` -- new
             tokens behind a cache, or a full sequence.  A right-padded
             training batch passes ``lengths`` and ``q_start=0``.
-        scale: factor of the scores, positive; default ``D ** -0.5``.
+        scale: factor of the scores, from 2^-126 to 2^126; default
+            ``D ** -0.5``.
 
     Returns:
         ``[B, Hq, Tq, D]`` over memory laid out ``[B, Tq, Hq, D]``, which
@@ -106,8 +107,8 @@ def window_attention(
     if window < 1 or sinks < 0:
         raise ValueError(f'window must be at least 1 and sinks at least 0, got {window}, {sinks}')
     scale = d ** -0.5 if scale is None else float(scale)
-    if not (scale > 0.0 and math.isfinite(scale)):
-        raise ValueError(f'scale must be positive, got {scale}')
+    if not _SMALLEST <= scale <= 1.0 / _SMALLEST:
+        raise ValueError(f'scale must be positive, a normal number of 32 bits, got {scale}')
     for name, t in (('lengths', lengths), ('q_start', q_start)):
         if isinstance(t, torch.Tensor) and (
                 t.dtype != torch.int32 or tuple(t.shape) != (b,) or t.device != q.device):

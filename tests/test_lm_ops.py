@@ -50,6 +50,13 @@ def test_attention_refuses_shapes(shapes, error):
         window_attention(q, k, v, window=2)
 
 
+@pytest.mark.parametrize('scale', [1e-46, 2.0 ** -127, -1.0, 1e39, float('inf')])
+def test_attention_refuses_a_scale_that_32_bits_do_not_hold(scale):
+    q, k, v = _qkv()
+    with pytest.raises(ValueError, match='scale'):
+        window_attention(q, k, v, window=2, scale=scale)
+
+
 def test_attention_refuses_types():
     q, k, v = _qkv()
     with pytest.raises(TypeError):

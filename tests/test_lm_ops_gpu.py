@@ -280,6 +280,17 @@ def test_fp16_gradients_beside_an_infinite_one(cuda):
         assert not bool(a[0, 1].isfinite().all())
 
 
+@pytest.mark.parametrize('dtype', sorted(DTYPES))
+def test_attention_at_the_smallest_scale(cuda, dtype):
+    """Scores of 0: the mean over the keys that a row sees.  Off by half a
+    step of the output, and of the probabilities' type for each term."""
+    dt = DTYPES[dtype]
+    q, k, v = (rand(cuda, 1, 2, 100, 64, seed=s, dtype=dt) for s in range(3))
+    out = window_attention(q, k, v, window=30, scale=2.0 ** -126)
+    want, tol = ref.attention(q, k, v, window=30, scale=2.0 ** -126)
+    ref.check('out', out, want[0], tol[0])
+
+
 TOKEN = [
     # b, hq, hk, tq, tk, d, window, sinks, lengths
     (1, 2, 2, 1, 1, 64, 1, 0, None),
