@@ -20,8 +20,6 @@ form.
 """
 from __future__ import annotations
 
-import math
-
 import torch
 
 from distributed_kfac_pytorch_amd.ops import _native as _nat
@@ -32,6 +30,7 @@ MAX_ENTRIES = 1024
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 _REDUCTIONS = ('none', 'sum', 'mean')
 _INF = float('inf')
+_LARGEST = 2.0 ** 63
 
 
 def _reference(z: torch.Tensor, teacher: torch.Tensor, index: torch.Tensor,
@@ -94,8 +93,9 @@ def topk_distill_loss(
             and gradient NaN.
         teacher_rest: ``[...]``, log-sum-exp of the teacher's other logits
             divided by the temperature; constant.
-        temperature: positive; the loss carries its square.
-        weight: factor of the loss.  Give a known factor (a mixing weight, one
+        temperature: positive, from 2^-63 to 2^63 (its square is a number of
+            32 bits); the loss carries the square.
+        weight: factor of the loss, finite in 32 bits.  Give a known factor (a mixing weight, one
             over the accumulation steps) here rather than multiply the result:
             in bf16 and fp32 the forward already writes the gradient, and a
             factor put on later costs another pass over it.
@@ -128,11 +128,11 @@ def topk_distill_loss(
         if t is not None and t.device != logits.device:
             raise ValueError('logits and the teacher must be on one device')
     temperature = float(temperature)
-    if not (temperature > 0.0 and math.isfinite(temperature)):
-        raise ValueError(f'temperature must be positive, got {temperature}')
+    if not 1.0 / _LARGEST <= temperature <= _LARGEST:
+        raise ValueError(f'temperature must be positive, from 2^-63 to 2^63, got {temperature}')
     weight = float(weight)
-    if not math.isfinite(weight):
-        raise ValueError(f'weight must be finite, got {weight}')
+    if not abs(weight) <= torch.finfo(torch.float32).max:
+        raise ValueError(f'weight must be finite in 32 bits, got {weight}')
     if reduction not in _REDUCTIONS:
         raise ValueError(f'reduction must be one of {_REDUCTIONS}, got {reduction!r}')
     teacher_logits = teacher_logits.detach()

@@ -107,6 +107,14 @@ def test_distill_refuses_options(change, error):
         topk_distill_loss(rand(3, 9), rand(3, 2), torch.zeros(3, 2, dtype=torch.int64), **change)
 
 
+@pytest.mark.parametrize('change', [
+    dict(temperature=1e-39), dict(temperature=1e39), dict(temperature=1e20), dict(temperature=1e-20),
+    dict(temperature=-1.0), dict(weight=1e39), dict(weight=-float('inf'))])
+def test_distill_refuses_factors_that_32_bits_do_not_hold(change):
+    with pytest.raises(ValueError, match=next(iter(change))):
+        topk_distill_loss(rand(3, 9), rand(3, 2), torch.zeros(3, 2, dtype=torch.int64), **change)
+
+
 @pytest.mark.parametrize('z, t, i, error', [
     (rand(3, 9), rand(3, 2), torch.zeros(3, 3, dtype=torch.int64), ValueError),
     (rand(3, 9), rand(2, 2), torch.zeros(2, 2, dtype=torch.int64), ValueError),
