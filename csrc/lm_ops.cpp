@@ -37,6 +37,12 @@ bool aligned16(const at::Tensor& t) {
   return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
 }
 
+// contiguous and at a multiple of 16 bytes, a copy if need be
+at::Tensor packed16(const at::Tensor& t) {
+  const at::Tensor c = t.contiguous();
+  return aligned16(c) ? c : c.clone();
+}
+
 // rows that 16-byte accesses can read: unit last stride, every other stride
 // of a dimension with more than one element a multiple of 16 bytes
 bool rows16(const at::Tensor& t) {
@@ -470,12 +476,12 @@ struct DistillFn : public torch::autograd::Function<DistillFn> {
                             const at::Tensor& index, const OptTensor& rest, double temperature,
                             double weight, int64_t reduction) {
     auto o = distill_run(z, teacher, index, rest, temperature, weight, reduction, true);
+    // the gradient as well: saved-tensor hooks (offloading, checkpoints) see it
     ctx->save_for_backward({z, teacher, index, rest.has_value() ? *rest : at::Tensor(), o.info,
-                            o.mean});
+                            o.mean, o.dz});
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["weight"] = weight;
     ctx->saved_data["reduction"] = reduction;
-    if (o.dz.defined()) ctx->saved_data["dz"] = o.dz;
     return o.loss;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -485,13 +491,17 @@ struct DistillFn : public torch::autograd::Function<DistillFn> {
     c10::hip::HIPGuardMasqueradingAsCUDA g(z.device());
     const at::Tensor up = grads[0].to(at::kFloat).contiguous();
     at::Tensor dz, u;
-    auto kept = ctx->saved_data.find("dz");
-    if (kept != ctx->saved_data.end()) {
+    if (sv[6].defined() && ctx->saved_data.count("spent") == 0) {
       // the gradient that the forward wrote is given away and scaled in
       // place, so it serves one backward pass; another one of the same graph
-      // (retain_graph) computes its own below
-      dz = kept->second.toTensor();
-      ctx->saved_data.erase(kept);
+      // (retain_graph) computes its own below.  Whatever becomes of it, the
+      // saved tensor's version stays: that other pass still unpacks it.
+      ctx->saved_data["spent"] = true;
+      dz = sv[6].variable_data();
+      TORCH_CHECK(dz.sizes() == z.sizes() && dz.scalar_type() == z.scalar_type() &&
+                      dz.device() == z.device(),
+                  "topk_distill_loss: a saved-tensor hook changed the stored gradient");
+      dz = packed16(dz);  // a hook may hand it back otherwise
       if (dz.numel() > 0)
         kfac::distill_scale(tag(z), dz.data_ptr(), dz.numel(), up.data_ptr<float>(), stream());
       C10_HIP_KERNEL_LAUNCH_CHECK();
@@ -503,7 +513,9 @@ struct DistillFn : public torch::autograd::Function<DistillFn> {
                      ctx->saved_data["weight"].toDouble());
     const bool rows = ctx->saved_data["reduction"].toInt() == 0;
     dz = at::empty(z.sizes(), z.options());
-    a.info = reinterpret_cast<float4*>(sv[4].data_ptr<float>());
+    const at::Tensor info = packed16(sv[4]);
+    TORCH_CHECK(info.is_cuda() && info.numel() == a.N * 8, "topk_distill_loss: saved statistics");
+    a.info = reinterpret_cast<float4*>(info.data_ptr<float>());
     a.upstream = up.data_ptr<float>();
     a.upstream_rows = rows;
     a.mean = rows ? nullptr : sv[5].data_ptr<float>();

@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from distributed_kfac_pytorch_amd.ops.attention import window_attention
 from distributed_kfac_pytorch_amd.ops.distill import topk_distill_loss
@@ -544,6 +545,47 @@ def test_distill_rows_in_registers_alone(cuda):
     loss = topk_distill_loss(z, t, torch.full_like(i, -1), teacher_rest=r)
     (g,) = torch.autograd.grad(loss, z)
     assert float(loss.detach()) == 0.0 and bool((g == 0).all())
+
+
+def test_distill_stored_gradient_and_saved_tensor_hooks(cuda):
+    """The gradient that the forward wrote goes through the hooks: moved to the
+    host and back, to other strides and odd addresses, or made anew by a
+    checkpoint, the answer is the same, and a second backward pass works."""
+    n, v = 256, 1036
+    z = rand(cuda, n, v, seed=1).requires_grad_()
+    t, i, _ = _teacher(cuda, n, v, 3, 1.0, False, 1)
+    one = torch.ones((), device=cuda)
+    (want,) = torch.autograd.grad(topk_distill_loss(z, t, i), z, one)
+
+    def odd(x):
+        if x.dim() < 2:
+            return x.cuda()
+        y = torch.empty(x.numel() + 1, dtype=x.dtype, device=cuda)[1:].view(x.shape)
+        return y.copy_(x)
+
+    def strided(x):
+        return x.cuda().transpose(-1, -2).contiguous().transpose(-1, -2) if x.dim() > 2 else x.cuda()
+
+    for unpack in (torch.Tensor.cuda, odd):
+        seen = []
+        with torch.autograd.graph.saved_tensors_hooks(
+                lambda x: seen.append(tuple(x.shape)) or x.cpu(), unpack):
+            loss = topk_distill_loss(z, t, i)
+        assert seen.count((1, n, v)) == 2, seen
+        (first,) = torch.autograd.grad(loss, z, one, retain_graph=True)
+        assert torch.equal(first, want)
+        first.zero_()
+        (again,) = torch.autograd.grad(loss, z, one)
+        torch.testing.assert_close(again, want, rtol=2.0 ** -18, atol=0)
+    # only the stored gradient's strides: the logits' are an argument's
+    count = []
+    with torch.autograd.graph.saved_tensors_hooks(
+            lambda x: (len(count), count.append(1), x.cpu())[::2],
+            lambda p: strided(p[1]) if p[0] > 4 else p[1].cuda()):
+        loss = topk_distill_loss(z, t, i)
+    assert torch.equal(torch.autograd.grad(loss, z, one)[0], want)
+    loss = torch.utils.checkpoint.checkpoint(topk_distill_loss, z, t, i, use_reentrant=False)
+    assert torch.equal(torch.autograd.grad(loss, z, one)[0], want)
 
 
 @pytest.mark.parametrize('rest', [False, True])
