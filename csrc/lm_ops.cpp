@@ -224,7 +224,14 @@ struct WindowAttnFn : public torch::autograd::Function<WindowAttnFn> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once_only("window_attention");
     auto sv = ctx->get_saved_variables();
-    const at::Tensor &q = sv[0], &k = sv[1], &v = sv[2], &out = sv[3], &lse = sv[4], &rest = sv[5];
+    // saved-tensor hooks may hand tensors back with other strides: out and rest
+    // are read with the strides that the forward gave them
+    const int64_t G = groups(sv[0], sv[1]);
+    const at::Tensor q = operand(sv[0], G), k = operand(sv[1], 1), v = operand(sv[2], 1);
+    const at::Tensor out = packed16(sv[3].transpose(1, 2)), lse = packed16(sv[4]);
+    const at::Tensor rest = sv[5].defined() ? packed16(sv[5]) : sv[5];
+    for (const auto* t : {&out, &lse, &rest})
+      if (t->defined()) on_device(*t, q, "what the forward saved");
     const AttnConf c = unpack(ctx->saved_data["conf"].toDoubleVector());
     const OptTensor lengths = sv[6].defined() ? OptTensor(sv[6]) : c10::nullopt;
     const OptTensor starts = sv[7].defined() ? OptTensor(sv[7]) : c10::nullopt;
@@ -237,7 +244,7 @@ struct WindowAttnFn : public torch::autograd::Function<WindowAttnFn> {
       dv.zero_();
     } else {
       a.out = out.data_ptr();
-      strides3(out, a.os);
+      strides3(out.transpose(1, 2), a.os);
       a.rest = rest.defined() ? rest.data_ptr() : nullptr;
       a.dout = go.data_ptr();
       strides3(go, a.dos);

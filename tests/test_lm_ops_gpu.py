@@ -292,6 +292,25 @@ def test_attention_at_the_smallest_scale(cuda, dtype):
     ref.check('out', out, want[0], tol[0])
 
 
+@pytest.mark.parametrize('dtype', sorted(DTYPES))
+@pytest.mark.parametrize('window', [8, 200])
+def test_attention_with_offloaded_tensors(cuda, window, dtype):
+    """Saved-tensor hooks hand tensors back contiguous, whatever they were:
+    the output lies [B, T, H, D] in memory, the operands are slices."""
+    b, t, h, d = 2, 90, 3, 32
+    qkv = rand(cuda, b, t, h, 3 * d, seed=1, dtype=DTYPES[dtype]).requires_grad_()
+    do = rand(cuda, b, h, t, d, seed=2, dtype=DTYPES[dtype])
+
+    def call():
+        q, k, v = qkv.permute(0, 2, 1, 3).split(d, dim=-1)
+        return window_attention(q, k, v, window=window, sinks=2)
+
+    (want,) = torch.autograd.grad(call(), qkv, do)
+    with torch.autograd.graph.save_on_cpu(pin_memory=True):
+        out = call()
+    assert torch.equal(torch.autograd.grad(out, qkv, do)[0], want)
+
+
 TOKEN = [
     # b, hq, hk, tq, tk, d, window, sinks, lengths
     (1, 2, 2, 1, 1, 64, 1, 0, None),
