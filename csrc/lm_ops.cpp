@@ -494,7 +494,8 @@ struct DistillFn : public torch::autograd::Function<DistillFn> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once_only("topk_distill_loss");
     auto sv = ctx->get_saved_variables();
-    const at::Tensor& z = sv[0];
+    // saved-tensor hooks may hand tensors back with other strides
+    const at::Tensor z = unit_last(sv[0]);
     c10::hip::HIPGuardMasqueradingAsCUDA g(z.device());
     const at::Tensor up = grads[0].to(at::kFloat).contiguous();
     at::Tensor dz, u;
@@ -514,9 +515,10 @@ struct DistillFn : public torch::autograd::Function<DistillFn> {
       C10_HIP_KERNEL_LAUNCH_CHECK();
       return {dz, u, u, u, u, u, u};
     }
-    const OptTensor rest = sv[3].defined() ? OptTensor(sv[3]) : c10::nullopt;
+    const OptTensor rest = sv[3].defined() ? OptTensor(sv[3].contiguous()) : c10::nullopt;
+    const at::Tensor teacher = sv[1].contiguous(), index = sv[2].contiguous();
     kfac::DistillArgs a =
-        distill_args(z, sv[1], sv[2], rest, ctx->saved_data["temperature"].toDouble(),
+        distill_args(z, teacher, index, rest, ctx->saved_data["temperature"].toDouble(),
                      ctx->saved_data["weight"].toDouble());
     const bool rows = ctx->saved_data["reduction"].toInt() == 0;
     dz = at::empty(z.sizes(), z.options());

@@ -583,7 +583,7 @@ def test_distill_stored_gradient_and_saved_tensor_hooks(cuda):
         return y.copy_(x)
 
     def strided(x):
-        return x.cuda().transpose(-1, -2).contiguous().transpose(-1, -2) if x.dim() > 2 else x.cuda()
+        return x.cuda().transpose(-1, -2).contiguous().transpose(-1, -2) if x.dim() > 1 else x.cuda()
 
     for unpack in (torch.Tensor.cuda, odd):
         seen = []
@@ -594,15 +594,16 @@ def test_distill_stored_gradient_and_saved_tensor_hooks(cuda):
         (first,) = torch.autograd.grad(loss, z, one, retain_graph=True)
         assert torch.equal(first, want)
         first.zero_()
+        # formed anew from the logits: the same formula, its factors multiplied
+        # in another order, a few dozen roundings of 2^-24 at most
         (again,) = torch.autograd.grad(loss, z, one)
         torch.testing.assert_close(again, want, rtol=2.0 ** -18, atol=0)
-    # only the stored gradient's strides: the logits' are an argument's
-    count = []
-    with torch.autograd.graph.saved_tensors_hooks(
-            lambda x: (len(count), count.append(1), x.cpu())[::2],
-            lambda p: strided(p[1]) if p[0] > 4 else p[1].cuda()):
-        loss = topk_distill_loss(z, t, i)
-    assert torch.equal(torch.autograd.grad(loss, z, one)[0], want)
+    for reduction in ('mean', 'none'):            # the gradient stored, and not
+        up = one if reduction == 'mean' else torch.full((n,), 1.0 / n, device=cuda)
+        with torch.autograd.graph.saved_tensors_hooks(torch.Tensor.cpu, strided):
+            loss = topk_distill_loss(z, t, i, reduction=reduction)
+        (g,) = torch.autograd.grad(loss, z, up)
+        torch.testing.assert_close(g, want, rtol=2.0 ** -18, atol=0)
     loss = torch.utils.checkpoint.checkpoint(topk_distill_loss, z, t, i, use_reentrant=False)
     assert torch.equal(torch.autograd.grad(loss, z, one)[0], want)
 
