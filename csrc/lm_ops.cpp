@@ -54,22 +54,27 @@ bool rows16(const at::Tensor& t) {
   return true;
 }
 
+// batch, head, token of [B, H, T, D].  The stride of a single token may be
+// anything and a tile's rows behind it are still placed by it: a row's length
+// keeps them apart and aligned.
+void strides3(const at::Tensor& t, int64_t* s) {
+  s[0] = t.stride(0);
+  s[1] = t.stride(1);
+  s[2] = t.size(2) > 1 ? t.stride(2) : t.size(3);
+}
+
 // An attention operand [B, H, T, D]: rows that 16-byte accesses can read, a
 // token's row no longer than the stride to the next (an expanded one is
 // not), and 64 rows of `group` heads within 2^31 bytes of the first, which
 // is what the kernels' 32-bit offsets reach.  Else a copy laid out
 // [B, T, H, D].
 at::Tensor operand(const at::Tensor& t, int64_t group) {
-  const int64_t reach = ((group - 1) * t.stride(1) + 64 * t.stride(2)) * (int64_t)t.element_size();
+  int64_t s[3];
+  strides3(t, s);
+  const int64_t reach = ((group - 1) * s[1] + 64 * s[2]) * (int64_t)t.element_size();
   if (rows16(t) && (t.size(2) <= 1 || t.stride(2) >= t.size(3)) && reach < ((int64_t)1 << 31) - 1024)
     return t;
   return t.transpose(1, 2).clone(at::MemoryFormat::Contiguous).transpose(1, 2);
-}
-
-void strides3(const at::Tensor& t, int64_t* s) {  // batch, head, token of [B, H, T, D]
-  s[0] = t.stride(0);
-  s[1] = t.stride(1);
-  s[2] = t.stride(2);
 }
 
 void once_only(const char* op) {

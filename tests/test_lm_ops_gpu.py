@@ -311,6 +311,23 @@ def test_attention_with_offloaded_tensors(cuda, window, dtype):
     assert torch.equal(torch.autograd.grad(out, qkv, do)[0], want)
 
 
+@pytest.mark.parametrize('dtype', sorted(DTYPES))
+@pytest.mark.parametrize('hq, hk', [(2, 2), (6, 2)])
+def test_attention_to_a_single_key_of_any_stride(cuda, dtype, hq, hk):
+    """[B, H, D] made [B, H, 1, D] with a token stride of 1 or 0: it says
+    nothing, and nothing goes by it."""
+    dt, b, d = DTYPES[dtype], 3, 40
+    q, k, v, do = (rand(cuda, b, h, d, seed=s, dtype=dt) for s, h in enumerate((hq, hk, hk, hq)))
+    want, tol = ref.attention(*(x[:, :, None] for x in (q, k, v)), window=4, do=do[:, :, None])
+    for view in (lambda x: x.unsqueeze(-1).transpose(2, 3),
+                 lambda x: x.as_strided((*x.shape[:2], 1, d), (*x.stride()[:2], 0, 1))):
+        x = [view(t).requires_grad_() for t in (q, k, v)]
+        out = window_attention(*x, window=4)
+        for name, *y in zip(('out', 'dq', 'dk', 'dv'),
+                            (out, *torch.autograd.grad(out, x, view(do))), want, tol):
+            ref.check(name, *y)
+
+
 TOKEN = [
     # b, hq, hk, tq, tk, d, window, sinks, lengths
     (1, 2, 2, 1, 1, 64, 1, 0, None),
