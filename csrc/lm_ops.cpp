@@ -68,13 +68,17 @@ void strides3(const at::Tensor& t, int64_t* s) {
 // not), and 64 rows of `group` heads within 2^31 bytes of the first, which
 // is what the kernels' 32-bit offsets reach.  Else a copy laid out
 // [B, T, H, D].
-at::Tensor operand(const at::Tensor& t, int64_t group) {
+bool in_reach(const at::Tensor& t, int64_t group) {
   int64_t s[3];
   strides3(t, s);
-  const int64_t reach = ((group - 1) * s[1] + 64 * s[2]) * (int64_t)t.element_size();
-  if (rows16(t) && (t.size(2) <= 1 || t.stride(2) >= t.size(3)) && reach < ((int64_t)1 << 31) - 1024)
-    return t;
-  return t.transpose(1, 2).clone(at::MemoryFormat::Contiguous).transpose(1, 2);
+  return ((group - 1) * s[1] + 64 * s[2]) * (int64_t)t.element_size() < ((int64_t)1 << 31) - 1024;
+}
+at::Tensor operand(const at::Tensor& t, int64_t group) {
+  if (rows16(t) && (t.size(2) <= 1 || t.stride(2) >= t.size(3)) && in_reach(t, group)) return t;
+  const at::Tensor c = t.transpose(1, 2).clone(at::MemoryFormat::Contiguous).transpose(1, 2);
+  TORCH_CHECK(in_reach(c, group), "window_attention: too large: 64 tokens of ", t.size(1),
+              " heads pass 2^31 bytes");
+  return c;
 }
 
 void once_only(const char* op) {

@@ -853,6 +853,18 @@ def test_too_large_is_refused_on_the_host(cuda):
                           torch.zeros(1, 1, dtype=torch.int32, device=cuda).expand(2 ** 24, 1))
 
 
+def test_more_heads_than_offsets_reach_are_refused(cuda):
+    """64 tokens of 65536 heads of 128 in fp32 are 2^31 bytes."""
+    x = torch.zeros(1, 2, 65536, 128, device=cuda).transpose(1, 2)
+    for heads, fits in ((65536, False), (32768, True)):
+        y = x[:, :heads] if not fits else x[:, :heads].contiguous()
+        if fits:
+            assert not bool(window_attention(y, y, y, window=1).any())
+        else:
+            with pytest.raises(RuntimeError, match='too large'):
+                window_attention(y, y, y, window=1)
+
+
 def test_gradients_of_gradients_are_refused(cuda):
     q = rand(cuda, 1, 1, 4, 8).requires_grad_()
     z = rand(cuda, 2, 9).requires_grad_()
