@@ -247,6 +247,14 @@ struct WindowAttnFn : public torch::autograd::Function<WindowAttnFn> {
     c10::hip::HIPGuardMasqueradingAsCUDA g(q.device());
     kfac::AttnArgs a = attn_args(q, k, v, lengths, starts, c);
     const at::Tensor go = operand(grads[0], a.G);
+    int64_t floats = 0;
+    kfac::attn_bwd_plan(a, &a.sink_groups, &a.far_chunks, &floats);
+    TORCH_CHECK((int64_t)(a.Tk + 63) / 64 + (int64_t)a.sink_groups * a.far_chunks <= 65535,
+                "window_attention: more than 65535 key blocks");
+    // the sinks' shares are joined by a thread for 4 elements
+    TORCH_CHECK(a.far_chunks == 0 ||
+                    (int64_t)a.B * a.Hkv * a.S * (a.D / 2) < ((int64_t)1 << 32) - 256,
+                "window_attention: too large: sinks of all sequences and heads");
     at::Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v);
     if (a.Tq == 0 || q.numel() == 0) {
       dk.zero_();
@@ -263,10 +271,6 @@ struct WindowAttnFn : public torch::autograd::Function<WindowAttnFn> {
       strides3(dq, a.dqs);
       strides3(dk, a.dks);
       strides3(dv, a.dvs);
-      int64_t floats = 0;
-      kfac::attn_bwd_plan(a, &a.sink_groups, &a.far_chunks, &floats);
-      TORCH_CHECK((int64_t)(a.Tk + 63) / 64 + (int64_t)a.sink_groups * a.far_chunks <= 65535,
-                  "window_attention: more than 65535 key blocks");
       a.bound_chunks = kfac::attn_bound_chunks(tag(q), a);
       const int64_t rows = lse.numel(), bounds = (int64_t)a.B * a.Hkv * a.bound_chunks * 2;
       // the sinks' shares (16-byte aligned), the bounds (8), delta, lse_keys

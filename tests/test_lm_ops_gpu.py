@@ -865,6 +865,15 @@ def test_more_heads_than_offsets_reach_are_refused(cuda):
                 window_attention(y, y, y, window=1)
 
 
+def test_more_sinks_than_a_launch_joins_are_refused(cuda):
+    q, k = (torch.zeros(1, 1, t, 128, dtype=torch.bfloat16, device=cuda).requires_grad_()
+            for t in (520, 16385))
+    x = [y.expand(4096, -1, -1, -1) for y in (q, k, k)]
+    out = window_attention(*x, window=1, sinks=16384)
+    with pytest.raises(RuntimeError, match='too large'):
+        torch.autograd.grad(out, (q, k), torch.zeros_like(out))
+
+
 def test_gradients_of_gradients_are_refused(cuda):
     q = rand(cuda, 1, 1, 4, 8).requires_grad_()
     z = rand(cuda, 2, 9).requires_grad_()
