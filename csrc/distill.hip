@@ -82,10 +82,16 @@ __device__ __forceinline__ void store_wide(E* p, const float* f) {
 // would put the same 2^-24 m on every probability of the row.
 struct Run {
   float m, s;
+  // 2^(b - base) with b as it was rounded: contracted with the product that
+  // formed either, the difference of two equal numbers would be that rounding
+  __device__ __forceinline__ static float down(float b, float base) {
+#pragma clang fp contract(off)
+    return ex2(b - base);
+  }
   __device__ __forceinline__ void join(float m2, float s2) {
     const float mm = fmaxf(m, m2);
     const float base = mm == KFAC_NEG_INF ? 0.f : mm;
-    s = s * ex2(m - base) + s2 * ex2(m2 - base);
+    s = s * down(m, base) + s2 * down(m2, base);
     m = mm;
   }
   // 2^(x c), the product not rounded
@@ -285,7 +291,7 @@ __global__ void __launch_bounds__(NT) stats_kernel(DistillArgs a) {
       }
       raw = mx;
       const float m = mx * c, base = m == KFAC_NEG_INF ? 0.f : m;
-      float s = out.s * ex2(out.m - base);
+      float s = out.s * Run::down(out.m, base);
 #pragma unroll
       for (int q = 0; q < U; ++q)
 #pragma unroll
@@ -486,7 +492,7 @@ row_kernel(DistillArgs a) {
     }
     raw = mx;
     const float m = mx * c, base = m == KFAC_NEG_INF ? 0.f : m;
-    float s = out.s * ex2(out.m - base);
+    float s = out.s * Run::down(out.m, base);
 #pragma unroll
     for (int i = 0; i < N; ++i) s += ex2(__builtin_fmaf(y[i], c, -base));
     out.s = s;

@@ -690,6 +690,22 @@ def test_distill_bad_rows_stay_alone(cuda):
     assert bool((g[keep][:, :100] == 0).all())
 
 
+@pytest.mark.parametrize('dtype', sorted(DTYPES))
+@pytest.mark.parametrize('rest', [False, True])
+@pytest.mark.parametrize('n', [3, 256])
+def test_distill_rows_of_one_large_value(cuda, n, rest, dtype):
+    """A constant on a row's logits changes nothing: its columns are equal, and
+    so are their powers, whatever the base of them rounds to."""
+    t, i, r = _teacher(cuda, n, 40001, 20, 0.7, rest, 5)
+    z = torch.full((n, 40001), 60000.0, dtype=DTYPES[dtype], device=cuda)
+    z *= torch.where(torch.arange(n, device=cuda) % 2 == 0, 1.0, -1.0).to(z.dtype)[:, None]
+    z.requires_grad_()
+    want = ref.distill(torch.zeros_like(z), t, i, rest=r, temperature=0.7)
+    loss = topk_distill_loss(z, t, i, teacher_rest=r, temperature=0.7)
+    ref.check('loss', loss, *want[:2])
+    ref.check('dz', *torch.autograd.grad(loss, z), *want[2:])
+
+
 # ------------------------------------------------------------ in use
 def _chain(x, conf):
     """The operators as a decoder's step runs them: qkv and logits from
