@@ -39,14 +39,17 @@ def _reference(z: torch.Tensor, teacher: torch.Tensor, index: torch.Tensor,
     there = index >= 0
     outside = (index >= z.shape[-1]).any(dim=-1)
     idx = torch.where(there & (index < z.shape[-1]), index, 0).long()
-    t = (teacher.to(work) / tau).masked_fill(~there, -_INF)
+    # the type's lowest value over a temperature under 1 is a number of 64 bits
+    t = (teacher.double() / tau).masked_fill(~there, -_INF)
     if rest is not None:
-        t = torch.cat([t, rest.to(work)[..., None]], dim=-1)
-    norm = torch.logsumexp(t, dim=-1, keepdim=True)
-    counts = there.any(dim=-1) & (norm[..., 0] != -_INF)
-    logp = t - norm.masked_fill(~counts[..., None], 0.0)
+        t = torch.cat([t, rest.double()[..., None]], dim=-1)
+    counts = there.any(dim=-1) & (t != -_INF).any(dim=-1)
+    logp = torch.log_softmax(torch.where(counts[..., None], t, 0.0), dim=-1).to(work)
     p = torch.exp(logp)
-    logq = torch.log_softmax(z.to(work) / tau, dim=-1)
+    # a row that does not count may hold anything
+    u = torch.where(counts[..., None], z, 0.0).to(work)
+    top = u.detach().amax(dim=-1, keepdim=True)
+    logq = torch.log_softmax((u - torch.where(top.isfinite(), top, 0.0)) / tau, dim=-1)
     k = index.shape[-1]
     weighs = there & (p[..., :k] != 0.0) & counts[..., None]
     diff = torch.where(weighs, logp[..., :k], 0.0) - torch.where(weighs, logq.gather(-1, idx), 0.0)

@@ -289,6 +289,27 @@ def _distill_case(n=4, v=23, k=5, seed=0, rest=False, tau=1.0, dtype=torch.float
     return z.to(dtype), t, i, r
 
 
+def lowest_case(dtype, tau, rest, v=40, k=5):
+    """Rows that are masked with the type's lowest value: some of the student's
+    logits, all of them, some of the teacher's entries, all of them.  The
+    answers are those of a row in which nothing is masked where only the mask
+    is left, and of no probability (2^-288 for the student, which has no place
+    in any type) in the mask's place where something is."""
+    low = torch.finfo(dtype).min
+    z, t, i, r = _distill_case(n=5, v=v, k=k, rest=rest, tau=tau, dtype=dtype)
+    clean_z, clean_t = z.clone(), t.clone()
+    spare = [c for c in range(v) if c not in i[1].tolist()][:9]  # none of the teacher's
+    z[1, spare], clean_z[1, spare] = low, -200.0 * tau
+    z[2], clean_z[2] = low, 0.0
+    t[3, 2:], clean_t[3, 2:] = torch.finfo(torch.float32).min, float('-inf')
+    t[4], clean_t[4] = torch.finfo(torch.float32).min, 0.0
+    if rest:
+        r[4] = float('-inf')     # nothing beside the masked entries
+    want = ref.distill(clean_z, clean_t, i, rest=r, temperature=tau, reduction='none')
+    assert all(bool(x.isfinite().all()) for x in want)
+    return z, t, i, r, want
+
+
 @pytest.mark.parametrize('rest', [False, True])
 @pytest.mark.parametrize('reduction', ['mean', 'sum', 'none'])
 @pytest.mark.parametrize('k, twist', [(1, ''), (5, ''), (5, 'padded'), (5, 'twice'), (23, ''),
@@ -322,6 +343,27 @@ def test_distill_differences_and_dense_limit():
     dense = torch.nn.functional.kl_div(torch.log_softmax(z, -1), torch.softmax(t, -1),
                                        reduction='batchmean')
     torch.testing.assert_close(got, dense)
+
+
+@pytest.mark.parametrize('rest', [False, True])
+@pytest.mark.parametrize('tau', [0.5, 1.0, 3.0])
+def test_distill_lowest_values(tau, rest):
+    z, t, i, r, want = lowest_case(torch.float32, tau, rest)
+    z.requires_grad_()
+    loss = topk_distill_loss(z, t, i, teacher_rest=r, temperature=tau, reduction='none')
+    ref.check('loss', loss, *want[:2])
+    ref.check('dz', *torch.autograd.grad(loss, z, torch.ones_like(loss)), *want[2:])
+
+
+def test_distill_rows_of_padding_may_hold_anything():
+    z, t, i, _ = _distill_case()
+    i[1:3] = -1
+    want = ref.distill(z, t, i)
+    z[1], z[2, 3] = float('-inf'), float('nan')
+    z.requires_grad_()
+    loss = topk_distill_loss(z, t, i)
+    ref.check('loss', loss, *want[:2])
+    ref.check('dz', *torch.autograd.grad(loss, z), *want[2:])
 
 
 def test_distill_index_behind_the_vocabulary_is_nan():
