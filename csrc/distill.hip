@@ -122,6 +122,22 @@ __device__ __forceinline__ Run wave_join(Run r) {
   return r;
 }
 
+// The floor of finite logits, for the lowest value of bf16 or fp32 that a row
+// may be masked with: its product with c passes the end of fp32 or has no
+// digits left to cancel.  -2^30 over c, or 2^24 where that is more, rounded to
+// a power of two, so that its own product with c is exact.  Beside a logit
+// above it everything at it has probability 0; a row with none above it
+// ("floored") is uniform over its finite logits.  That takes no operation of
+// the loops over a row: their bases are kept at the floor or above, and a row
+// whose base is the floor is counted once more.
+__device__ __forceinline__ float floor_of(float c) {
+  const int e = 30 - __builtin_amdgcn_frexp_expf(c);
+  return -__builtin_amdgcn_ldexpf(1.f, e > 24 ? e : 24);
+}
+__device__ __forceinline__ float floored(float x, float low) {
+  return x == KFAC_NEG_INF ? x : fmaxf(x, low) + (x - x);  // NaN stays
+}
+
 __device__ __forceinline__ int64_t index_at(const DistillArgs& a, int64_t i) {
   return a.index64 ? reinterpret_cast<const int64_t*>(a.index)[i]
                    : (int64_t)reinterpret_cast<const int32_t*>(a.index)[i];
@@ -130,6 +146,11 @@ __device__ __forceinline__ int64_t index_at(const DistillArgs& a, int64_t i) {
 template <typename E>
 __device__ __forceinline__ const E* row_of(const DistillArgs& a, int64_t n) {
   return reinterpret_cast<const E*>(a.z) + (n / a.inner) * a.zs0 + (n % a.inner) * a.zs1;
+}
+
+// nothing above the floor, and no NaN
+__device__ __forceinline__ bool is_floored(const Run& all, float low, float c) {
+  return all.m <= low * c && all.s == all.s;
 }
 
 // A row's statistics, as the backward pass finds them.
@@ -150,12 +171,18 @@ __device__ __forceinline__ void store_info(const DistillArgs& a, int64_t n, cons
   a.info[2 * n + 1] = make_float4(i.teacher.m, i.teacher.s, i.r, i.unused);
 }
 
+// the log-sum of the teacher's other logits
+__device__ __forceinline__ float rest_of(const DistillArgs& a, int64_t n) {
+  return a.rest != nullptr ? floored(a.rest[n], floor_of(kLog2e)) : KFAC_NEG_INF;
+}
+
 // The teacher's part of a row's info, by one wave.  An index behind the
 // vocabulary makes the teacher's sum NaN, and with it the loss and gradient.
 __device__ __forceinline__ void teacher_of(const DistillArgs& a, int64_t n, RowInfo& info) {
   const int lane = threadIdx.x & 63;
   const float c = kLog2e / a.temperature;
-  const float rest = a.rest != nullptr ? a.rest[n] : KFAC_NEG_INF;
+  const float low = floor_of(c);
+  const float rest = rest_of(a, n);
   Run t{KFAC_NEG_INF, 0.f};
   bool some = false, far = false;
   for (int k = lane; k < a.K; k += 64) {
@@ -163,7 +190,7 @@ __device__ __forceinline__ void teacher_of(const DistillArgs& a, int64_t n, RowI
     if (j < 0) continue;
     some = true;
     far |= j >= a.V;
-    t.add(a.teacher[n * a.K + k], c);
+    t.add(floored(a.teacher[n * a.K + k], low), c);
   }
   t = wave_join(t);
   t.add(rest, kLog2e);
@@ -180,18 +207,19 @@ __device__ __forceinline__ void teacher_of(const DistillArgs& a, int64_t n, RowI
 template <typename F>
 __device__ __forceinline__ float row_loss(const DistillArgs& a, int64_t n, const RowInfo& i,
                                           F raw) {
-  const float c = kLog2e / a.temperature;
+  const float c = kLog2e / a.temperature, low = floor_of(c);
   float loss = 0.f;
   for (int k = threadIdx.x & 63; k < a.K; k += 64) {
     const int64_t j = index_at(a, n * a.K + k);
     if (j < 0 || j >= a.V) continue;
-    const float tl = a.teacher[n * a.K + k];
+    const float tl = floored(a.teacher[n * a.K + k], low);
     const float p = i.teacher.part(tl, c);
-    if (p > 0.f) loss += p * (i.teacher.log2part(tl, c) - i.all.log2part(raw(k, j), c));
+    if (p > 0.f)
+      loss += p * (i.teacher.log2part(tl, c) - i.all.log2part(floored(raw(k, j), low), c));
   }
   loss = wave_reduce_sum(loss);
   if (i.r > 0.f)
-    loss += i.r * (i.teacher.log2part(a.rest[n], kLog2e) -
+    loss += i.r * (i.teacher.log2part(rest_of(a, n), kLog2e) -
                    ((i.tail.m - i.all.m) + (log2f(i.tail.s) - log2f(i.all.s))));
   // p = 0 terms drop out, but not what makes the row undefined
   if (i.all.s != i.all.s || i.all.s == 0.f || i.teacher.s != i.teacher.s) loss = __builtin_nanf("");
@@ -210,7 +238,7 @@ __device__ void finish_row(const DistillArgs& a, int64_t n, const Run& all, cons
   }
 }
 
-// The gradient of the columns outside I is f 2^(x c - base).
+// The gradient of the columns outside I is f power(x).
 struct Outside {
   float base, f;
   __device__ __forceinline__ Outside(const RowInfo& i, float g, bool rest) {
@@ -224,6 +252,11 @@ struct Outside {
     }
     if (i.teacher.s != i.teacher.s) f = i.teacher.s;
   }
+  __device__ __forceinline__ float power(float x, float c) const {
+    return ex2(__builtin_fmaf(x, c, -base));
+  }
+  // of a floored row: uniform over its finite logits
+  __device__ __forceinline__ float flat(float x) const { return x > KFAC_NEG_INF ? 1.f : 0.f; }
 };
 
 // Statistics of a slice of a row: part = {tail m, s, member m, s}.
@@ -254,8 +287,9 @@ __global__ void __launch_bounds__(NT) stats_kernel(DistillArgs a) {
   }
   some = __syncthreads_or(some);
 
+  const float low = floor_of(c);
   Run out{KFAC_NEG_INF, 0.f}, in{KFAC_NEG_INF, 0.f};
-  float raw = KFAC_NEG_INF;  // largest logit so far
+  float raw = low;  // largest logit so far, the floor at least
   if (some) {
     const int64_t nv = (c1 - c0) / N;
     for (int64_t v0 = tid; v0 < nv; v0 += (int64_t)NT * U) {
@@ -281,7 +315,7 @@ __global__ void __launch_bounds__(NT) stats_kernel(DistillArgs a) {
 #pragma unroll
             for (int i = 0; i < N; ++i)
               if ((b >> i) & 1u) {
-                in.add(y[q][i], c);
+                in.add(floored(y[q][i], low), c);
                 y[q][i] = KFAC_NEG_INF;
               }
           }
@@ -290,12 +324,12 @@ __global__ void __launch_bounds__(NT) stats_kernel(DistillArgs a) {
         for (int i = 0; i < N; ++i) mx = fmaxf(mx, y[q][i]);
       }
       raw = mx;
-      const float m = mx * c, base = m == KFAC_NEG_INF ? 0.f : m;
-      float s = out.s * Run::down(out.m, base);
+      const float m = mx * c;
+      float s = out.s * Run::down(out.m, m);
 #pragma unroll
       for (int q = 0; q < U; ++q)
 #pragma unroll
-        for (int i = 0; i < N; ++i) s += ex2(__builtin_fmaf(y[q][i], c, -base));
+        for (int i = 0; i < N; ++i) s += ex2(__builtin_fmaf(y[q][i], c, -m));
       out.s = s;
       out.m = m;
     }
@@ -303,14 +337,13 @@ __global__ void __launch_bounds__(NT) stats_kernel(DistillArgs a) {
     if (rem < c1) {
       const int at = (int)(rem - c0);
       const bool member = REST && ((bits[at >> 5] >> (at & 31)) & 1u);
-      (member ? in : out).add(up<E>(z[rem]), c);
+      (member ? in : out).add(floored(up<E>(z[rem]), low), c);
     }
   }
   out = wave_join(out);
   if (REST) in = wave_join(in);
   if ((tid & 63) == 0) red[tid >> 6] = make_float4(out.m, out.s, in.m, in.s);
   __syncthreads();
-  if (tid >= 64) return;
   out = Run{red[0].x, red[0].y};
   in = Run{red[0].z, red[0].w};
 #pragma unroll
@@ -318,6 +351,20 @@ __global__ void __launch_bounds__(NT) stats_kernel(DistillArgs a) {
     out.join(red[w].x, red[w].y);
     in.join(red[w].z, red[w].w);
   }
+  if (some && is_floored(joined(out, in), low, c)) {
+    float count = 0.f;
+    for (int64_t i = c0 + tid; i < c1; i += NT) {
+      const bool member = REST && ((bits[(i - c0) >> 5] >> ((i - c0) & 31)) & 1u);
+      count += !member && up<E>(z[i]) > KFAC_NEG_INF ? 1.f : 0.f;
+    }
+    count = wave_reduce_sum(count);
+    __syncthreads();
+    if ((tid & 63) == 0) red[tid >> 6].x = count;
+    __syncthreads();
+    out = Run{low * c, 0.f};
+    for (int w = 0; w < NT / 64; ++w) out.s += red[w].x;
+  }
+  if (tid >= 64) return;
   if (a.splits > 1) {
     if (tid == 0) a.part[blockIdx.x] = make_float4(out.m, out.s, in.m, in.s);
     return;
@@ -446,7 +493,7 @@ row_kernel(DistillArgs a) {
     const int64_t j = index_at(a, n * a.K + k);
     const bool in = j >= 0 && j < V;
     at[k] = in ? (int)j : -1;
-    pk[k] = in ? info.teacher.part(a.teacher[n * a.K + k], c) : 0.f;
+    pk[k] = in ? info.teacher.part(floored(a.teacher[n * a.K + k], floor_of(c)), c) : 0.f;
     xk[k] = in ? up<E>(z[j]) : 0.f;
     if (REST && in) atomicOr(&bits[j >> 5], 1u << (j & 31));
   }
@@ -467,8 +514,9 @@ row_kernel(DistillArgs a) {
       if (k < a.K && part == 0) pj[k] = p;
     }
   }
+  const float low = floor_of(c);
   Run out{KFAC_NEG_INF, 0.f}, in{KFAC_NEG_INF, 0.f};
-  float raw = KFAC_NEG_INF;  // largest logit so far
+  float raw = low;  // largest logit so far, the floor at least
 #pragma unroll
   for (int q = 0; q < VPT; ++q) {
     if (REST) {
@@ -478,7 +526,7 @@ row_kernel(DistillArgs a) {
 #pragma unroll
         for (int i = 0; i < N; ++i)
           if ((b >> i) & 1u) {
-            in.add(up<E>(x[q][i]), c);
+            in.add(floored(up<E>(x[q][i]), low), c);
             x[q][i] = (E)KFAC_NEG_INF;
           }
       }
@@ -491,16 +539,16 @@ row_kernel(DistillArgs a) {
       mx = fmaxf(mx, y[i]);
     }
     raw = mx;
-    const float m = mx * c, base = m == KFAC_NEG_INF ? 0.f : m;
-    float s = out.s * Run::down(out.m, base);
+    const float m = mx * c;
+    float s = out.s * Run::down(out.m, m);
 #pragma unroll
-    for (int i = 0; i < N; ++i) s += ex2(__builtin_fmaf(y[i], c, -base));
+    for (int i = 0; i < N; ++i) s += ex2(__builtin_fmaf(y[i], c, -m));
     out.s = s;
     out.m = m;
   }
   if (rem < V) {
     const bool member = REST && ((bits[rem >> 5] >> (rem & 31)) & 1u);
-    (member ? in : out).add(last, c);
+    (member ? in : out).add(floored(last, low), c);
   }
   out = wave_join(out);
   if (REST) in = wave_join(in);
@@ -513,22 +561,41 @@ row_kernel(DistillArgs a) {
     out.join(red[w].x, red[w].y);
     if (REST) in.join(red[w].z, red[w].w);
   }
-  info.tail = out;
   info.all = REST ? joined(out, in) : out;
+  const bool flat = is_floored(info.all, low, c);
+  if (flat) {
+    float count = 0.f;
+    for (int i = tid; i < V; i += kRowThreads) {
+      const bool member = REST && ((bits[i >> 5] >> (i & 31)) & 1u);
+      count += !member && up<E>(z[i]) > KFAC_NEG_INF ? 1.f : 0.f;
+    }
+    count = wave_reduce_sum(count);
+    __syncthreads();
+    if ((tid & 63) == 0) red[tid >> 6].x = count;
+    __syncthreads();
+    out = Run{low * c, 0.f};
+    for (int w = 0; w < kRowThreads / 64; ++w) out.s += red[w].x;
+    info.all = REST ? joined(out, in) : out;
+  }
+  info.tail = out;
   const float g = a.temperature * a.mean[0];
   const Outside o(info, g, REST);
+  if (flat) {
+    for (int i = tid; i < V; i += kRowThreads) d[i] = (E)(o.f * o.flat(up<E>(z[i])));
+  } else {
 #pragma unroll
-  for (int q = 0; q < VPT; ++q) {
-    const int v = tid + q * kRowThreads;
-    stay_packed(x[q]);
-    if (v < nv) {
-      vec y;
+    for (int q = 0; q < VPT; ++q) {
+      const int v = tid + q * kRowThreads;
+      stay_packed(x[q]);
+      if (v < nv) {
+        vec y;
 #pragma unroll
-      for (int i = 0; i < N; ++i) y[i] = (E)(o.f * ex2(__builtin_fmaf(up<E>(x[q][i]), c, -o.base)));
-      put(d + (int64_t)v * N, y);
+        for (int i = 0; i < N; ++i) y[i] = (E)(o.f * o.power(up<E>(x[q][i]), c));
+        put(d + (int64_t)v * N, y);
+      }
     }
+    if (rem < V) d[rem] = (E)(o.f * o.power(last, c));
   }
-  if (rem < V) d[rem] = (E)(o.f * ex2(__builtin_fmaf(last, c, -o.base)));
   if (tid < 64) {
     const float loss = row_loss(a, n, info, [&](int k, int64_t) { return xk[k]; });
     if (tid == 0) {
@@ -539,7 +606,7 @@ row_kernel(DistillArgs a) {
   __syncthreads();
   const float nan = info.teacher.s != info.teacher.s ? info.teacher.s : 0.f;
   for (int k = tid; k < a.K; k += kRowThreads)
-    if (at[k] >= 0) d[at[k]] = (E)(g * (info.all.part(xk[k], c) - pj[k]) + nan);
+    if (at[k] >= 0) d[at[k]] = (E)(g * (info.all.part(floored(xk[k], low), c) - pj[k]) + nan);
 }
 
 // dz *= *factor, in place; nothing to do where that is 1
@@ -577,6 +644,8 @@ __global__ void __launch_bounds__(NT) grad_kernel(DistillArgs a) {
   const float c = kLog2e / a.temperature;
   const RowInfo info = load_info(a, n);
   const bool counts = !(info.r < 0.f);
+  const float low = floor_of(c);
+  const bool flat = counts && is_floored(info.all, low, c);
   float g = a.upstream[a.upstream_rows ? n : 0] * a.temperature;
   g *= a.mean != nullptr ? a.mean[0] : a.weight;
   const Outside o(info, g, REST);
@@ -584,10 +653,12 @@ __global__ void __launch_bounds__(NT) grad_kernel(DistillArgs a) {
     for (int k = tid; k < a.K; k += NT) {
       const int64_t j = index_at(a, n * a.K + k);
       at[k] = j >= c0 && j < c1 ? (int)(j - c0) : -1;
-      pk[k] = info.teacher.part(a.teacher[n * a.K + k], c);
+      pk[k] = info.teacher.part(floored(a.teacher[n * a.K + k], low), c);
     }
   }
-  const int64_t nv = (c1 - c0) / N;
+  const int64_t nv = flat ? 0 : (c1 - c0) / N;
+  if (flat)
+    for (int64_t i = c0 + tid; i < c1; i += NT) d[i] = (E)(o.f * o.flat(up<E>(z[i])));
   for (int64_t v0 = tid; v0 < nv; v0 += (int64_t)NT * U) {
     float y[U][N];
 #pragma unroll
@@ -600,14 +671,13 @@ __global__ void __launch_bounds__(NT) grad_kernel(DistillArgs a) {
       const int64_t v = v0 + (int64_t)q * NT;
       if (v < nv) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) y[q][i] = counts ? o.f * ex2(__builtin_fmaf(y[q][i], c, -o.base)) : 0.f;
+        for (int i = 0; i < N; ++i) y[q][i] = counts ? o.f * o.power(y[q][i], c) : 0.f;
         store_wide<E, ALIGNED_D>(d + c0 + v * N, y[q]);
       }
     }
   }
   const int64_t rem = c0 + nv * N + tid;
-  if (rem < c1)
-    d[rem] = (E)(counts ? o.f * ex2(__builtin_fmaf(up<E>(z[rem]), c, -o.base)) : 0.f);
+  if (rem < c1 && !flat) d[rem] = (E)(counts ? o.f * o.power(up<E>(z[rem]), c) : 0.f);
   if (!counts) return;
   __syncthreads();
   for (int k = tid; k < a.K; k += NT) {
@@ -615,7 +685,7 @@ __global__ void __launch_bounds__(NT) grad_kernel(DistillArgs a) {
     if (j < 0) continue;
     float p = 0.f;  // an index given twice counts with both its parts
     for (int i = 0; i < a.K; ++i) p += at[i] == j ? pk[i] : 0.f;
-    d[c0 + j] = (E)(g * (info.all.part(up<E>(z[c0 + j]), c) - p));
+    d[c0 + j] = (E)(g * (info.all.part(floored(up<E>(z[c0 + j]), low), c) - p));
   }
 }
 

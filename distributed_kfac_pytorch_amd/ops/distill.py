@@ -86,7 +86,9 @@ def topk_distill_loss(
     which ``K`` entries a row are known.
 
     Args:
-        logits: bf16, fp16 or fp32, any strides with a unit last one.
+        logits: bf16, fp16 or fp32, any strides with a unit last one.  Columns
+            masked with -inf or the type's lowest value have no probability;
+            a row of nothing but the lowest value is uniform over its columns.
         teacher_logits: ``[..., K]``, the teacher's logits of the entries
             (not divided by the temperature), 1 <= K <= 1024; constant.
         teacher_index: int32 or int64 ``[..., K]``, their columns.  A negative

@@ -10,6 +10,7 @@ from distributed_kfac_pytorch_amd.ops.attention import window_attention
 from distributed_kfac_pytorch_amd.ops.distill import topk_distill_loss
 from distributed_kfac_pytorch_amd.ops.rotary import rotary_axes
 from tests import lm_reference as ref
+from tests.test_lm_ops import lowest_case
 
 pytestmark = pytest.mark.gpu
 
@@ -688,6 +689,27 @@ def test_distill_bad_rows_stay_alone(cuda):
     (g,) = torch.autograd.grad(loss, z3, torch.ones_like(loss))
     assert bool(g[keep].isfinite().all())
     assert bool((g[keep][:, :100] == 0).all())
+
+
+@pytest.mark.parametrize('dtype', sorted(DTYPES))
+@pytest.mark.parametrize('rest', [False, True])
+@pytest.mark.parametrize('tau', [0.5, 1.0, 3.0])
+@pytest.mark.parametrize('stored', [False, True])
+def test_distill_lowest_values(cuda, stored, tau, rest, dtype):
+    z, t, i, r, want = lowest_case(DTYPES[dtype], tau, rest)
+    copies = 60 if stored else 1                  # 300 rows: the forward writes the gradient
+    zz, tt, ii = (x.repeat(copies, 1).to(cuda) for x in (z, t, i))
+    rr = r.repeat(copies).to(cuda) if rest else None
+    zz.requires_grad_()
+    conf = dict(teacher_rest=rr, temperature=tau)
+    loss = topk_distill_loss(zz, tt, ii, reduction='none', **conf)
+    ref.check('loss', loss, want[0].repeat(copies), want[1].repeat(copies))
+    total = loss.sum() if not stored else topk_distill_loss(zz, tt, ii, reduction='sum', **conf)
+    if stored:
+        bound = want[1].sum() * copies + 2.0 ** -24 * want[0].sum().abs() * copies
+        ref.check('sum', total, want[0].sum() * copies, bound)
+    (g,) = torch.autograd.grad(total, zz)
+    ref.check('dz', g, want[2].repeat(copies, 1), want[3].repeat(copies, 1))
 
 
 @pytest.mark.parametrize('dtype', sorted(DTYPES))
