@@ -814,6 +814,39 @@ def test_chain_in_two_graphs(cuda):
             assert all(torch.equal(a, b) for a, b in zip(kept, eager)), (rep, n)
 
 
+def test_fp16_attention_in_a_graph_beside_eager_passes(cuda):
+    """Forward and backward captured once, replayed with upstream gradients of
+    very different sizes and eager passes in between."""
+    q, k, v, do = (rand(cuda, 2, h, 600, 64, seed=s).half() for s, h in enumerate((4, 2, 2, 4)))
+    ln = torch.tensor([600, 333], dtype=torch.int32, device=cuda)
+    x = [t.requires_grad_() for t in (q, k, v)]
+
+    def call():
+        out = window_attention(*x, window=90, sinks=3, lengths=ln, q_start=0)
+        return [out, *torch.autograd.grad(out, x, do)]
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        call()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept = call()
+    for seed, size in ((5, 1.0), (6, 2.0 ** -12), (7, 2.0 ** 11), (8, 1.0)):
+        with torch.no_grad():
+            do.copy_(rand(cuda, 2, 4, 600, 64, seed=seed).half() * size)
+            q.copy_(rand(cuda, 2, 4, 600, 64, seed=seed + 10).half())
+            ln[1] = 100 * (seed - 4)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in kept]
+        for a, b in zip(got, call()):
+            assert torch.equal(a, b), seed
+            assert bool(a.isfinite().all()), seed
+
+
 def test_offsets_behind_32_bits(cuda):
     """Operands of more than 2^31 elements: what lies at their end is what a
     small call on a copy of it gives, bit for bit."""
