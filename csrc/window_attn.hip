@@ -253,6 +253,16 @@ __device__ __forceinline__ typename Ops<T>::frag acc_frag(const v16f& a, int s) 
   return __builtin_convertvector(f, typename Ops<T>::frag);
 }
 
+// what that rounding took away, rounded itself
+template <typename T>
+__device__ __forceinline__ typename Ops<T>::frag acc_rest(const v16f& a, int s,
+                                                          typename Ops<T>::frag rounded) {
+  v8f f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = a[8 * s + i] - (float)rounded[i];
+  return __builtin_convertvector(f, typename Ops<T>::frag);
+}
+
 // 8 elements of a global row from element d on; zeros behind D (D % 8 == 0)
 // and where the row is not `ok`.  Those lanes read `there`, the tensor's
 // beginning: with a branch round the load, a row's loads would wait for each
@@ -863,7 +873,8 @@ __device__ __forceinline__ float score_factor(const AttnArgs& a) {
 // batch 49 us.  The fixed order of KeyGrad::rows64 costs the second wave of a
 // SIMD its registers here (57 us for the latter), four waves a SIMD with 128
 // registers are no faster (49).
-template <typename T, int DP, int NW>
+// FINE: see attn_keeps_rest.
+template <typename T, int DP, int NW, bool FINE>
 __global__ void __launch_bounds__(64 * NW, (kRowFit<T, DP>)) dq_kernel(AttnArgs a) {
   constexpr int KD = DP / 16, ND = DP / 32;
   typedef typename Ops<T>::frag frag;
@@ -888,7 +899,7 @@ __global__ void __launch_bounds__(64 * NW, (kRowFit<T, DP>)) dq_kernel(AttnArgs 
 #pragma unroll
     for (int i = 0; i < 8; ++i) delta += (float)gf[k][i] * (float)of[i];
   }
-  if (sizeof(T) == 2 && a.rest != nullptr) {
+  if (FINE) {
 #pragma unroll
     for (int k = 0; k < KD; ++k) {
       const frag rf = global_frag<T>(a.rest, rest, k * 16 + 8 * h, a.D, w.p >= 0);
@@ -948,9 +959,14 @@ __global__ void __launch_bounds__(64 * NW, (kRowFit<T, DP>)) dq_kernel(AttnArgs 
 #pragma unroll
       for (int ss = 0; ss < 2; ++ss) {
         const frag sf = acc_frag<T>(s, ss);
+        frag rest;
+        if constexpr (FINE) rest = acc_rest<T>(s, ss, sf);
 #pragma unroll
-        for (int d = 0; d < ND; ++d)
-          dq[d] = Ops<T>::mma(col_frag<T, DP>(K, at, sub * 32 + ss * 16, d * 32), sf, dq[d]);
+        for (int d = 0; d < ND; ++d) {
+          const frag kf = col_frag<T, DP>(K, at, sub * 32 + ss * 16, d * 32);
+          dq[d] = Ops<T>::mma(kf, sf, dq[d]);
+          if constexpr (FINE) dq[d] = Ops<T>::mma(kf, rest, dq[d]);
+        }
       }
     }
   });
@@ -1057,7 +1073,7 @@ struct RowStream {
 // dk and dv: a wave owns 32 keys.  S = Q K^T and dP = dO V^T have a row's
 // scores in register order, so dV^T += dO^T P and dK^T += Q^T dS take P and
 // dS from where they are.
-template <typename T, int DP>
+template <typename T, int DP, bool FINE>
 struct KeyGrad {
   static constexpr int KD = DP / 16, ND = DP / 32;
   typedef typename Ops<T>::frag frag;
@@ -1227,10 +1243,14 @@ struct KeyGrad {
 #pragma unroll
     for (int ss = 0; ss < 2; ++ss) {
       const frag pf = acc_frag<T>(s, ss), sf = acc_frag<T>(dp, ss);
+      frag rest;
+      if constexpr (FINE) rest = acc_rest<T>(dp, ss, sf);
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
         dv[d] = Ops<T>::mma(col_frag<T, DP>(b.g, at, i0 + ss * 16, d * 32), pf, dv[d]);
-        dk[d] = Ops<T>::mma(col_frag<T, DP>(b.q, at, i0 + ss * 16, d * 32), sf, dk[d]);
+        const frag qf = col_frag<T, DP>(b.q, at, i0 + ss * 16, d * 32);
+        dk[d] = Ops<T>::mma(qf, sf, dk[d]);
+        if constexpr (FINE) dk[d] = Ops<T>::mma(qf, rest, dk[d]);
       }
     }
   }
@@ -1245,7 +1265,7 @@ struct KeyGrad {
 // KG groups of 32 keys and, for each, RS waves that take every RS-th 32 rows
 // of a tile and add up at the end: where there are fewer waves than the chip
 // can hold, a key's rows are the time that is left to divide.
-template <typename T, int DP, int KG, int RS>
+template <typename T, int DP, int KG, int RS, bool FINE>
 __global__ void __launch_bounds__(64 * KG * RS, (kKeyFit<T, DP>))
 dkv_kernel(AttnArgs a, int key_blocks) {
   constexpr int ND = DP / 32, LD = kLd<T, DP>, NW = KG * RS, NT = 64 * NW, BM = 32 * KG;
@@ -1262,7 +1282,7 @@ dkv_kernel(AttnArgs a, int key_blocks) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Seq seq = sequence(a, b);
   const RowStream<T, DP, NW> rs(a, b, hk, wave);
-  KeyGrad<T, DP> kg;
+  KeyGrad<T, DP, FINE> kg;
 
   if ((int)blockIdx.y >= key_blocks) {
     const int item = (int)blockIdx.y - key_blocks;
@@ -1326,7 +1346,7 @@ dkv_kernel(AttnArgs a, int key_blocks) {
   kg.init(a, b, hk, key, kr);
   auto step = [&](const RowBuf<T>& buf, int t0) {
     kg.at.fresh();
-    if constexpr (RS == 1 && sizeof(T) == 2) {
+    if constexpr (RS == 1 && sizeof(T) == 2 && !FINE) {
       if (kr.coverage(t0) != 0 || kr.coverage(t0 + 32) != 0) kg.rows64(a, buf, t0, kr);
       return;
     }
@@ -1418,24 +1438,31 @@ void forward_dp(const AttnArgs& a, hipStream_t st) {
   }
 }
 
-template <typename T, int DP>
-void backward_dp(const AttnArgs& a, hipStream_t st) {
+template <typename T, int DP, bool FINE>
+void backward_fine(const AttnArgs& a, hipStream_t st) {
   constexpr int QN = kRowWaves, KG = kKeyWaves<DP>;
   const unsigned bh = (unsigned)(a.B * a.Hkv);
-  dq_kernel<T, DP, QN><<<dim3(bh, (unsigned)ceil_div((int64_t)a.Tq * a.G, 32 * QN)), 64 * QN, 0,
-                         st>>>(a);
+  dq_kernel<T, DP, QN, FINE><<<dim3(bh, (unsigned)ceil_div((int64_t)a.Tq * a.G, 32 * QN)), 64 * QN,
+                               0, st>>>(a);
   const int kb = (int)ceil_div(a.Tk, 32 * KG);
   const dim3 grid(bh, (unsigned)(kb + a.sink_groups * a.far_chunks));
   // up to one wave a SIMD: two share a group of keys (fp32 padded batch, 520
   // waves: 60 -> 44 us)
   if (KG == 2 && (int64_t)bh * kb * KG <= 1024)
-    dkv_kernel<T, DP, KG, KG == 2 ? 2 : 1><<<grid, 64 * KG * 2, 0, st>>>(a, kb);
+    dkv_kernel<T, DP, KG, KG == 2 ? 2 : 1, FINE><<<grid, 64 * KG * 2, 0, st>>>(a, kb);
   else
-    dkv_kernel<T, DP, KG, 1><<<grid, 64 * KG, 0, st>>>(a, kb);
+    dkv_kernel<T, DP, KG, 1, FINE><<<grid, 64 * KG, 0, st>>>(a, kb);
   if (a.far_chunks > 0) {
     const int64_t n = (int64_t)bh * a.S * 2 * (a.D / 4);
     join_kv_kernel<T><<<(unsigned)ceil_div(n, NT), NT, 0, st>>>(a);
   }
+}
+
+template <typename T, int DP>
+void backward_dp(const AttnArgs& a, hipStream_t st) {
+  if constexpr (sizeof(T) == 2)
+    if (a.rest != nullptr) return backward_fine<T, DP, true>(a, st);
+  backward_fine<T, DP, false>(a, st);
 }
 
 template <typename T>
@@ -1456,13 +1483,16 @@ void backward_type(const AttnArgs& a, hipStream_t st) {
 
 }  // namespace
 
-// dP - delta is small where few keys share the weight, and the rounding of o
-// then weighs in delta: with a window of 2 the gradients of q and k are off by
-// 0.0037 of their norm (bf16), and by 0.0024 when delta also counts what that
-// rounding took away, of which their own rounding is 0.0017; of 6 0.0027, of 30
-// 0.0025, 0.0024 with it.  The first rows of a short sequence see as few keys.
-// Writing and reading it costs a tenth of the pass
-// (GPT-NeoX batch, window 256: 171 us against 155).
+// dP - delta is small where few keys share the weight, and two roundings then
+// weigh in the gradients of q and k: that of o, which delta goes by, and that
+// of P (dP - delta) itself.  With a window of 2 and neither mended they are off
+// by 0.0037 of their norm (bf16), of 6 0.0027, of 30 0.0025; with delta counting
+// what o's rounding took away by 0.0025 at each, and with the product taken in
+// two parts (FINE: two matrix instructions for one, and no rows64) by 0.0018,
+// where their own rounding is 0.0017.  The first rows of a short sequence see
+// as few keys.  GPT-NeoX batch with window 100: 135 us without the two parts,
+// 142 with; 8192 tokens, heads of 128, window 100: 171, 194.  Over 128 keys
+// neither is done (0.0025; window 256, delta's part alone: 155 -> 171 us).
 bool attn_keeps_rest(const AttnArgs& a) { return std::min<int64_t>((int64_t)a.W + a.S, a.Tk) <= 128; }
 
 void attn_plan(const AttnArgs& a, int* splits, int64_t* floats) {

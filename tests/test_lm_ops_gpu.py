@@ -190,6 +190,46 @@ def test_fp16_rows_of_small_probabilities(cuda, tq, hq):
     assert float(err) <= 2.0 ** -10 + 2.0 ** -16, float(err)
 
 
+@pytest.mark.parametrize('dtype', ['bf16', 'fp16'])
+@pytest.mark.parametrize('d', [16, 64, 96, 128])
+@pytest.mark.parametrize('heads', [1, 30])
+def test_short_windows_round_their_gradients_once(cuda, heads, d, dtype):
+    """8 keys of probability 1/8 each (queries of 0, or keys of 0), so that
+    probabilities and outputs are exact in 32 bits: what is left of the
+    gradients' error is their own rounding, half a step, and terms of second
+    order: what o's rounding took away is itself rounded (u^2 of o, or half of
+    fp16's smallest step), and so is what the rounding of P (dP - delta) did."""
+    dt, n, rows, w = DTYPES[dtype], 263, 256, 8
+    u, tiny = ref.half(dt), ref.smallest(dt)
+    x, v = (rand(cuda, 1, heads, t, d, seed=s) for s, t in ((0, n), (1, n)))
+    do = rand(cuda, 1, heads, rows, d, seed=2, dtype=dt)
+    v, some = v.to(dt), (x + 16.0).to(dt)
+    for name in ('dq', 'dk'):
+        q = torch.zeros_like(do) if name == 'dq' else some[:, :, :rows].contiguous()
+        k = torch.zeros_like(some) if name == 'dk' else some
+        leaf = (q if name == 'dq' else k).requires_grad_()
+        (got,) = torch.autograd.grad(window_attention(q, k, v, window=w), leaf, do)
+        V, D, K, Q = (y.detach().cpu().double() for y in (v, do, k, q))
+        see = (torch.arange(n) >= torch.arange(rows)[:, None]) & (
+            torch.arange(n) < torch.arange(rows)[:, None] + w)
+        p = (see / w).double()
+        o = p @ V
+        dp, delta = D @ V.transpose(2, 3), (D * o).sum(-1, keepdim=True)
+        ds = p * (dp - delta)
+        size = D.abs() @ V.abs().transpose(2, 3) + (D.abs() * o.abs()).sum(-1, keepdim=True)
+        e = p * ((D.abs() * (u * u * o.abs() + tiny)).sum(-1, keepdim=True)
+                 + 2.0 ** -24 * 4 * (d + 16) * size) + u * u * ds.abs()
+        f = d ** -0.5
+        if name == 'dq':
+            want, off = f * ds @ K, f * (e + 2.0 ** -20 * ds.abs()) @ K.abs()
+        else:
+            want = f * ds.transpose(2, 3) @ Q
+            off = f * (e + 2.0 ** -20 * ds.abs()).transpose(2, 3) @ Q.abs()
+        # half a step of a number of this size (frexp: below 2^exponent)
+        half_step = u * torch.ldexp(torch.ones(()).double(), torch.frexp(want.abs() + off)[1] - 1)
+        ref.check(name, got, want, off + torch.maximum(half_step, torch.tensor(tiny).double()))
+
+
 def _signs(dev, n, d):
     """[1, 1, n, d] of rows +1, -1, +1, .."""
     x = torch.where(torch.arange(n, device=dev) % 2 == 0, 1.0, -1.0).half()
