@@ -24,7 +24,7 @@
 // loss afterwards is multiplied into the gradient in place by the backward
 // pass, which costs a read and a write more and, where it is no power of
 // two, a second rounding.  16384 rows of 50304 bf16 logits: 0.67 ms for loss
-// and gradient, 4.96 TB/s, a copy's rate.  The other calls (fp16, whose range does not hold
+// and gradient, 4.9 TB/s, a copy's rate.  The other calls (fp16, whose range does not hold
 // the unscaled gradient of a mean over thousands of rows; few rows, each cut
 // into slices; reduction 'none'; more columns) read the logits once forward
 // and once more backward.

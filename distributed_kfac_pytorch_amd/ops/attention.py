@@ -9,8 +9,10 @@ outside its sequence (``p < 0`` or ``p >= lengths[b]``) is padding: its output
 is zero and nothing flows back through it.
 
 GPU tensors run the native kernels (scores are never written to memory;
-scores, softmax statistics and sums in 32 bits, probabilities rounded to the
-inputs' dtype for the second product), CPU tensors the same formula in torch.
+scores, softmax statistics and sums in 32 bits, probabilities and score
+gradients rounded to the inputs' dtype for the products that follow, in fp16 at
+a power of two that keeps them clear of its subnormals and its end), CPU
+tensors the same formula in torch.
 The backward pass sums in a fixed order: no atomics, bit-reproducible.
 """
 from __future__ import annotations
@@ -87,8 +89,9 @@ def window_attention(
     Returns:
         ``[B, Hq, Tq, D]`` over memory laid out ``[B, Tq, Hq, D]``, which
         ``transpose(1, 2).flatten(2)`` reads without a copy.  Gradients flow
-        to ``q``, ``k`` and ``v``.  Infinities and NaN inside a sequence may
-        reach other rows of it.
+        to ``q``, ``k`` and ``v``.  Rows of padding and keys that no row sees
+        may hold anything; infinities and NaN in what is seen may reach other
+        rows of their sequence and head.
     """
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
         raise ValueError(f'q must be [B, Hq, Tq, D], k and v [B, Hk, Tk, D], got '
