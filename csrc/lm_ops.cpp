@@ -185,7 +185,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attn_forward(const at::Tensor& q,
                                                             const AttnConf& c, bool training) {
   c10::hip::HIPGuardMasqueradingAsCUDA g(q.device());
   kfac::AttnArgs a = attn_args(q, k, v, lengths, starts, c);
-  at::Tensor out = at::empty({a.B, a.Tq, a.Hq, a.D}, q.options()).transpose(1, 2);
+  // no transposed view of a buffer: in-place operations on a view that was made
+  // without recording are refused later
+  const int64_t row = (int64_t)a.Hq * a.D;
+  at::Tensor out =
+      at::empty_strided({a.B, a.Hq, a.Tq, a.D}, {a.Tq * row, a.D, row, 1}, q.options());
   at::Tensor lse, rest;
   if (training) {
     lse = at::empty({a.B * a.Hkv, (int64_t)a.Tq * a.G}, q.options().dtype(at::kFloat));
@@ -452,16 +456,18 @@ struct DistillOut {
   at::Tensor loss, info, mean, dz;
 };
 
-// reduction: 0 none, 1 sum, 2 mean; grad: a backward pass will follow
+// reduction: 0 none (of the shape `lead`), 1 sum, 2 mean; grad: a backward pass
+// will follow
 DistillOut distill_run(const at::Tensor& z, const at::Tensor& teacher, const at::Tensor& index,
                        const OptTensor& rest, double temperature, double weight,
-                       int64_t reduction, bool grad) {
+                       int64_t reduction, const std::vector<int64_t>& lead, bool grad) {
   c10::hip::HIPGuardMasqueradingAsCUDA g(z.device());
   kfac::DistillArgs a = distill_args(z, teacher, index, rest, temperature, weight);
   const auto f32 = z.options().dtype(at::kFloat);
   DistillOut o;
   o.info = at::empty({a.N, 8}, f32);
-  at::Tensor rows = at::empty({a.N}, f32);
+  at::Tensor rows = at::empty(lead, f32);
+  TORCH_CHECK(rows.numel() == a.N, "topk_distill_loss: rows");
   a.info = reinterpret_cast<float4*>(o.info.data_ptr<float>());
   a.row_loss = rows.data_ptr<float>();
   o.loss = rows;
@@ -494,8 +500,8 @@ DistillOut distill_run(const at::Tensor& z, const at::Tensor& teacher, const at:
 struct DistillFn : public torch::autograd::Function<DistillFn> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& z, const at::Tensor& teacher,
                             const at::Tensor& index, const OptTensor& rest, double temperature,
-                            double weight, int64_t reduction) {
-    auto o = distill_run(z, teacher, index, rest, temperature, weight, reduction, true);
+                            double weight, int64_t reduction, const std::vector<int64_t>& lead) {
+    auto o = distill_run(z, teacher, index, rest, temperature, weight, reduction, lead, true);
     // the gradient as well: saved-tensor hooks (offloading, checkpoints) see it
     ctx->save_for_backward({z, teacher, index, rest.has_value() ? *rest : at::Tensor(), o.info,
                             o.mean, o.dz});
@@ -526,7 +532,7 @@ struct DistillFn : public torch::autograd::Function<DistillFn> {
       if (dz.numel() > 0)
         kfac::distill_scale(tag(z), dz.data_ptr(), dz.numel(), up.data_ptr<float>(), stream());
       C10_HIP_KERNEL_LAUNCH_CHECK();
-      return {dz, u, u, u, u, u, u};
+      return {dz, u, u, u, u, u, u, u};
     }
     const OptTensor rest = sv[3].defined() ? OptTensor(sv[3].contiguous()) : c10::nullopt;
     const at::Tensor teacher = sv[1].contiguous(), index = sv[2].contiguous();
@@ -545,17 +551,17 @@ struct DistillFn : public torch::autograd::Function<DistillFn> {
     a.dz_aligned = rows16(dz);
     kfac::distill_backward(tag(z), a, stream());
     C10_HIP_KERNEL_LAUNCH_CHECK();
-    return {dz, u, u, u, u, u, u};
+    return {dz, u, u, u, u, u, u, u};
   }
 };
 
 at::Tensor topk_distill_loss(const at::Tensor& z, const at::Tensor& teacher,
                              const at::Tensor& index, const OptTensor& rest, double temperature,
-                             double weight, int64_t reduction) {
+                             double weight, int64_t reduction, const std::vector<int64_t>& lead) {
   reverse_only("topk_distill_loss", {&z});
   if (records({&z}))
-    return DistillFn::apply(z, teacher, index, rest, temperature, weight, reduction);
-  return distill_run(z, teacher, index, rest, temperature, weight, reduction, false).loss;
+    return DistillFn::apply(z, teacher, index, rest, temperature, weight, reduction, lead);
+  return distill_run(z, teacher, index, rest, temperature, weight, reduction, lead, false).loss;
 }
 
 }  // namespace
@@ -569,5 +575,5 @@ void bind_lm_ops(pybind11::module& m) {
         py::arg("table"), py::arg("halves"));
   m.def("topk_distill_loss", &topk_distill_loss, py::arg("logits"), py::arg("teacher"),
         py::arg("index"), py::arg("rest"), py::arg("temperature"),
-        py::arg("weight"), py::arg("reduction"));
+        py::arg("weight"), py::arg("reduction"), py::arg("lead"));
 }

@@ -53,7 +53,9 @@ def _reference(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, s
         e = torch.exp(s - m.masked_fill(m == float('-inf'), 0.0))
         total = e.sum(dim=-1, keepdim=True)
         o = torch.where(rows, (e / total.masked_fill(total == 0.0, 1.0)) @ vv, 0.0)
-    return o.to(q.dtype).transpose(1, 2).contiguous().transpose(1, 2)
+    b, h, t, d = o.shape
+    return torch.empty_strided((b, h, t, d), (t * h * d, d, h * d, 1), dtype=q.dtype,
+                               device=q.device).copy_(o)
 
 
 def window_attention(

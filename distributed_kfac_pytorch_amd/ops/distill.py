@@ -152,8 +152,7 @@ def topk_distill_loss(
         z = z[(None,) * (3 - z.dim())]
     elif z.dim() > 3:
         z = z.flatten(0, -3)
-    loss = _nat.native().topk_distill_loss(  # type: ignore[union-attr]
+    return _nat.native().topk_distill_loss(  # type: ignore[union-attr]
         z, teacher_logits.float().contiguous(), teacher_index.contiguous(),
         None if rest is None else rest.float().contiguous(), temperature,
-        weight, _REDUCTIONS.index(reduction))
-    return loss.view(lead) if reduction == 'none' else loss
+        weight, _REDUCTIONS.index(reduction), lead)

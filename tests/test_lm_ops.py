@@ -144,7 +144,7 @@ def test_the_kernels_refuse_tangents():
         if lib is not None:
             for call in (lambda: lib.window_attention(q, q, dq, None, None, 2, 0, 0, False, 1.0),
                          lambda: lib.rotary_axes(dq, q, pos, table, False),
-                         lambda: lib.topk_distill_loss(dz, t, i, None, 1.0, 1.0, 2)):
+                         lambda: lib.topk_distill_loss(dz, t, i, None, 1.0, 1.0, 2, [1, 2])):
                 with pytest.raises(RuntimeError, match='forward-mode'):
                     call()
         for out in (window_attention(q, q, dq, window=2), rotary_axes(dq, q, pos, sections=(4,))[0],
@@ -226,6 +226,18 @@ def test_autocast_changes_nothing():
         assert torch.equal(a, b)
     q = torch.empty(1, 2, 4, 8, device='meta')        # a device without autocast
     assert window_attention(q, q, q, window=2).shape == q.shape
+
+
+def test_attention_output_is_a_tensor_of_its_own():
+    """[B, T, H, D] in memory and no view: in-place operations on what a frozen
+    part gave are allowed."""
+    q = rand(2, 4, 6, 8)
+    with torch.no_grad():
+        out = window_attention(q, q, q, window=3)
+    assert out.transpose(1, 2).is_contiguous() and out._base is None
+    adapter = torch.ones_like(out).requires_grad_()
+    out += adapter
+    assert bool((torch.autograd.grad(out.sum(), adapter)[0] == 1).all())
 
 
 def test_attention_differences():

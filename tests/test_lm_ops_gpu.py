@@ -1011,6 +1011,51 @@ def test_forward_mode_is_refused(cuda):
                 call()
 
 
+def test_results_are_tensors_of_their_own(cuda):
+    """In-place operations on what a frozen part gave, as on the CPU: the
+    attention's output is no view of a buffer that autograd knows."""
+    q, z = rand(cuda, 2, 4, 6, 16), rand(cuda, 5, 9)
+    pos = torch.arange(6, device=cuda)[:, None]
+    t, i, _ = _teacher(cuda, 5, 9, 2, 1.0, False, 1)
+    with torch.no_grad():
+        outs = [window_attention(q, q, q, window=3), *rotary_axes(q, q, pos, sections=(8,)),
+                topk_distill_loss(z, t, i, reduction='none')]
+    for out in outs:
+        adapter = torch.full_like(out, 2.0).requires_grad_()
+        want = out + adapter.detach()
+        out += adapter
+        assert torch.equal(out, want)
+        (g,) = torch.autograd.grad(out.sum(), adapter)
+        assert bool((g == 1).all())
+
+
+@pytest.mark.parametrize('dtype', sorted(DTYPES))
+def test_nothing_at_all(cuda, dtype):
+    dt = DTYPES[dtype]
+    for shapes in (((0, 4, 5, 16), (0, 2, 7, 16)), ((2, 4, 0, 16), (2, 2, 7, 16)),
+                   ((2, 4, 5, 16), (2, 2, 0, 16)), ((2, 0, 5, 16), (2, 2, 7, 16))):
+        q, k, v = (rand(cuda, *s, dtype=dt).requires_grad_() for s in (*shapes, shapes[1]))
+        out = window_attention(q, k, v, window=3, sinks=1)
+        assert out.shape == q.shape and not bool(out.any())
+        for x, g in zip((q, k, v), torch.autograd.grad(out, (q, k, v), torch.ones_like(out))):
+            assert g.shape == x.shape and not bool(g.any())
+    for lead in ((0,), (2, 0), (0, 3), (3, 0, 2)):
+        z = rand(cuda, *lead, 11, dtype=dt).requires_grad_()
+        t, i = rand(cuda, *lead, 3), torch.zeros(*lead, 3, dtype=torch.int64, device=cuda)
+        for reduction in ('none', 'sum', 'mean'):
+            loss = topk_distill_loss(z, t, i, teacher_rest=rand(cuda, *lead), reduction=reduction)
+            assert loss.shape == (lead if reduction == 'none' else ()) and not bool(loss.any())
+            (g,) = torch.autograd.grad(loss.sum(), z)
+            assert g.shape == z.shape
+    pos = torch.zeros(5, 1, dtype=torch.int64, device=cuda)
+    q, k = rand(cuda, 0, 2, 5, 16, dtype=dt), rand(cuda, 0, 1, 5, 16, dtype=dt)
+    assert [x.shape for x in rotary_axes(q, k, pos, sections=(8,))] == [q.shape, k.shape]
+    q, k = (rand(cuda, 2, h, 5, 16, dtype=dt).requires_grad_() for h in (0, 1))
+    out = rotary_axes(q, k, pos, sections=(8,))
+    assert torch.equal(out[1], k)
+    assert torch.equal(torch.autograd.grad(out[1].sum(), k)[0], torch.ones_like(k))
+
+
 def test_one_operand_learns(cuda):
     q, k, v = (rand(cuda, 1, 2, 40, 16, seed=s) for s in range(3))
     do = rand(cuda, 1, 2, 40, 16, seed=5)
