@@ -391,10 +391,13 @@ struct RotaryFn : public torch::autograd::Function<RotaryFn> {
     once_only("rotary_axes");
     const auto kept = ctx->saved_data.begin();
     const RotaryConf c{kept->second.toTensor(), kept->first == "halves"};
-    auto [dq, dk] = rotary_run(unit_last(grads[0]), unit_last(grads[1]),
-                               ctx->get_saved_variables()[0], c, -1.0);
+    // no heads of an operand that needs no gradient
+    const bool need[2] = {ctx->needs_input_grad(0), ctx->needs_input_grad(1)};
+    for (int i = 0; i < 2; ++i)
+      grads[i] = need[i] ? unit_last(grads[i]) : grads[i].narrow(1, 0, 0);
+    auto [dq, dk] = rotary_run(grads[0], grads[1], ctx->get_saved_variables()[0], c, -1.0);
     at::Tensor u;
-    return {dq, dk, u, u, u};
+    return {need[0] ? dq : u, need[1] ? dk : u, u, u, u};
   }
 };
 

@@ -1011,6 +1011,18 @@ def test_forward_mode_is_refused(cuda):
                 call()
 
 
+@pytest.mark.parametrize('layout', ['interleaved', 'halves'])
+@pytest.mark.parametrize('learns', [0, 1])
+def test_rotary_turns_what_needs_a_gradient(cuda, learns, layout):
+    x = [rand(cuda, 2, h, 7, 32, seed=h) for h in (3, 2)]
+    do = [rand(cuda, 2, h, 7, 32, seed=h + 5) for h in (3, 2)]
+    pos = torch.arange(7, device=cuda)[:, None]
+    x[learns].requires_grad_()
+    out = rotary_axes(*x, pos, sections=(16,), layout=layout)
+    (g,) = torch.autograd.grad(out, x[learns], do)
+    ref.check('dx', g, *ref.rotary(do[learns], pos, sections=(16,), layout=layout, sign=-1.0))
+
+
 def test_results_are_tensors_of_their_own(cuda):
     """In-place operations on what a frozen part gave, as on the CPU: the
     attention's output is no view of a buffer that autograd knows."""
